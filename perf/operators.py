@@ -1,0 +1,235 @@
+"""The 8-bit operators of the scene MLP's layers, as a user's program calls them, and their plain forms.
+
+Three operators (nicecore.lowbit):
+
+  rows     quantize_rows(x), then its dequantize(): every row of x as signed 8-bit codes with one
+           32-bit scale, s = amax / 127, q = the integer nearest to x / s (ties to even).
+  product  quantized_linear(x, W8, bias): x's rows quantised as above, multiplied with a weight that
+           is held in 8 bits with a scale for each output channel, y = (q . w) s_x s_w + b [, ReLU].
+  layer    checkpointed_linear(x, W, b, relu): one training step of a layer, y = a W^T + b with
+           a = x or ReLU(x), whose backward pass has only an 8-bit checkpoint of a: codes with one
+           power of two for each 32 neighbouring channels.
+               dx = (dy W) . [x > 0],  dW = dy^T a8,  db = sum of dy's rows
+           a8 = the checkpoint's values: k 2^e with 2^e the least power of two for which 127 2^e (254 2^e where
+           a is a ReLU's output, which needs no sign) holds the group's largest magnitude, k the
+           nearest integer (ties to even).
+
+A case: op, tokens (rows), inputs (K), outputs (N), type of x and of the result, relu.
+"""
+import math
+
+import torch
+
+own = False
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+SIZE = {"f32": 4, "bf16": 2, "f16": 2}
+
+
+def listed():
+    return [
+        # what a mapper keeps of one tracker batch: 200 pixels' hidden units
+        {"name": "rows 200x256 f32", "op": "rows", "tokens": 200, "inputs": 256, "outputs": 0, "type": "f32", "relu": False},
+        # a long batch of wide tokens, bound by memory
+        {"name": "rows 16384x4096 bf16", "op": "rows", "tokens": 16384, "inputs": 4096, "outputs": 0, "type": "bf16", "relu": False},
+        # one point through one hidden layer: latency alone
+        {"name": "product 1x256x256 f32", "op": "product", "tokens": 1, "inputs": 256, "outputs": 256, "type": "f32", "relu": True},
+        # one token against a large weight: the weight's bytes
+        {"name": "product 1x8192x8192 bf16", "op": "product", "tokens": 1, "inputs": 8192, "outputs": 8192, "type": "bf16", "relu": False},
+        # a few requests served together
+        {"name": "product 32x4096x4096 bf16", "op": "product", "tokens": 32, "inputs": 4096, "outputs": 4096, "type": "bf16", "relu": False},
+        # odd everywhere: the Fourier features' width, rows that fill no tile
+        {"name": "product 777x93x1001 f16", "op": "product", "tokens": 777, "inputs": 93, "outputs": 1001, "type": "f16", "relu": True},
+        # a long prompt: bound by the matrix cores
+        {"name": "product 16384x4096x4096 bf16", "op": "product", "tokens": 16384, "inputs": 4096, "outputs": 4096, "type": "bf16", "relu": False},
+        # the first layer of the scene MLP on a tracker batch
+        {"name": "layer 200x93x256 f32", "op": "layer", "tokens": 200, "inputs": 93, "outputs": 256, "type": "f32", "relu": False},
+        # a hidden layer of the scene MLP on a mapper iteration: 5,000 rays of 44 samples
+        {"name": "layer 220000x256x256 f32", "op": "layer", "tokens": 220000, "inputs": 256, "outputs": 256, "type": "f32", "relu": True},
+        # a wide layer in 32 bits
+        {"name": "layer 2048x1024x4096 f32", "op": "layer", "tokens": 2048, "inputs": 1024, "outputs": 4096, "type": "f32", "relu": True},
+        # odd everywhere, 16 bits
+        {"name": "layer 1237x517x1031 f16", "op": "layer", "tokens": 1237, "inputs": 517, "outputs": 1031, "type": "f16", "relu": True},
+        # a training batch of wide tokens: the largest
+        {"name": "layer 8192x4096x4096 bf16", "op": "layer", "tokens": 8192, "inputs": 4096, "outputs": 4096, "type": "bf16", "relu": True},
+    ]
+
+
+def _size(rng, low, high):
+    """Spread over the logarithm; one in three a multiple of 64, the others as they fall."""
+    n = int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+    if rng.random() < 1 / 3:
+        n = max(64, (n + 32) // 64 * 64)
+    return min(max(n, low), high)
+
+
+def draw(rng):
+    op = rng.choice(("rows", "product", "product", "layer", "layer"))
+    kind = rng.choice(("f32", "bf16", "f16"))
+    while True:
+        m = _size(rng, 1, 220000)
+        k = _size(rng, 32, 8192)
+        n = 0 if op == "rows" else _size(rng, 32, 8192)
+        passes = {"rows": 1, "product": 1, "layer": 3}[op]
+        if m * max(k, n) <= 16384 * 4096 and m * k * max(n, 1) * passes <= 3 * 8192 * 4096 * 4096:
+            break
+    return {"op": op, "tokens": m, "inputs": k, "outputs": n, "type": kind, "relu": op != "rows" and rng.random() < 0.5}
+
+
+def _inputs(gen, m, k, kind):
+    """Activations as layers see them: channels of unlike size and a few large values."""
+    x = torch.randn(m, k, generator=gen, device="cuda")
+    x = x * torch.exp(0.5 * torch.randn(k, generator=gen, device="cuda"))
+    x = torch.where(torch.rand(m, k, generator=gen, device="cuda") < 1e-3, 8 * x, x)
+    return x.to(TYPES[kind])
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    m, k, n, kind = case["tokens"], case["inputs"], case["outputs"], case["type"]
+    state = {"op": case["op"], "relu": case["relu"], "x": _inputs(gen, m, k, kind)}
+    if case["op"] == "rows":
+        return state
+    w = torch.randn(n, k, generator=gen, device="cuda") / math.sqrt(k)
+    state["b"] = (0.1 * torch.randn(n, generator=gen, device="cuda")).to(TYPES[kind])
+    if case["op"] == "product":
+        if own:
+            from nicecore import lowbit
+            state["w"] = lowbit.quantize_rows(w)
+        else:
+            state["w"] = _rows(w)
+        return state
+    state["w"] = w.to(TYPES[kind])
+    state["dy"] = (1e-2 * torch.randn(m, n, generator=gen, device="cuda")).to(TYPES[kind])
+    for leaf in ("x", "w", "b"):
+        state[leaf].requires_grad_(True)
+    return state
+
+
+# ---- the plain forms: 32 bits, rounded once at the end ------------------------------------------
+
+def _rows(x):
+    """(codes as int8, scales): the quotient in 64 bits, since one next to a half decides a code."""
+    s = (x.float().abs().amax(1) / 127).clamp_min(2.0 ** -126)
+    q = torch.round(x.double() / s.double()[:, None])
+    return q.clamp_(-127, 127).to(torch.int8), s
+
+
+def _checkpoint(a, unsigned):
+    """The values that the 8-bit checkpoint of a [m, k] (float32) stands for."""
+    m, k = a.shape
+    g = torch.zeros(m, (k + 31) // 32 * 32, device=a.device)
+    g[:, :k] = a
+    g = g.view(m, -1, 32)
+    top = g.abs().amax(2, keepdim=True)
+    # the biased exponent of the least power of two 2^(E - 127) with 127/64 2^(E - 127) >= top
+    e = (top.view(torch.int32) + 0x1FFFF) >> 23
+    step = (e - (7 if unsigned else 6)).clamp_min(1)
+    step = (step << 23).view(torch.float32)
+    v = torch.round(g / step).clamp_(-127, 254 if unsigned else 127) * step
+    return v.reshape(m, -1)[:, :k]
+
+
+def _over_tokens(u, v):
+    """u^T v, a sum over rows; a long one in slices, whose sums are added, as one of 32 bits would lose digits."""
+    m = u.shape[0]
+    if m <= 16384:
+        return u.t() @ v
+    u, v = (torch.nn.functional.pad(t, (0, 0, 0, -m % 4096)).view(-1, 4096, t.shape[1]) for t in (u, v))
+    return torch.bmm(u.transpose(1, 2), v).sum(0)
+
+
+def _plain(state):
+    x = state["x"].detach()
+    kind = x.dtype
+    if state["op"] == "rows":
+        q, s = _rows(x)
+        return {"values": (q.float() * s[:, None]).to(kind), "scales": s}
+    b = state["b"].detach().float()
+    if state["op"] == "product":
+        q, s = _rows(x)
+        wq, ws = state["w"]
+        y = (q.float() @ wq.float().t()) * s[:, None] * ws + b
+        return (y.clamp_min(0) if state["relu"] else y).to(kind)
+    w, dy, x = state["w"].detach().float(), state["dy"].float(), x.float()
+    a = x.clamp_min(0) if state["relu"] else x
+    y = a @ w.t() + b
+    a8 = _checkpoint(a, state["relu"])
+    dx = dy @ w
+    if state["relu"]:
+        dx = dx * (x > 0)
+    return {"y": y.to(kind), "dx": dx.to(kind), "dw": _over_tokens(dy, a8).to(kind), "db": dy.sum(0).to(kind)}
+
+
+def run(state):
+    if not own:
+        with torch.no_grad():
+            return _plain(state)
+    from nicecore import lowbit
+    if state["op"] == "rows":
+        q = lowbit.quantize_rows(state["x"])
+        return {"values": q.dequantize(), "scales": q.scales}
+    if state["op"] == "product":
+        return lowbit.quantized_linear(state["x"], state["w"], state["b"], relu=state["relu"])
+    leaves = state["x"], state["w"], state["b"]
+    y = lowbit.checkpointed_linear(*leaves, relu=state["relu"])
+    dx, dw, db = torch.autograd.grad(y, leaves, state["dy"])
+    return {"y": y.detach(), "dx": dx, "dw": dw, "db": db}
+
+
+def work(case):
+    m, k, n, size = case["tokens"], case["inputs"], case["outputs"], SIZE[case["type"]]
+    if case["op"] == "rows":  # x in, its values and scales out; a maximum, a quotient and a rounding each
+        return {"bytes": 2 * m * k * size + 4 * m, "flops": 3 * m * k}
+    if case["op"] == "product":  # x, the codes and scales of the weight, the bias; y
+        return {"bytes": m * k * size + n * k + 4 * n + n * size + m * n * size, "flops": 2 * m * n * k}
+    # x, W, b and dy in; y, dx, dW and db out; three products
+    return {"bytes": size * (2 * m * k + 2 * m * n + 2 * n * k + 2 * n), "flops": 6 * m * n * k}
+
+
+# ---- the definitions in 64 bits -----------------------------------------------------------------
+
+def _nearest_codes(v):
+    """Row codes and scales of float64 rows: the scale is a number of 32 bits, the quotient is not rounded."""
+    largest = v.abs().max(dim=1).values
+    scale = torch.clamp((largest / 127).float(), min=torch.finfo(torch.float32).tiny).double()
+    return torch.clamp((v / scale.unsqueeze(1)).round(), -127, 127), scale
+
+
+def _checkpoint_values(a, most):
+    """most: the largest multiple of the step that a code holds."""
+    m, k = a.shape
+    groups = torch.nn.functional.pad(a, (0, -k % 32)).reshape(m, -1, 32)
+    largest = groups.abs().max(dim=2, keepdim=True).values
+    fraction, _ = torch.frexp(largest)  # largest = fraction 2^power, fraction in [1/2, 1)
+    bits = 7 if most == 127 else 8
+    two = torch.where(largest > 0, largest / fraction, 1.0)  # 2^power, exactly
+    step = torch.clamp(two * 2.0 ** -bits * torch.where(fraction > most / 2.0 ** bits, 2.0, 1.0), min=2.0 ** -126)
+    return ((groups / step).round().clamp(-127, most) * step).reshape(m, -1)[:, :k]
+
+
+def exact(case, seed):
+    global own
+    was, own = own, False
+    try:
+        state = prepare(case, seed)
+    finally:
+        own = was
+    with torch.no_grad():
+        x = state["x"].detach().double()
+        if case["op"] == "rows":
+            q, s = _nearest_codes(x)
+            return {"values": q * s.unsqueeze(1), "scales": s}
+        b = state["b"].detach().double()
+        if case["op"] == "product":
+            q, s = _nearest_codes(x)
+            wq, ws = state["w"]
+            y = torch.outer(s, ws.double()) * torch.matmul(q, wq.double().t().contiguous()) + b
+            return torch.relu(y) if case["relu"] else y
+        w, dy = state["w"].detach().double(), state["dy"].double()
+        a = torch.relu(x) if case["relu"] else x
+        dx = torch.matmul(dy, w)
+        return {"y": torch.addmm(b, a, w.t().contiguous()),
+                "dx": torch.where(x > 0, dx, torch.zeros_like(dx)) if case["relu"] else dx,
+                "dw": torch.matmul(dy.t().contiguous(), _checkpoint_values(a, 254 if case["relu"] else 127)),
+                "db": dy.sum(dim=0)}
