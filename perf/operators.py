@@ -17,6 +17,8 @@ Three operators (nicecore.lowbit):
 A case: op, tokens (rows), inputs (K), outputs (N), type of x and of the result, relu.
 """
 import math
+import os
+import sys
 
 import torch
 
@@ -24,6 +26,14 @@ own = False
 
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 SIZE = {"f32": 4, "bf16": 2, "f16": 2}
+
+
+def _lowbit():
+    package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "nice-slam-annotation_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    from nicecore import lowbit
+    return lowbit
 
 
 def listed():
@@ -94,8 +104,7 @@ def prepare(case, seed):
     state["b"] = (0.1 * torch.randn(n, generator=gen, device="cuda")).to(TYPES[kind])
     if case["op"] == "product":
         if own:
-            from nicecore import lowbit
-            state["w"] = lowbit.quantize_rows(w)
+            state["w"] = _lowbit().quantize_rows(w)
         else:
             state["w"] = _rows(w)
         return state
@@ -165,7 +174,7 @@ def run(state):
     if not own:
         with torch.no_grad():
             return _plain(state)
-    from nicecore import lowbit
+    lowbit = _lowbit()
     if state["op"] == "rows":
         q = lowbit.quantize_rows(state["x"])
         return {"values": q.dequantize(), "scales": q.scales}
