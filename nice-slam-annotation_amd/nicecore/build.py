@@ -27,6 +27,9 @@ LIB = os.path.join(HERE, "libnicecore.so")
 SOURCES = ["nc_abi.hip", "nc_rays.hip", "nc_mlp.hip", "nc_grid.hip", "nc_det.hip", "nc_sample.hip", "nc_frustum.hip", "nc_adam.hip",
            "nc_sparse.hip", "nc_pdf.hip", "nc_imap.hip"]
 ARCH = os.environ.get("NICECORE_ARCH", "gfx950")
+# No packed-FP32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong
+# results on this hardware now and then.  hipcc's host pass says that it does not know the feature.
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 SRC_EXT = (".hip", ".h", ".hpp", ".cpp")
@@ -119,7 +122,7 @@ def build(force: bool = False, verbose: bool = False, extra=(), out: str | None 
 
 def _build_locked(lib: str, verbose: bool, extra, csrc: str, variant: str) -> str:
     vid = variant_suffix([*extra, variant] if variant else extra)
-    flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall",
+    flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", *NO_PACKED_FP32, "-Wall",
              "-Wno-unused-function", "-Wno-unused-variable", "-I", INCLUDE, "-I", csrc,
              f'-DNC_SRC_HASH="{source_hash()}{vid}"', *extra]
     # one hipcc per source in parallel, then one link: the wall time is the slowest file

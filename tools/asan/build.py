@@ -24,7 +24,7 @@ OUT_DIR = os.path.join(REPO, "build", "asan")
 EXE = os.path.join(OUT_DIR, "abi_host_check")
 SAN = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
        "-Xarch_host", "-fno-omit-frame-pointer", "-Xarch_host", "-fno-sanitize-recover=undefined"]
-FLAGS = [f"--offload-arch={B.ARCH}", "-O1", "-g", "-std=c++17", "-fPIC", "-ffp-contract=off",
+FLAGS = [f"--offload-arch={B.ARCH}", "-O1", "-g", "-std=c++17", "-fPIC", "-ffp-contract=off", *B.NO_PACKED_FP32,
          "-I", B.INCLUDE, "-I", B.CSRC, *SAN]
 
 
