@@ -23,6 +23,9 @@
  *   nc_adam_step        torch.optim.Adam / SparseAdam step (src/Mapper.py:462-485, :625)
  *   nc_sample_pdf       src/common.py:19-63 sample_pdf (importance sampling,
  *                       Renderer.py:244-250 when N_importance > 0).
+ *   nc_encode_rows ...  8-bit layer operators for the scene MLP's layers (decoder.py:190-219):
+ *   nc_layer_*          row codes, the 8-bit product, the layer whose backward keeps an
+ *                       8-bit checkpoint of its input (end of this file).
  *   nc_sparse_rows_*    the touched-voxel gradient of a feature grid too large for a
  *                       dense gradient: the reference's dense
  *                       grid.grad / val[mask] gradient (Mapper.py:392-404, :620-627)
@@ -55,7 +58,7 @@
 extern "C" {
 #endif
 
-#define NC_ABI_VERSION 11
+#define NC_ABI_VERSION 12
 #define NC_MAX_SAMPLES 64 /* n_strat + n_surf per ray (one wavefront per ray) */
 #define NC_MAX_SURF 32
 
@@ -471,7 +474,8 @@ int64_t nc_param_count(int decoder);
 /* sizeof() of the ABI structs, for binding-layout checks:
  * 0 nc_render_args, 1 nc_points_args, 2 nc_grid, 3 nc_decoder_params, 4 nc_sample_args, 5 nc_frustum_args,
  * 6 nc_sparse_rows, 7 nc_pdf_args, 8 nc_adam_args, 9 nc_adam_segment, 10 nc_imap_render_args,
- * 11 nc_imap_points_args, 12 nc_imap_params, 13 nc_grid_rows_args. */
+ * 11 nc_imap_points_args, 12 nc_imap_params, 13 nc_grid_rows_args, 14 nc_codes_args,
+ * 15 nc_qlinear_args, 16 nc_layer_args. */
 size_t nc_struct_size(int which);
 
 size_t nc_render_workspace_bytes(const nc_render_args* args);
@@ -575,6 +579,88 @@ int nc_imap_points_backward(const nc_imap_points_args* args, void* workspace, si
  * read-only introspection (the tests score weight gradients against a float64 truth
  * evaluated on the same ReLU branches).  Returns -1 for a bad layer or arguments. */
 int64_t nc_imap_points_activation_offset(const nc_imap_points_args* args, int layer);
+
+/* ---- 8-bit layer operators (ABI v12) ---------------------------------------------
+ * Codes are kept in rows of code_stride bytes, a multiple of 128 and at least the number of
+ * columns, 16-byte aligned; behind the last column the encoder writes codes of 0. */
+#define NC_F32 0
+#define NC_F16 1
+#define NC_BF16 2
+#define NC_CODES_ROW 0   /* int8, float scale per row: s = max(fl(amax / 127), 2^-126), q = nearest to x / s */
+#define NC_CODES_GROUP 1 /* int8, one byte b per 32 columns: the step is 2^(b - 127), the least with 127 steps >= amax */
+#define NC_CODES_RELU 2  /* uint8 of max(x, 0): 0 where x <= 0, else 1 + the number of steps (254 steps >= amax) */
+#define NC_MAX_INPUTS 131072 /* 127^2 * 131072 < 2^31: an int32 sum of code products cannot overflow */
+
+typedef struct nc_codes_args {
+  int32_t abi_version;
+  int32_t dtype;       /* of x and values */
+  int32_t format;      /* NC_CODES_* */
+  int32_t reserved;
+  int64_t rows, cols;
+  int64_t stride;      /* elements between rows of x / values */
+  int64_t code_stride;
+  const void* x;       /* encode */
+  uint8_t* codes;      /* [rows][code_stride] */
+  void* scales;        /* NC_CODES_ROW: float [rows]; else uint8 [rows][code_stride / 32] */
+  void* values;        /* decode */
+} nc_codes_args;
+/* A row (group) that holds an infinity or NaN decodes to NaN throughout. */
+int nc_encode_rows(const nc_codes_args* args, void* stream);
+int nc_decode_rows(const nc_codes_args* args, void* stream);
+
+/* out[m][n] = (sum_k qx[m][k] qw[n][k]) sx[m] sw[n] + bias[n], then ReLU if asked.  x is encoded by
+ * the call (NC_CODES_ROW, in the workspace), or given as codes with x = NULL. */
+typedef struct nc_qlinear_args {
+  int32_t abi_version;
+  int32_t dtype;       /* of x */
+  int32_t out_dtype, bias_dtype;
+  int32_t relu;
+  int32_t reserved;
+  int64_t rows, inputs, outputs;
+  const void* x;       /* [rows][x_stride], or NULL */
+  int64_t x_stride;
+  const uint8_t* x_codes; /* with x = NULL */
+  const float* x_scales;
+  int64_t code_stride; /* of x_codes and w_codes */
+  const uint8_t* w_codes; /* [outputs][code_stride] */
+  const float* w_scales;  /* [outputs] */
+  const void* bias;    /* [outputs] or NULL */
+  void* out;           /* [rows][out_stride] */
+  int64_t out_stride;
+} nc_qlinear_args;
+size_t nc_quantized_linear_workspace_bytes(const nc_qlinear_args* args);
+int nc_quantized_linear(const nc_qlinear_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = a W^T + bias, a = relu ? max(x, 0) : x; the forward also writes a's codes (NC_CODES_RELU or
+ * NC_CODES_GROUP), all that the backward reads of x:
+ *   dx = (dy W) [code != 0 if relu],  dw = dy^T value(codes),  db = sum_m dy.
+ * codes may be NULL in a forward without a backward.  Every output of the backward may be NULL.
+ * The workspace of either call is free again when the call's work on the stream has ended. */
+typedef struct nc_layer_args {
+  int32_t abi_version;
+  int32_t dtype;       /* of every tensor; products and sums in 32 bits */
+  int32_t relu;
+  int32_t reserved;
+  int64_t rows, inputs, outputs;
+  const void* x;       /* forward */
+  int64_t x_stride;
+  const void* w;       /* [outputs][w_stride] */
+  int64_t w_stride;
+  const void* bias;    /* [outputs] or NULL */
+  void* y;             /* [rows][y_stride] */
+  int64_t y_stride;
+  uint8_t* codes;      /* [rows][code_stride] */
+  uint8_t* steps;      /* [rows][code_stride / 32] */
+  int64_t code_stride;
+  const void* dy;      /* backward: [rows][dy_stride] */
+  int64_t dy_stride;
+  void* dx;            /* [rows][inputs] */
+  void* dw;            /* [outputs][inputs] */
+  void* db;            /* [outputs] */
+} nc_layer_args;
+size_t nc_layer_workspace_bytes(const nc_layer_args* args, int backward);
+int nc_layer_forward(const nc_layer_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int nc_layer_backward(const nc_layer_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -17,6 +17,7 @@
 
 #include "nc_device.h"
 #include "nc_internal.h"
+#include "nc_lowbit.h"
 #include "nc_wimage.h"
 
 using namespace nc;
@@ -41,14 +42,15 @@ enum KernelId {
   KID_PARAM_REDUCE, KID_RAY_GRADS, KID_POINTS_ASSEMBLE, KID_POINTS_SPLIT, KID_POINTS_GRADS, KID_GRID_BWD, KID_MLP_DW,
   KID_GRID_GATHER, KID_LOSS, KID_DET_SCATTER, KID_SAMPLE_RAYS, KID_SAMPLE_POSE_GRAD, KID_FRUSTUM, KID_ROWS_CLEAR,
   KID_ROWS_MERGE, KID_ROWS_CLAIM, KID_PARAM_RAY, KID_SAMPLE_PDF, KID_ADAM, KID_IMAP_GEMM, KID_IMAP_FOURIER, KID_GRID_ROWS,
-  KID_COMPOSITE_FWD_LOSS, KID_COUNT
+  KID_COMPOSITE_FWD_LOSS, KID_CODES, KID_LOW_GEMM, KID_LOW_WGRAD, KID_COUNT
 };
 const char* kKernelNames[KID_COUNT] = {"k_depth_max", "k_ray_setup", "k_mlp_fwd", "k_composite_fwd",
                                        "k_composite_bwd", "k_mlp_dx", "k_param_reduce", "k_ray_grads",
                                        "k_points_assemble", "k_points_split_grad", "k_points_grads", "k_grid_bwd",
                                        "k_mlp_dw", "k_grid_gather", "k_loss", "k_det_scatter",
                                        "k_sample_rays", "k_sample_pose_grad", "k_frustum_mask", "k_rows_clear", "k_rows_merge", "k_rows_compact", "k_param_ray_reduce", "k_sample_pdf", "k_adam",
-                                       "k_imap_gemm", "k_imap_fourier", "k_grid_rows", "k_composite_fwd_loss"};
+                                       "k_imap_gemm", "k_imap_fourier", "k_grid_rows", "k_composite_fwd_loss",
+                                       "k_codes", "k_low_gemm", "k_low_wgrad"};
 struct TimedLaunch {
   hipEvent_t b, e;
   int id;
@@ -824,6 +826,9 @@ size_t nc_struct_size(int which) {
     case 11: return sizeof(nc_imap_points_args);
     case 12: return sizeof(nc_imap_params);
     case 13: return sizeof(nc_grid_rows_args);
+    case 14: return sizeof(nc_codes_args);
+    case 15: return sizeof(nc_qlinear_args);
+    case 16: return sizeof(nc_layer_args);
   }
   return 0;
 }
@@ -1586,6 +1591,370 @@ int nc_imap_points_backward(const nc_imap_points_args* a, void* ws, size_t ws_by
   if (!a->g_pts && !a->dec.grad) return 0;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return imap_mlp_backward(a->dec, a->n_points, ws, w, a->g_raw, a->g_pts, s);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// 8-bit layer operators (ABI v12, nc_lowbit.h): [encode] -> k_low_gemm; the layer's forward
+// is encode (codes + the 16-bit copy or planes of the input) -> k_low_gemm, its backward
+// encode (dY's copy or planes) -> transpose (W) -> k_low_gemm (dX) -> k_low_wgrad -> sums.
+// ---------------------------------------------------------------------------
+namespace {
+
+int64_t elem_size(int dtype) { return dtype == NC_F32 ? 4 : 2; }
+bool dtype_ok(int dtype) { return dtype == NC_F32 || dtype == NC_F16 || dtype == NC_BF16; }
+
+int check_codes(const void* codes, int64_t stride, int64_t cols) {
+  if (stride < cols || stride % CODE_ALIGN != 0) return fail(-1, "nicecore: code_stride must be a multiple of 128 that holds the columns");
+  if (reinterpret_cast<uintptr_t>(codes) & 15) return fail(-1, "nicecore: codes must be 16-byte aligned");
+  return 0;
+}
+
+int check_matrix(int64_t rows, int64_t inputs, int64_t outputs) {
+  if (rows < 0 || inputs < 1 || outputs < 1) return fail(-1, "nicecore: need rows >= 0, inputs >= 1, outputs >= 1");
+  if (inputs > NC_MAX_INPUTS || outputs > NC_MAX_INPUTS) return fail(-1, "nicecore: inputs and outputs must not exceed 131072");
+  if (rows > INT32_MAX) return fail(-1, "nicecore: rows must be below 2^31");
+  return 0;
+}
+
+int check_codes_args(const nc_codes_args* a) {
+  if (!a) return fail(-1, "nicecore: args is NULL");
+  if (a->abi_version != NC_ABI_VERSION) return fail(-2, "nicecore: ABI version mismatch");
+  if (!dtype_ok(a->dtype)) return fail(-1, "nicecore: unknown dtype");
+  if (a->format < NC_CODES_ROW || a->format > NC_CODES_RELU) return fail(-1, "nicecore: unknown code format");
+  if (int e = check_matrix(a->rows, a->cols, 1)) return e;
+  if (a->stride < 0) return fail(-1, "nicecore: negative row stride");
+  return check_codes(a->codes, a->code_stride, a->cols);
+}
+
+CodeCtx codes_ctx(const nc_codes_args* a) {
+  CodeCtx c;
+  std::memset(&c, 0, sizeof(c));
+  c.dtype = a->dtype;
+  c.format = a->format;
+  c.rows = a->rows;
+  c.cols = a->cols;
+  c.x = a->x;
+  c.x_stride = a->stride;
+  c.codes = a->codes;
+  c.code_stride = a->code_stride;
+  c.scales = a->scales;
+  c.values = a->values;
+  return c;
+}
+
+int run_encode(const CodeCtx& c, hipStream_t s) {
+  return check_hip(timed(KID_CODES, s, [&] { return launch_encode(c, s); }), "encode");
+}
+int run_low_gemm(const LowGemm& g, hipStream_t s) {
+  return check_hip(timed(KID_LOW_GEMM, s, [&] { return launch_low_gemm(g, s); }), "k_low_gemm");
+}
+
+// a 16-bit matrix that the matrix kernels can read in place: whole 128-byte slices (cols a multiple
+// of 64), 16-byte aligned rows, offsets inside a tile below 2^32
+bool in_place(int dtype, const void* p, int64_t cols, int64_t stride) {
+  return dtype != NC_F32 && cols % ROW_ALIGN == 0 && stride % 8 == 0 && stride >= cols && stride <= (int64_t(1) << 22) &&
+         (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+// [rows][cols] as the matrix kernels read it: in place, or a padded copy / three planes in the workspace
+struct Operand {
+  bool copy;
+  size_t at, bytes;        // workspace
+  int64_t stride, plane;   // elements
+};
+Operand operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t stride, bool change, size_t& o) {
+  Operand r;
+  r.copy = change || !in_place(dtype, p, cols, stride);
+  r.at = o;
+  r.stride = r.copy ? round_up(cols, ROW_ALIGN) : stride;
+  r.plane = r.copy ? rows * r.stride : 0;
+  r.bytes = r.copy ? (size_t)(dtype == NC_F32 ? 3 : 1) * (size_t)r.plane * 2 : 0;
+  o = align256(o + r.bytes);
+  return r;
+}
+
+struct LayerWs {
+  Operand x, w, dy, wt;
+  size_t part = 0, dbpart = 0, total = 0;
+  int32_t splits = 0, slices = 0;
+  int64_t rows_per = 0;
+};
+
+void layer_layout(const nc_layer_args* a, bool backward, LayerWs& w) {
+  size_t o = 0;
+  if (!backward) {
+    w.x = operand(a->dtype, a->x, a->rows, a->inputs, a->x_stride, a->relu != 0, o);
+    w.w = operand(a->dtype, a->w, a->outputs, a->inputs, a->w_stride, false, o);
+  } else {
+    w.dy = operand(a->dtype, a->dy, a->rows, a->outputs, a->dy_stride, false, o);
+    w.wt = operand(a->dtype, nullptr, a->inputs, a->outputs, 0, true, o);
+    low_wgrad_splits(a->rows, a->outputs, a->inputs, w.splits, w.rows_per);
+    w.part = o;
+    o = align256(o + (size_t)w.splits * (size_t)a->outputs * (size_t)a->inputs * 4);
+    w.slices = (int32_t)((a->rows + 511) / 512);
+    if (w.slices > 256) w.slices = 256;
+    w.dbpart = o;
+    o = align256(o + (size_t)w.slices * (size_t)a->outputs * 4);
+  }
+  w.total = o;
+}
+
+int layer_check(const nc_layer_args* a) {
+  if (!a) return fail(-1, "nicecore: args is NULL");
+  if (a->abi_version != NC_ABI_VERSION) return fail(-2, "nicecore: ABI version mismatch");
+  if (!dtype_ok(a->dtype)) return fail(-1, "nicecore: unknown dtype");
+  if (int e = check_matrix(a->rows, a->inputs, a->outputs)) return e;
+  if (a->x_stride < 0 || a->w_stride < 0 || a->dy_stride < 0 || a->y_stride < 0) return fail(-1, "nicecore: negative row stride");
+  return 0;
+}
+
+int copy_operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t stride, bool relu, const Operand& op,
+                 void* ws, hipStream_t s, uint8_t* codes = nullptr, uint8_t* steps = nullptr, int64_t code_stride = 0) {
+  CodeCtx c;
+  std::memset(&c, 0, sizeof(c));
+  c.dtype = dtype;
+  c.format = codes ? (relu ? NC_CODES_RELU : NC_CODES_GROUP) : -1;
+  c.rows = rows;
+  c.cols = cols;
+  c.x = p;
+  c.x_stride = stride;
+  c.codes = codes;
+  c.code_stride = code_stride;
+  c.scales = steps;
+  c.relu = relu ? 1 : 0;
+  if (op.copy) {
+    c.copy = at<uint16_t>(ws, op.at);
+    c.copy_stride = op.stride;
+    c.plane = op.plane;
+  }
+  if (!codes && !op.copy) return 0;
+  return run_encode(c, s);
+}
+
+LowGemm layer_gemm(int dtype, const void* A, const Operand& oa, const void* B, const Operand& ob, void* ws, int64_t M,
+                   int64_t N, int64_t K) {
+  LowGemm g;
+  std::memset(&g, 0, sizeof(g));
+  g.A = oa.copy ? at<uint8_t>(ws, oa.at) : static_cast<const uint8_t*>(A);
+  g.B = ob.copy ? at<uint8_t>(ws, ob.at) : static_cast<const uint8_t*>(B);
+  g.lda = 2 * oa.stride;
+  g.ldb = 2 * ob.stride;
+  g.plane_a = 2 * oa.plane;
+  g.plane_b = 2 * ob.plane;
+  g.M = M;
+  g.N = N;
+  g.slices = (int32_t)((K + ROW_ALIGN - 1) / ROW_ALIGN);
+  g.segments = dtype == NC_F32 ? 6 : 1;
+  g.mode = dtype == NC_F16 ? LOW_F16 : LOW_BF16;
+  g.out_dtype = dtype;
+  g.bias_dtype = dtype;
+  return g;
+}
+
+int qlinear_check(const nc_qlinear_args* a) {
+  if (!a) return fail(-1, "nicecore: args is NULL");
+  if (a->abi_version != NC_ABI_VERSION) return fail(-2, "nicecore: ABI version mismatch");
+  if ((a->x && !dtype_ok(a->dtype)) || !dtype_ok(a->out_dtype) || (a->bias && !dtype_ok(a->bias_dtype)))
+    return fail(-1, "nicecore: unknown dtype");
+  if (int e = check_matrix(a->rows, a->inputs, a->outputs)) return e;
+  if (a->x_stride < 0 || a->out_stride < 0) return fail(-1, "nicecore: negative row stride");
+  if (int e = check_codes(a->w_codes, a->code_stride, a->inputs)) return e;
+  if (!a->x)
+    if (int e = check_codes(a->x_codes, a->code_stride, a->inputs)) return e;
+  return 0;
+}
+
+struct QlinearWs {
+  size_t codes = 0, scales = 0, total = 0;
+};
+void qlinear_layout(const nc_qlinear_args* a, QlinearWs& w) {
+  size_t o = 0;
+  if (a->x) {
+    w.codes = o;
+    o = align256(o + (size_t)a->rows * (size_t)a->code_stride);
+    w.scales = o;
+    o = align256(o + (size_t)a->rows * 4);
+  }
+  w.total = o > 0 ? o : 256;
+}
+
+}  // namespace
+
+extern "C" {
+
+int nc_encode_rows(const nc_codes_args* a, void* stream) {
+  if (int e = check_codes_args(a)) return e;
+  if (a->rows == 0) return 0;
+  if (!a->x || !a->codes || !a->scales) return fail(-1, "nicecore: NULL x, codes or scales");
+  return run_encode(codes_ctx(a), reinterpret_cast<hipStream_t>(stream));
+}
+
+int nc_decode_rows(const nc_codes_args* a, void* stream) {
+  if (int e = check_codes_args(a)) return e;
+  if (a->rows == 0) return 0;
+  if (!a->values || !a->codes || !a->scales) return fail(-1, "nicecore: NULL values, codes or scales");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return check_hip(timed(KID_CODES, s, [&] { return launch_decode(codes_ctx(a), s); }), "decode");
+}
+
+size_t nc_quantized_linear_workspace_bytes(const nc_qlinear_args* a) {
+  if (qlinear_check(a)) return 0;
+  QlinearWs w;
+  qlinear_layout(a, w);
+  return w.total;
+}
+
+int nc_quantized_linear(const nc_qlinear_args* a, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = qlinear_check(a)) return e;
+  QlinearWs w;
+  qlinear_layout(a, w);
+  if (a->rows == 0) return 0;
+  if (!ws || ws_bytes < w.total) return fail(-1, "nicecore: workspace too small");
+  if (!a->w_codes || !a->w_scales || !a->out || (!a->x && (!a->x_codes || !a->x_scales)))
+    return fail(-1, "nicecore: NULL x, codes, scales or output");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const uint8_t* xc = a->x_codes;
+  const float* xs = a->x_scales;
+  if (a->x) {
+    CodeCtx c;
+    std::memset(&c, 0, sizeof(c));
+    c.dtype = a->dtype;
+    c.format = NC_CODES_ROW;
+    c.rows = a->rows;
+    c.cols = a->inputs;
+    c.x = a->x;
+    c.x_stride = a->x_stride;
+    c.codes = at<uint8_t>(ws, w.codes);
+    c.code_stride = a->code_stride;
+    c.scales = at<float>(ws, w.scales);
+    if (int e = run_encode(c, s)) return e;
+    xc = c.codes;
+    xs = at<float>(ws, w.scales);
+  }
+  LowGemm g;
+  std::memset(&g, 0, sizeof(g));
+  g.A = xc;
+  g.B = a->w_codes;
+  g.lda = g.ldb = a->code_stride;
+  g.M = a->rows;
+  g.N = a->outputs;
+  g.slices = (int32_t)((a->inputs + CODE_ALIGN - 1) / CODE_ALIGN);
+  g.segments = 1;
+  g.mode = LOW_I8;
+  g.out_dtype = a->out_dtype;
+  g.bias_dtype = a->bias_dtype;
+  g.relu = a->relu != 0;
+  g.out = a->out;
+  g.ldc = a->out_stride;
+  g.bias = a->bias;
+  g.row_scale = xs;
+  g.col_scale = a->w_scales;
+  return run_low_gemm(g, s);
+}
+
+size_t nc_layer_workspace_bytes(const nc_layer_args* a, int backward) {
+  if (layer_check(a)) return 0;
+  LayerWs w;
+  layer_layout(a, backward != 0, w);
+  return w.total > 0 ? w.total : 256;
+}
+
+int nc_layer_forward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = layer_check(a)) return e;
+  LayerWs w;
+  layer_layout(a, false, w);
+  if (a->codes)
+    if (int e = check_codes(a->codes, a->code_stride, a->inputs)) return e;
+  if (a->rows == 0) return 0;
+  if (!a->x || !a->w || !a->y || (a->codes && !a->steps)) return fail(-1, "nicecore: NULL x, w, y or steps");
+  if (w.total && (!ws || ws_bytes < w.total)) return fail(-1, "nicecore: workspace too small");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (int e = copy_operand(a->dtype, a->x, a->rows, a->inputs, a->x_stride, a->relu != 0, w.x, ws, s, a->codes, a->steps,
+                           a->code_stride))
+    return e;
+  if (int e = copy_operand(a->dtype, a->w, a->outputs, a->inputs, a->w_stride, false, w.w, ws, s)) return e;
+  LowGemm g = layer_gemm(a->dtype, a->x, w.x, a->w, w.w, ws, a->rows, a->outputs, a->inputs);
+  g.out = a->y;
+  g.ldc = a->y_stride;
+  g.bias = a->bias;
+  return run_low_gemm(g, s);
+}
+
+int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = layer_check(a)) return e;
+  LayerWs w;
+  layer_layout(a, true, w);
+  if (!a->dx && !a->dw && !a->db) return 0;
+  if (!a->dy && a->rows > 0) return fail(-1, "nicecore: NULL dy");
+  if ((a->dw || (a->dx && a->relu)) && a->rows > 0) {
+    if (!a->codes || !a->steps) return fail(-1, "nicecore: NULL codes or steps");
+    if (int e = check_codes(a->codes, a->code_stride, a->inputs)) return e;
+  }
+  if (a->dx && !a->w) return fail(-1, "nicecore: NULL w");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int64_t nk = a->outputs * a->inputs;
+  if (a->rows == 0) {  // empty sums
+    if (a->dw)
+      if (int e = check_hip(launch_sum_parts(nullptr, nk, 0, a->dw, a->dtype, s), "sum_parts")) return e;
+    if (a->db)
+      if (int e = check_hip(launch_sum_parts(nullptr, a->outputs, 0, a->db, a->dtype, s), "sum_parts")) return e;
+    return 0;
+  }
+  if (!ws || ws_bytes < w.total) return fail(-1, "nicecore: workspace too small");
+  if (a->dx || a->dw)
+    if (int e = copy_operand(a->dtype, a->dy, a->rows, a->outputs, a->dy_stride, false, w.dy, ws, s)) return e;
+  if (a->dx) {
+    TransposeCtx t;
+    t.dtype = a->dtype;
+    t.rows = a->outputs;
+    t.cols = a->inputs;
+    t.src = a->w;
+    t.src_stride = a->w_stride;
+    t.dst = at<uint16_t>(ws, w.wt.at);
+    t.dst_stride = w.wt.stride;
+    t.plane = w.wt.plane;
+    if (int e = check_hip(timed(KID_CODES, s, [&] { return launch_transpose(t, s); }), "transpose")) return e;
+    LowGemm g = layer_gemm(a->dtype, a->dy, w.dy, nullptr, w.wt, ws, a->rows, a->inputs, a->outputs);
+    g.out = a->dx;
+    g.ldc = a->inputs;
+    if (a->relu) {
+      g.mask = a->codes;
+      g.ldm = a->code_stride;
+    }
+    if (int e = run_low_gemm(g, s)) return e;
+  }
+  if (a->dw) {
+    LowWgrad g;
+    std::memset(&g, 0, sizeof(g));
+    g.dy = w.dy.copy ? at<uint16_t>(ws, w.dy.at) : static_cast<const uint16_t*>(a->dy);
+    g.ldy = w.dy.stride;
+    g.plane = w.dy.plane;
+    g.planes = a->dtype == NC_F32 ? 3 : 1;
+    g.f16 = a->dtype == NC_F16;
+    g.relu = a->relu != 0;
+    g.codes = a->codes;
+    g.steps = a->steps;
+    g.code_stride = a->code_stride;
+    g.M = a->rows;
+    g.N = a->outputs;
+    g.K = a->inputs;
+    g.part = at<float>(ws, w.part);
+    g.splits = w.splits;
+    g.rows_per = w.rows_per;
+    if (int e = check_hip(timed(KID_LOW_WGRAD, s, [&] { return launch_low_wgrad(g, s); }), "k_low_wgrad")) return e;
+    if (int e = check_hip(timed(KID_LOW_WGRAD, s, [&] { return launch_sum_parts(g.part, nk, w.splits, a->dw, a->dtype, s); }),
+                          "sum_parts"))
+      return e;
+  }
+  if (a->db) {
+    float* part = at<float>(ws, w.dbpart);
+    if (int e = check_hip(launch_col_sums(a->dy, a->dtype, a->rows, a->outputs, a->dy_stride, w.slices, part, s), "col_sums"))
+      return e;
+    if (int e = check_hip(launch_sum_parts(part, a->outputs, w.slices, a->db, a->dtype, s), "sum_parts")) return e;
+  }
+  return 0;
 }
 
 }  // extern "C"

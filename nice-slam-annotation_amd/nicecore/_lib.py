@@ -12,7 +12,7 @@ from ctypes import POINTER, c_double, c_float, c_int, c_int32, c_int64, c_size_t
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libnicecore.so")
 
-NC_ABI_VERSION = 11
+NC_ABI_VERSION = 12
 NC_SAVE_FOR_BACKWARD = 1
 NC_DETERMINISTIC = 2
 NC_SAVE_POINT_JACOBIAN = 4
@@ -157,6 +157,33 @@ class NcImapPointsArgs(ctypes.Structure):
                 ("dec", NcImapParams), ("raw", c_void_p), ("g_raw", c_void_p), ("g_pts", c_void_p)]
 
 
+NC_F32, NC_F16, NC_BF16 = 0, 1, 2
+NC_CODES_ROW, NC_CODES_GROUP, NC_CODES_RELU = 0, 1, 2
+NC_MAX_INPUTS = 131072
+
+
+class NcCodesArgs(ctypes.Structure):
+    _fields_ = [("abi_version", c_int32), ("dtype", c_int32), ("format", c_int32), ("reserved", c_int32),
+                ("rows", c_int64), ("cols", c_int64), ("stride", c_int64), ("code_stride", c_int64),
+                ("x", c_void_p), ("codes", c_void_p), ("scales", c_void_p), ("values", c_void_p)]
+
+
+class NcQlinearArgs(ctypes.Structure):
+    _fields_ = [("abi_version", c_int32), ("dtype", c_int32), ("out_dtype", c_int32), ("bias_dtype", c_int32),
+                ("relu", c_int32), ("reserved", c_int32),
+                ("rows", c_int64), ("inputs", c_int64), ("outputs", c_int64), ("x", c_void_p), ("x_stride", c_int64),
+                ("x_codes", c_void_p), ("x_scales", c_void_p), ("code_stride", c_int64), ("w_codes", c_void_p),
+                ("w_scales", c_void_p), ("bias", c_void_p), ("out", c_void_p), ("out_stride", c_int64)]
+
+
+class NcLayerArgs(ctypes.Structure):
+    _fields_ = [("abi_version", c_int32), ("dtype", c_int32), ("relu", c_int32), ("reserved", c_int32),
+                ("rows", c_int64), ("inputs", c_int64), ("outputs", c_int64), ("x", c_void_p), ("x_stride", c_int64),
+                ("w", c_void_p), ("w_stride", c_int64), ("bias", c_void_p), ("y", c_void_p), ("y_stride", c_int64),
+                ("codes", c_void_p), ("steps", c_void_p), ("code_stride", c_int64),
+                ("dy", c_void_p), ("dy_stride", c_int64), ("dx", c_void_p), ("dw", c_void_p), ("db", c_void_p)]
+
+
 NC_ADAM_DENSE = 0
 NC_ADAM_SPARSE_ROWS = 1
 
@@ -193,6 +220,13 @@ EXPORTS = {
     "nc_imap_points_forward": (c_int, [POINTER(NcImapPointsArgs), c_void_p, c_size_t, c_void_p]),
     "nc_imap_points_backward": (c_int, [POINTER(NcImapPointsArgs), c_void_p, c_size_t, c_void_p]),
     "nc_imap_points_activation_offset": (c_int64, [POINTER(NcImapPointsArgs), c_int]),
+    "nc_encode_rows": (c_int, [POINTER(NcCodesArgs), c_void_p]),
+    "nc_decode_rows": (c_int, [POINTER(NcCodesArgs), c_void_p]),
+    "nc_quantized_linear_workspace_bytes": (c_size_t, [POINTER(NcQlinearArgs)]),
+    "nc_quantized_linear": (c_int, [POINTER(NcQlinearArgs), c_void_p, c_size_t, c_void_p]),
+    "nc_layer_workspace_bytes": (c_size_t, [POINTER(NcLayerArgs), c_int]),
+    "nc_layer_forward": (c_int, [POINTER(NcLayerArgs), c_void_p, c_size_t, c_void_p]),
+    "nc_layer_backward": (c_int, [POINTER(NcLayerArgs), c_void_p, c_size_t, c_void_p]),
     "nc_sparse_merge_temp_bytes": (c_size_t, [c_int64, c_int64]),
     "nc_sparse_rows_merge": (c_int, [POINTER(NcSparseRows), POINTER(NcSparseRows), c_void_p, c_void_p,
                                      c_int32, c_int64, c_void_p, c_size_t, c_void_p]),
@@ -286,7 +320,8 @@ KERNEL_IDS = {"k_depth_max": 0, "k_ray_setup": 1, "k_mlp_fwd": 2, "k_composite_f
               "k_sample_rays": 16, "k_sample_pose_grad": 17, "k_frustum_mask": 18,
               "k_rows_clear": 19, "k_rows_merge": 20, "k_rows_compact": 21,
               "k_param_ray_reduce": 22, "k_sample_pdf": 23, "k_adam": 24,
-              "k_imap_gemm": 25, "k_imap_fourier": 26, "k_grid_rows": 27, "k_composite_fwd_loss": 28}
+              "k_imap_gemm": 25, "k_imap_fourier": 26, "k_grid_rows": 27, "k_composite_fwd_loss": 28,
+              "k_codes": 29, "k_low_gemm": 30, "k_low_wgrad": 31}
 
 
 class KernelTimer:

@@ -25,7 +25,7 @@ CSRC = os.path.join(PKG_ROOT, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB = os.path.join(HERE, "libnicecore.so")
 SOURCES = ["nc_abi.hip", "nc_rays.hip", "nc_mlp.hip", "nc_grid.hip", "nc_det.hip", "nc_sample.hip", "nc_frustum.hip", "nc_adam.hip",
-           "nc_sparse.hip", "nc_pdf.hip", "nc_imap.hip"]
+           "nc_sparse.hip", "nc_pdf.hip", "nc_imap.hip", "nc_lowbit.hip", "nc_lowgemm.hip"]
 ARCH = os.environ.get("NICECORE_ARCH", "gfx950")
 # No packed-FP32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong
 # results on this hardware now and then.  hipcc's host pass says that it does not know the feature.
