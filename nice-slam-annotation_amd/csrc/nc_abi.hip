@@ -1654,14 +1654,15 @@ int run_low_gemm(const LowGemm& g, hipStream_t s) {
 // a 16-bit matrix that the matrix kernels can read in place: whole 128-byte slices (cols a multiple
 // of 64), 16-byte aligned rows, offsets inside a tile below 2^32
 bool in_place(int dtype, const void* p, int64_t cols, int64_t stride) {
-  return dtype != NC_F32 && cols % ROW_ALIGN == 0 && stride % 8 == 0 && stride >= cols && stride <= (int64_t(1) << 22) &&
+  return dtype != NC_F32 && cols % ROW_ALIGN == 0 && stride % 8 == 0 && stride >= cols && stride <= NC_MAX_STRIDE &&
          (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
-// [rows][cols] as the matrix kernels read it: in place, or a padded copy / three planes in the workspace
+// [rows][cols] as the matrix kernels read it: in place, or a padded copy (float B: three planes) in the
+// workspace; float A is read as it is
 struct Operand {
   bool copy;
-  size_t at, bytes;        // workspace
+  size_t at;               // workspace
   int64_t stride, plane;   // elements
 };
 Operand operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t stride, bool change, size_t& o) {
@@ -1670,34 +1671,41 @@ Operand operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t st
   r.at = o;
   r.stride = r.copy ? round_up(cols, ROW_ALIGN) : stride;
   r.plane = r.copy ? rows * r.stride : 0;
-  r.bytes = r.copy ? (size_t)(dtype == NC_F32 ? 3 : 1) * (size_t)r.plane * 2 : 0;
-  o = align256(o + r.bytes);
+  o = align256(o + (r.copy ? (size_t)(dtype == NC_F32 ? 3 : 1) * (size_t)r.plane * 2 : 0));
   return r;
+}
+Operand operand_a(int dtype, const void* p, int64_t rows, int64_t cols, int64_t stride, bool change, size_t& o) {
+  if (dtype == NC_F32) return Operand{false, o, stride, 0};
+  return operand(dtype, p, rows, cols, stride, change, o);
 }
 
 struct LayerWs {
-  Operand x, w, dy, wt;
-  size_t part = 0, dbpart = 0, total = 0;
-  int32_t splits = 0, slices = 0;
+  Operand a, b;            // the forward's x and W, the backward's dY and W^T
+  size_t gemm_part = 0, part = 0, sums = 0, total = 0;
+  int32_t gemm_splits = 1, splits = 0, pieces = 0;
   int64_t rows_per = 0;
 };
 
+int layer_mode(int dtype) { return dtype == NC_F32 ? LOW_F32 : dtype == NC_F16 ? LOW_F16 : LOW_BF16; }
+
 void layer_layout(const nc_layer_args* a, bool backward, LayerWs& w) {
   size_t o = 0;
+  const int64_t n = backward ? a->inputs : a->outputs, k = backward ? a->outputs : a->inputs;
   if (!backward) {
-    w.x = operand(a->dtype, a->x, a->rows, a->inputs, a->x_stride, a->relu != 0, o);
-    w.w = operand(a->dtype, a->w, a->outputs, a->inputs, a->w_stride, false, o);
+    w.a = operand_a(a->dtype, a->x, a->rows, k, a->x_stride, a->relu != 0, o);
+    w.b = operand(a->dtype, a->w, n, k, a->w_stride, false, o);
   } else {
-    w.dy = operand(a->dtype, a->dy, a->rows, a->outputs, a->dy_stride, false, o);
-    w.wt = operand(a->dtype, nullptr, a->inputs, a->outputs, 0, true, o);
-    low_wgrad_splits(a->rows, a->outputs, a->inputs, w.splits, w.rows_per);
+    w.a = operand_a(a->dtype, a->dy, a->rows, k, a->dy_stride, false, o);
+    w.b = operand(a->dtype, nullptr, n, k, 0, true, o);
+    low_wgrad_splits(a->dtype, a->rows, a->outputs, a->inputs, w.splits, w.pieces, w.rows_per);
     w.part = o;
     o = align256(o + (size_t)w.splits * (size_t)a->outputs * (size_t)a->inputs * 4);
-    w.slices = (int32_t)((a->rows + 511) / 512);
-    if (w.slices > 256) w.slices = 256;
-    w.dbpart = o;
-    o = align256(o + (size_t)w.slices * (size_t)a->outputs * 4);
+    w.sums = o;
+    o = align256(o + (size_t)w.splits * (size_t)w.pieces * (size_t)a->outputs * 4);
   }
+  w.gemm_splits = low_gemm_splits(layer_mode(a->dtype), a->rows, n, k);
+  w.gemm_part = o;
+  if (w.gemm_splits > 1) o = align256(o + (size_t)w.gemm_splits * (size_t)a->rows * (size_t)n * 4);
   w.total = o;
 }
 
@@ -1707,9 +1715,11 @@ int layer_check(const nc_layer_args* a) {
   if (!dtype_ok(a->dtype)) return fail(-1, "nicecore: unknown dtype");
   if (int e = check_matrix(a->rows, a->inputs, a->outputs)) return e;
   if (a->x_stride < 0 || a->w_stride < 0 || a->dy_stride < 0 || a->y_stride < 0) return fail(-1, "nicecore: negative row stride");
+  if (a->x_stride > NC_MAX_STRIDE || a->dy_stride > NC_MAX_STRIDE) return fail(-1, "nicecore: row strides must not exceed 2^22 elements");
   return 0;
 }
 
+// the copy of an operand (relu: of max(x, 0)) and, for 16-bit types, the checkpoint's codes with it
 int copy_operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t stride, bool relu, const Operand& op,
                  void* ws, hipStream_t s, uint8_t* codes = nullptr, uint8_t* steps = nullptr, int64_t code_stride = 0) {
   CodeCtx c;
@@ -1733,23 +1743,23 @@ int copy_operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t s
   return run_encode(c, s);
 }
 
-LowGemm layer_gemm(int dtype, const void* A, const Operand& oa, const void* B, const Operand& ob, void* ws, int64_t M,
-                   int64_t N, int64_t K) {
+LowGemm layer_gemm(int dtype, const void* A, const void* B, const LayerWs& w, void* ws, int64_t M, int64_t N, int64_t K) {
   LowGemm g;
   std::memset(&g, 0, sizeof(g));
-  g.A = oa.copy ? at<uint8_t>(ws, oa.at) : static_cast<const uint8_t*>(A);
-  g.B = ob.copy ? at<uint8_t>(ws, ob.at) : static_cast<const uint8_t*>(B);
-  g.lda = 2 * oa.stride;
-  g.ldb = 2 * ob.stride;
-  g.plane_a = 2 * oa.plane;
-  g.plane_b = 2 * ob.plane;
+  g.A = w.a.copy ? at<uint8_t>(ws, w.a.at) : static_cast<const uint8_t*>(A);
+  g.B = w.b.copy ? at<uint8_t>(ws, w.b.at) : static_cast<const uint8_t*>(B);
+  g.lda = (dtype == NC_F32 ? 4 : 2) * w.a.stride;
+  g.ldb = 2 * w.b.stride;
+  g.plane_b = 2 * w.b.plane;
   g.M = M;
   g.N = N;
-  g.slices = (int32_t)((K + ROW_ALIGN - 1) / ROW_ALIGN);
-  g.segments = dtype == NC_F32 ? 6 : 1;
-  g.mode = dtype == NC_F16 ? LOW_F16 : LOW_BF16;
+  g.K = K;
+  g.mode = layer_mode(dtype);
+  g.slices = (int32_t)(dtype == NC_F32 ? (K + 31) / 32 : (K + ROW_ALIGN - 1) / ROW_ALIGN);
   g.out_dtype = dtype;
   g.bias_dtype = dtype;
+  g.splits = w.gemm_splits;
+  g.part = at<float>(ws, w.gemm_part);
   return g;
 }
 
@@ -1767,16 +1777,23 @@ int qlinear_check(const nc_qlinear_args* a) {
 }
 
 struct QlinearWs {
-  size_t codes = 0, scales = 0, total = 0;
+  size_t codes = 0, scales = 0, part = 0, total = 0;
+  int32_t splits = 1;
+  bool small = false, fused = false;  // k_low_small, encoding x itself
 };
 void qlinear_layout(const nc_qlinear_args* a, QlinearWs& w) {
   size_t o = 0;
-  if (a->x) {
+  w.fused = a->x && low_small_encodes(a->rows, a->outputs, a->inputs);
+  w.small = w.fused || a->rows <= 64;
+  if (a->x && !w.fused) {
     w.codes = o;
     o = align256(o + (size_t)a->rows * (size_t)a->code_stride);
     w.scales = o;
     o = align256(o + (size_t)a->rows * 4);
   }
+  if (!w.small) w.splits = low_gemm_splits(LOW_I8, a->rows, a->outputs, a->inputs);
+  w.part = o;
+  if (w.splits > 1) o = align256(o + (size_t)w.splits * (size_t)a->rows * (size_t)a->outputs * 4);
   w.total = o > 0 ? o : 256;
 }
 
@@ -1817,7 +1834,7 @@ int nc_quantized_linear(const nc_qlinear_args* a, void* ws, size_t ws_bytes, voi
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const uint8_t* xc = a->x_codes;
   const float* xs = a->x_scales;
-  if (a->x) {
+  if (a->x && !w.fused) {
     CodeCtx c;
     std::memset(&c, 0, sizeof(c));
     c.dtype = a->dtype;
@@ -1840,8 +1857,10 @@ int nc_quantized_linear(const nc_qlinear_args* a, void* ws, size_t ws_bytes, voi
   g.lda = g.ldb = a->code_stride;
   g.M = a->rows;
   g.N = a->outputs;
+  g.K = a->inputs;
   g.slices = (int32_t)((a->inputs + CODE_ALIGN - 1) / CODE_ALIGN);
-  g.segments = 1;
+  g.splits = w.splits;
+  g.part = at<float>(ws, w.part);
   g.mode = LOW_I8;
   g.out_dtype = a->out_dtype;
   g.bias_dtype = a->bias_dtype;
@@ -1851,7 +1870,13 @@ int nc_quantized_linear(const nc_qlinear_args* a, void* ws, size_t ws_bytes, voi
   g.bias = a->bias;
   g.row_scale = xs;
   g.col_scale = a->w_scales;
-  return run_low_gemm(g, s);
+  if (!w.small) return run_low_gemm(g, s);
+  LowSmall p;
+  p.g = g;
+  p.x_dtype = w.fused ? a->dtype : -1;
+  p.x = a->x;
+  p.x_stride = a->x_stride;
+  return check_hip(timed(KID_LOW_GEMM, s, [&] { return launch_low_small(p, s); }), "k_low_small");
 }
 
 size_t nc_layer_workspace_bytes(const nc_layer_args* a, int backward) {
@@ -1871,14 +1896,22 @@ int nc_layer_forward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* st
   if (!a->x || !a->w || !a->y || (a->codes && !a->steps)) return fail(-1, "nicecore: NULL x, w, y or steps");
   if (w.total && (!ws || ws_bytes < w.total)) return fail(-1, "nicecore: workspace too small");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (int e = copy_operand(a->dtype, a->x, a->rows, a->inputs, a->x_stride, a->relu != 0, w.x, ws, s, a->codes, a->steps,
-                           a->code_stride))
-    return e;
-  if (int e = copy_operand(a->dtype, a->w, a->outputs, a->inputs, a->w_stride, false, w.w, ws, s)) return e;
-  LowGemm g = layer_gemm(a->dtype, a->x, w.x, a->w, w.w, ws, a->rows, a->outputs, a->inputs);
+  const bool f32 = a->dtype == NC_F32;
+  if (!f32)
+    if (int e = copy_operand(a->dtype, a->x, a->rows, a->inputs, a->x_stride, a->relu != 0, w.a, ws, s, a->codes, a->steps,
+                             a->code_stride))
+      return e;
+  if (int e = copy_operand(a->dtype, a->w, a->outputs, a->inputs, a->w_stride, false, w.b, ws, s)) return e;
+  LowGemm g = layer_gemm(a->dtype, a->x, a->w, w, ws, a->rows, a->outputs, a->inputs);
   g.out = a->y;
   g.ldc = a->y_stride;
   g.bias = a->bias;
+  if (f32) {
+    g.a_relu = a->relu != 0;
+    g.codes = a->codes;
+    g.steps = a->steps;
+    g.code_stride = a->code_stride;
+  }
   return run_low_gemm(g, s);
 }
 
@@ -1895,16 +1928,16 @@ int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* s
   if (a->dx && !a->w) return fail(-1, "nicecore: NULL w");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int64_t nk = a->outputs * a->inputs;
-  if (a->rows == 0) {  // empty sums
-    if (a->dw)
-      if (int e = check_hip(launch_sum_parts(nullptr, nk, 0, a->dw, a->dtype, s), "sum_parts")) return e;
-    if (a->db)
-      if (int e = check_hip(launch_sum_parts(nullptr, a->outputs, 0, a->db, a->dtype, s), "sum_parts")) return e;
-    return 0;
-  }
+  SumParts sum;
+  std::memset(&sum, 0, sizeof(sum));
+  sum.n[0] = nk;
+  sum.n[1] = a->outputs;
+  sum.out[0] = a->dw;
+  sum.out[1] = a->db;
+  if (a->rows == 0) return check_hip(launch_sum_parts(sum, a->dtype, s), "sum_parts");  // empty sums
   if (!ws || ws_bytes < w.total) return fail(-1, "nicecore: workspace too small");
-  if (a->dx || a->dw)
-    if (int e = copy_operand(a->dtype, a->dy, a->rows, a->outputs, a->dy_stride, false, w.dy, ws, s)) return e;
+  if (a->dtype != NC_F32)
+    if (int e = copy_operand(a->dtype, a->dy, a->rows, a->outputs, a->dy_stride, false, w.a, ws, s)) return e;
   if (a->dx) {
     TransposeCtx t;
     t.dtype = a->dtype;
@@ -1912,11 +1945,11 @@ int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* s
     t.cols = a->inputs;
     t.src = a->w;
     t.src_stride = a->w_stride;
-    t.dst = at<uint16_t>(ws, w.wt.at);
-    t.dst_stride = w.wt.stride;
-    t.plane = w.wt.plane;
+    t.dst = at<uint16_t>(ws, w.b.at);
+    t.dst_stride = w.b.stride;
+    t.plane = w.b.plane;
     if (int e = check_hip(timed(KID_CODES, s, [&] { return launch_transpose(t, s); }), "transpose")) return e;
-    LowGemm g = layer_gemm(a->dtype, a->dy, w.dy, nullptr, w.wt, ws, a->rows, a->inputs, a->outputs);
+    LowGemm g = layer_gemm(a->dtype, a->dy, nullptr, w, ws, a->rows, a->inputs, a->outputs);
     g.out = a->dx;
     g.ldc = a->inputs;
     if (a->relu) {
@@ -1925,14 +1958,12 @@ int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* s
     }
     if (int e = run_low_gemm(g, s)) return e;
   }
-  if (a->dw) {
+  if (a->dw || a->db) {
     LowWgrad g;
     std::memset(&g, 0, sizeof(g));
-    g.dy = w.dy.copy ? at<uint16_t>(ws, w.dy.at) : static_cast<const uint16_t*>(a->dy);
-    g.ldy = w.dy.stride;
-    g.plane = w.dy.plane;
-    g.planes = a->dtype == NC_F32 ? 3 : 1;
-    g.f16 = a->dtype == NC_F16;
+    g.dy = w.a.copy ? at<uint16_t>(ws, w.a.at) : a->dy;
+    g.ldy = w.a.copy ? w.a.stride : a->dy_stride;
+    g.dtype = a->dtype;
     g.relu = a->relu != 0;
     g.codes = a->codes;
     g.steps = a->steps;
@@ -1941,18 +1972,23 @@ int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* s
     g.N = a->outputs;
     g.K = a->inputs;
     g.part = at<float>(ws, w.part);
+    g.sums = at<float>(ws, w.sums);
+    g.want_dw = a->dw != nullptr;
+    g.want_db = a->db != nullptr;
+    g.pieces = a->dtype == NC_F32 && a->dw ? 1 : w.pieces;
+    const int32_t db_parts = w.splits * g.pieces;
+    if (w.splits == 1) g.dw = a->dw;
+    if (db_parts == 1) g.db = a->db;
     g.splits = w.splits;
     g.rows_per = w.rows_per;
     if (int e = check_hip(timed(KID_LOW_WGRAD, s, [&] { return launch_low_wgrad(g, s); }), "k_low_wgrad")) return e;
-    if (int e = check_hip(timed(KID_LOW_WGRAD, s, [&] { return launch_sum_parts(g.part, nk, w.splits, a->dw, a->dtype, s); }),
-                          "sum_parts"))
-      return e;
-  }
-  if (a->db) {
-    float* part = at<float>(ws, w.dbpart);
-    if (int e = check_hip(launch_col_sums(a->dy, a->dtype, a->rows, a->outputs, a->dy_stride, w.slices, part, s), "col_sums"))
-      return e;
-    if (int e = check_hip(launch_sum_parts(part, a->outputs, w.slices, a->db, a->dtype, s), "sum_parts")) return e;
+    sum.part[0] = g.part;
+    sum.part[1] = g.sums;
+    sum.parts[0] = w.splits;
+    sum.parts[1] = db_parts;
+    if (g.dw) sum.out[0] = nullptr;
+    if (g.db) sum.out[1] = nullptr;
+    if (int e = check_hip(timed(KID_LOW_WGRAD, s, [&] { return launch_sum_parts(sum, a->dtype, s); }), "sum_parts")) return e;
   }
   return 0;
 }

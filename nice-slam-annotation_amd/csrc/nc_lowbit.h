@@ -1,7 +1,7 @@
 // nc_lowbit.h — the 8-bit layer operators: formats, launch contexts and device helpers.
 //
 // Three code formats (nc_code_format):
-//   NC_CODES_ROW    int8 codes, one float scale per row: s = max(fl(amax / 127), 2^-126),
+//   NC_CODES_ROW    int8 codes, one float scale per row: s = max(fl(amax fl(1 / 127)), 2^-126),
 //                   q = the integer nearest to x / s (ties to even), value = q s.
 //   NC_CODES_GROUP  int8 codes, one byte per 32 neighbouring columns: the step is the power of
 //                   two 2^(byte - 127), the least one with 127 steps >= the group's amax.
@@ -68,10 +68,9 @@ struct LowGemm {
   const uint8_t* A;        // rows of lda bytes: int8 codes or 16-bit elements, 128-byte slices
   const uint8_t* B;
   int64_t lda, ldb;        // bytes
-  int64_t plane_a, plane_b;  // bytes between planes (segments > 1)
+  int64_t plane_b;         // bytes between planes (LOW_F32)
   int64_t M, N;
-  int32_t slices;          // 128-byte slices of a row
-  int32_t segments;        // 1, or 6: the plane pairs of a float product
+  int32_t slices;          // 128-byte slices of a row (LOW_F32: of 32 columns)
   int32_t mode;            // LOW_I8 / LOW_BF16 / LOW_F16
   int32_t out_dtype, bias_dtype, relu;
   void* out;               // [M][ldc] elements
@@ -81,32 +80,59 @@ struct LowGemm {
   const float* col_scale;
   const uint8_t* mask;     // output zeroed where the code [m][n] is 0, or NULL
   int64_t ldm;
+  // LOW_F32: A is float [M][lda / 4] with K columns, split into planes while it is staged (B: three planes,
+  // slices of 32 columns); a_relu: of max(A, 0); codes: its 8-bit checkpoint is written besides
+  int64_t K;
+  int32_t a_relu;
+  uint8_t* codes;
+  uint8_t* steps;
+  int64_t code_stride;
+  // a sum cut into `splits` parts, part[split][M][N] (float, LOW_I8: int32), when the tiles are few
+  int32_t splits;
+  float* part;
 };
-enum LowMode { LOW_I8 = 0, LOW_BF16, LOW_F16 };
+enum LowMode { LOW_I8 = 0, LOW_BF16, LOW_F16, LOW_F32 };
 int launch_low_gemm(const LowGemm& g, hipStream_t s);
+// LOW_I8 for few rows or few columns: x (of x_dtype, [M][x_stride]) encoded within the kernel, or -1: given codes
+struct LowSmall {
+  LowGemm g;               // A: the codes (x_dtype = -1)
+  int32_t x_dtype;
+  const void* x;
+  int64_t x_stride;
+};
+bool low_small_encodes(int64_t M, int64_t N, int64_t K);
+int launch_low_small(const LowSmall& a, hipStream_t s);
+int low_gemm_splits(int mode, int64_t M, int64_t N, int64_t K);
 
 // ---- dW[n][k] = sum_m dY[m][n] value(code[m][k]) --------------------------------------------------
 struct LowWgrad {
-  const uint16_t* dy;      // planes x [M][ldy]: 16-bit elements, rows 16-byte aligned
-  int64_t ldy, plane;      // elements
-  int32_t planes;          // 1 or 3
-  int32_t f16, relu;       // element type (else bfloat16), code format (RELU else GROUP)
+  const void* dy;          // [M][ldy] of dtype; 16-bit rows are 16-byte aligned
+  int64_t ldy;             // elements
+  int32_t dtype, relu;     // nc_dtype; code format (RELU else GROUP)
   const uint8_t* codes;
   const uint8_t* steps;
   int64_t code_stride;
   int64_t M, N, K;
   float* part;             // [splits][N][K]
+  float* sums;             // [splits][pieces][N]: the columns' sums of dY (float with want_dw: pieces = 1)
+  int32_t pieces;
+  void* dw;                // splits = 1: dW itself, of dtype; else NULL
+  void* db;                // one part: the sums themselves; else NULL
+  int32_t want_dw, want_db;
   int32_t splits;
   int64_t rows_per;        // rows of a split, a multiple of 64
 };
 int launch_low_wgrad(const LowWgrad& g, hipStream_t s);
-void low_wgrad_splits(int64_t M, int64_t N, int64_t K, int32_t& splits, int64_t& rows_per);
+void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, int32_t& splits, int32_t& pieces, int64_t& rows_per);
 
-// out[e] = sum_s part[s][e] in order, as dtype
-int launch_sum_parts(const float* part, int64_t n, int32_t splits, void* out, int32_t dtype, hipStream_t s);
-// part[slice][c] = sums of x's columns over a slice of rows
-int launch_col_sums(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t stride, int32_t slices,
-                    float* part, hipStream_t s);
+// out[e] = sum_s part[s][e], in order, as dtype, for two matrices in one launch; out = NULL: none
+struct SumParts {
+  const float* part[2];
+  int64_t n[2];
+  int32_t parts[2];
+  void* out[2];
+};
+int launch_sum_parts(const SumParts& a, int32_t dtype, hipStream_t s);
 
 // ---- device helpers -------------------------------------------------------------------------------
 __device__ __forceinline__ float bf16_f32(uint16_t b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
@@ -121,32 +147,129 @@ __device__ __forceinline__ uint16_t f32_elem(float x) {  // round to nearest eve
   return DT == NC_BF16 ? f32_bf16(x) : __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-// x = p[0] + p[1] + p[2] in bfloat16, each the rounding of what is left: 24 significant bits at
-// least for |x| >= 2^-100.  A finite x whose rounding would overflow is cut instead; an
-// infinity or NaN goes into the first plane alone.
-__device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const uint32_t mag = u & 0x7fffffffu;
-  p[0] = f32_bf16(x);
-  if (mag >= 0x7f7f8000u) {  // would round to infinity, or is not finite
-    const bool nan = mag > 0x7f800000u;
-    p[0] = nan ? 0x7fc0 : (uint16_t)(u >> 16);
-    if (mag >= 0x7f800000u) {
-      p[1] = p[2] = 0;
-      return;
-    }
+__device__ __forceinline__ float relu_keep_nan(float x) { return x < 0.f ? 0.f : x; }
+
+// x = x0 + x1 + x2, exactly, in bfloat16: each plane is what is left cut to its upper half (8 significant
+// bits, 24 in all; the third is whole by then).  Of 8 values: a plane is 4 words.  An infinity or NaN
+// leaves a NaN in the second plane.
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+}
+__device__ __forceinline__ float cut_bf16(float x) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u);
+}
+__device__ __forceinline__ void split3(const float (&x)[8], uint4 (&plane)[3]) {
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = x[e];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    plane[k] = uint4{upper_halves(r[0], r[1]), upper_halves(r[2], r[3]), upper_halves(r[4], r[5]), upper_halves(r[6], r[7])};
+    if (k < 2)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = r[e] - cut_bf16(r[e]);
   }
-  const float r1 = x - bf16_f32(p[0]);
-  p[1] = f32_bf16(r1);
-  p[2] = f32_bf16(r1 - bf16_f32(p[1]));
 }
 
 // biased exponent of a group's step from the bits of its amax (magnitude bits)
 __device__ __forceinline__ int step_byte(uint32_t amax, bool relu) {
-  if (amax >= 0x7f800000u) return 255;
-  int e = (int)((amax + 0x1ffffu) >> 23);  // + 1 when the mantissa is over 127/64
-  e = (e > 254 ? 254 : e) - (relu ? 7 : 6);
-  return e < 1 ? 1 : e;
+  const int e = min((int)((amax + 0x1ffffu) >> 23), 254) - (relu ? 7 : 6);  // + 1 when the mantissa is over 127/64
+  return amax >= 0x7f800000u ? 255 : max(e, 1);
+}
+
+// 8 columns [8 c, 8 c + 8) of a row as float; those behind the last are copies of others (clear8 zeroes them).
+// No branch: what a branch loads is waited for where its sides meet.  VEC: 16-byte aligned rows of a
+// multiple of 8 columns.
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const void* x, int64_t off, int64_t c, int64_t cols, float (&v)[8]) {
+  if (VEC) {
+    const int64_t last = cols / 8 - 1, at = off + 8 * (c < last ? c : last);
+    if (DT == NC_F32) {
+      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + at);
+      const float4 a = p[0], b = p[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + at);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = elem_f32<DT>((uint16_t)w[j]);
+        v[2 * j + 1] = elem_f32<DT>((uint16_t)(w[j] >> 16));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t k = 8 * c + j, at = off + (k < cols ? k : cols - 1);
+      v[j] = DT == NC_F32 ? reinterpret_cast<const float*>(x)[at] : elem_f32<DT>(reinterpret_cast<const uint16_t*>(x)[at]);
+    }
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void clear8(int64_t c, int64_t cols, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (VEC ? 8 * c : 8 * c + j) < cols ? v[j] : 0.f;
+}
+inline bool load8_vec(const void* p, int64_t stride, int64_t cols, int dtype) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * (dtype == NC_F32 ? 4 : 2)) % 16 == 0 && cols % 8 == 0;
+}
+
+__device__ __forceinline__ uint2 pack8(const int (&q)[8]) {
+  uint2 r;
+  r.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | (uint32_t)(q[3] & 255) << 24;
+  r.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | (uint32_t)(q[7] & 255) << 24;
+  return r;
+}
+
+__device__ __forceinline__ uint32_t mag_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+// The code is the integer nearest to the exact quotient x / s: t = rint(x rcp) is at most one off
+// next to a half, and the remainder x - t s (exact in a fused multiply-add there: its grid is half an
+// ulp of s and it is below s) says on which side of s / 2 the quotient lies.
+__device__ __forceinline__ int row_code(float x, float s, float rcp) {
+  float t = __builtin_rintf(x * rcp);
+  const float r = __builtin_fmaf(-t, s, x), h = 0.5f * s;
+  const bool odd = ((int)t & 1) != 0;
+  if (r > h || (r == h && odd)) t += 1.f;
+  else if (r < -h || (r == -h && odd)) t -= 1.f;
+  return (int)__builtin_fminf(__builtin_fmaxf(t, -127.f), 127.f);
+}
+
+// a row's scale from its amax (magnitude bits)
+__device__ __forceinline__ float row_scale(uint32_t top) {
+  return __builtin_fmaxf(__builtin_bit_cast(float, top) * (1.f / 127.f), 0x1p-126f);
+}
+__device__ __forceinline__ uint2 row_codes(const float (&v)[8], bool bad, float s, float rcp) {
+  int q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] = bad ? 0 : row_code(v[e], s, rcp);
+  return pack8(q);
+}
+
+// the codes of 8 columns and the step byte of their group, whose other columns the three lanes beside
+// (lane ^ 1, 2, 3) hold
+template <bool RELU>
+__device__ __forceinline__ uint2 group_codes(const float (&v)[8], int& sb) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {  // RELU: x <= 0 counts as 0 (a NaN does not)
+    const uint32_t m = mag_bits(v[e]);
+    top = max(top, RELU && v[e] <= 0.f ? 0u : m);
+  }
+  top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true));  // lane ^ 1
+  top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4e, 0xf, 0xf, true));  // lane ^ 2
+  sb = step_byte(top, RELU);
+  const float inv = __builtin_bit_cast(float, (uint32_t)(254 - min(sb, 253)) << 23);
+  int q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = __builtin_rintf(v[e] * inv);
+    const float c = __builtin_fminf(__builtin_fmaxf(t, RELU ? 0.f : -127.f), RELU ? 254.f : 127.f);
+    const int k = sb == 255 ? 0 : (int)c;
+    q[e] = RELU ? (v[e] <= 0.f ? 0 : 1 + k) : k;
+  }
+  return pack8(q);
 }
 
 }  // namespace nc

@@ -8,36 +8,6 @@ namespace nc {
 
 static inline unsigned blocks_of(int64_t n, int b) { return (unsigned)((n + b - 1) / b); }
 
-// 8 columns [8 c, 8 c + 8) of a row as float, 0 behind the last one
-template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const void* x, int64_t off, int64_t c, int64_t cols, float (&v)[8]) {
-  if (DT == NC_F32) {
-    const float* p = reinterpret_cast<const float*>(x) + off + 8 * c;
-    if (VEC && 8 * c + 8 <= cols) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 8 * c + j < cols ? p[j] : 0.f;
-    }
-  } else {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(x) + off + 8 * c;
-    if (VEC && 8 * c + 8 <= cols) {
-      const uint4 a = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = elem_f32<DT>((uint16_t)w[j]);
-        v[2 * j + 1] = elem_f32<DT>((uint16_t)(w[j] >> 16));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 8 * c + j < cols ? elem_f32<DT>(p[j]) : 0.f;
-    }
-  }
-}
-
 template <int DT, bool VEC>
 __device__ __forceinline__ void store8(void* x, int64_t off, int64_t c, int64_t cols, const float (&v)[8]) {
   if (DT == NC_F32) {
@@ -70,29 +40,36 @@ __device__ __forceinline__ void store8(void* x, int64_t off, int64_t c, int64_t 
   }
 }
 
-__device__ __forceinline__ uint2 pack8(const int (&q)[8]) {
-  uint2 r;
-  r.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | (uint32_t)(q[3] & 255) << 24;
-  r.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | (uint32_t)(q[7] & 255) << 24;
-  return r;
-}
-
 // ---- rows with one scale ---------------------------------------------------------------------------
-// The code is the integer nearest to the exact quotient x / s: t = rint(x rcp) is at most one off
-// next to a half, and the remainder x - t s (exact in a fused multiply-add there: its grid is half an
-// ulp of s and it is below s) says on which side of s / 2 the quotient lies.
-__device__ __forceinline__ int row_code(float x, float s, float rcp) {
-  float t = __builtin_rintf(x * rcp);
-  const float r = __builtin_fmaf(-t, s, x), h = 0.5f * s;
-  const bool odd = ((int)t & 1) != 0;
-  if (r > h || (r == h && odd)) t += 1.f;
-  else if (r < -h || (r == -h && odd)) t -= 1.f;
-  return (int)__builtin_fminf(__builtin_fmaxf(t, -127.f), 127.f);
+// Rows of up to 512 columns: LPR lanes (16, 32 or 64) own a row, R rows each, all loads first.
+template <int DT, bool VEC, int LPR, int R>
+__global__ void __launch_bounds__(256) k_encode_short_rows(const CodeCtx a) {
+  const int c = threadIdx.x % LPR;
+  const int64_t r0 = ((int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR) * R, chunks = a.code_stride / 8;
+  float v[R][8];
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int64_t r = r0 + j < a.rows ? r0 + j : a.rows - 1;
+    load8<DT, VEC>(a.x, r * a.x_stride, c, a.cols, v[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    uint32_t top = 0;
+    clear8<VEC>(c, a.cols, v[j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, mag_bits(v[j][e]));
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    const bool bad = top >= 0x7f800000u;
+    const float s = row_scale(top);
+    const uint2 w = row_codes(v[j], bad, s, 1.f / s);
+    if (r0 + j >= a.rows) continue;
+    if (c == 0) reinterpret_cast<float*>(a.scales)[r0 + j] = bad ? __builtin_nanf("") : s;
+    if (c < chunks) reinterpret_cast<uint2*>(a.codes + (r0 + j) * a.code_stride)[c] = w;
+  }
 }
 
-__device__ __forceinline__ uint32_t mag_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
-
-// NT threads (64 or 1024) own a row; C > 0: its 8-column chunks t, t + NT, ... stay in registers
+// NT threads (64, 256 or 1024) own a row; C > 0: its 8-column chunks t, t + NT, ... stay in registers
 // (C of them a thread), C = 0: any length, read twice (the second time from the cache).
 template <int DT, bool VEC, int NT, int C>
 __global__ void __launch_bounds__(NT == 64 ? 256 : NT) k_encode_rows(const CodeCtx a) {
@@ -108,16 +85,18 @@ __global__ void __launch_bounds__(NT == 64 ? 256 : NT) k_encode_rows(const CodeC
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const int64_t c = t + (int64_t)NT * j;
-      if (c < chunks) load8<DT, VEC>(a.x, off, c, a.cols, v[j]);
-      else
+      load8<DT, VEC>(a.x, off, c, a.cols, v[j]);
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
+    for (int j = 0; j < C; ++j) {
+      clear8<VEC>(t + (int64_t)NT * j, a.cols, v[j]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = max(top, mag_bits(v[j][e]));
     }
   } else {
     for (int64_t c = t; 8 * c < a.cols; c += NT) {
       load8<DT, VEC>(a.x, off, c, a.cols, v[0]);
+      clear8<VEC>(c, a.cols, v[0]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = max(top, mag_bits(v[0][e]));
     }
@@ -132,7 +111,7 @@ __global__ void __launch_bounds__(NT == 64 ? 256 : NT) k_encode_rows(const CodeC
     for (int w = 1; w < NT / 64; ++w) top = max(top, red[w]);
   }
   const bool bad = top >= 0x7f800000u;
-  const float s = __builtin_fmaxf(__builtin_bit_cast(float, top) / 127.f, 0x1p-126f);
+  const float s = row_scale(top);
   const float rcp = 1.f / s;
   if (t == 0) reinterpret_cast<float*>(a.scales)[r] = bad ? __builtin_nanf("") : s;
   uint2* out = reinterpret_cast<uint2*>(a.codes + r * a.code_stride);
@@ -141,18 +120,13 @@ __global__ void __launch_bounds__(NT == 64 ? 256 : NT) k_encode_rows(const CodeC
     for (int j = 0; j < C; ++j) {
       const int64_t c = t + (int64_t)NT * j;
       if (c >= chunks) break;
-      int q[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = bad ? 0 : row_code(v[j][e], s, rcp);
-      out[c] = pack8(q);
+      out[c] = row_codes(v[j], bad, s, rcp);
     }
   } else {
     for (int64_t c = t; c < chunks; c += NT) {
       load8<DT, VEC>(a.x, off, c, a.cols, v[0]);
-      int q[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = bad ? 0 : row_code(v[0][e], s, rcp);
-      out[c] = pack8(q);
+      clear8<VEC>(c, a.cols, v[0]);
+      out[c] = row_codes(v[0], bad, s, rcp);
     }
   }
 }
@@ -168,54 +142,28 @@ __global__ void __launch_bounds__(256) k_encode_groups(const CodeCtx a, int64_t 
   const int64_t r = id / row_chunks, c = id - r * row_chunks;
   float v[8];
   load8<DT, VEC>(a.x, r * a.x_stride, c, a.cols, v);
+  clear8<VEC>(c, a.cols, v);
   constexpr bool RELU = FMT == NC_CODES_RELU;
   if (FMT >= 0) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t m = mag_bits(v[e]);
-      top = max(top, RELU && !(v[e] > 0.f) && !(v[e] != v[e]) ? 0u : m);
-    }
-    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
-    const int sb = step_byte(top, RELU);
-    const float inv = __builtin_bit_cast(float, (uint32_t)(254 - (sb < 254 ? sb : 253)) << 23);
-    int q[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float t = __builtin_rintf(v[e] * inv);
-      if (RELU) {
-        const int k = sb == 255 ? 0 : (int)__builtin_fminf(__builtin_fmaxf(t, 0.f), 254.f);
-        q[e] = v[e] > 0.f || v[e] != v[e] ? 1 + k : 0;
-      } else {
-        q[e] = sb == 255 ? 0 : (int)__builtin_fminf(__builtin_fmaxf(t, -127.f), 127.f);
-      }
-    }
+    int sb;
+    const uint2 w = group_codes<RELU>(v, sb);
     if (8 * c < a.code_stride) {
-      *reinterpret_cast<uint2*>(a.codes + r * a.code_stride + 8 * c) = pack8(q);
+      *reinterpret_cast<uint2*>(a.codes + r * a.code_stride + 8 * c) = w;
       if ((c & 3) == 0) reinterpret_cast<uint8_t*>(a.scales)[r * (a.code_stride / CODE_GROUP) + (c >> 2)] = (uint8_t)sb;
     }
   }
   if (OUT > 0 && 8 * c < a.copy_stride) {
     if (a.relu) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = v[e] > 0.f || v[e] != v[e] ? v[e] : 0.f;
+      for (int e = 0; e < 8; ++e) v[e] = relu_keep_nan(v[e]);
     }
     if (OUT == 1) {
       store8<DT == NC_F32 ? NC_BF16 : DT, true>(a.copy, r * a.copy_stride, c, a.copy_stride, v);  // exact: v is of that type
     } else {
-      uint16_t p[8][3];
+      uint4 p[3];
+      split3(v, p);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) split3(v[e], p[e]);
-#pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        uint4 w;
-        w.x = p[0][k] | (uint32_t)p[1][k] << 16;
-        w.y = p[2][k] | (uint32_t)p[3][k] << 16;
-        w.z = p[4][k] | (uint32_t)p[5][k] << 16;
-        w.w = p[6][k] | (uint32_t)p[7][k] << 16;
-        *reinterpret_cast<uint4*>(a.copy + k * a.plane + r * a.copy_stride + 8 * c) = w;
-      }
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(a.copy + k * a.plane + r * a.copy_stride + 8 * c) = p[k];
     }
   }
 }
@@ -263,52 +211,39 @@ __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
     const int64_t r = r0 + rr, c = c0 + cc;
     if (c >= a.cols) continue;  // r < dst_stride: whole tiles of 64
     uint16_t* d = a.dst + c * a.dst_stride + r;
-    if (DT == NC_F32) {
-      uint16_t p[3];
-      split3(tile[rr][cc], p);
-      d[0] = p[0];
-      d[a.plane] = p[1];
-      d[2 * a.plane] = p[2];
+    float x = tile[rr][cc];
+    if (DT == NC_F32) {  // split3, one value
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        d[k * a.plane] = (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16);
+        x = x - cut_bf16(x);
+      }
     } else {
-      d[0] = f32_elem<DT>(tile[rr][cc]);
+      d[0] = f32_elem<DT>(x);
     }
   }
 }
 
 // ---- sums in a fixed order ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) k_sum_parts(const float* part, int64_t n, int32_t splits, void* out, int32_t dtype) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// V neighbouring elements a thread
+template <int DT, int V>
+__global__ void __launch_bounds__(256) k_sum_parts(const SumParts a, unsigned first_blocks) {
+  const int w = blockIdx.x >= first_blocks ? 1 : 0;
+  const int64_t n = a.n[w], e = ((int64_t)(blockIdx.x - (w ? first_blocks : 0)) * 256 + threadIdx.x) * V;
   if (e >= n) return;
-  float t = 0.f;
-  for (int k = 0; k < splits; ++k) t += part[k * n + e];
-  if (dtype == NC_F32) reinterpret_cast<float*>(out)[e] = t;
-  else reinterpret_cast<uint16_t*>(out)[e] = dtype == NC_BF16 ? f32_elem<NC_BF16>(t) : f32_elem<NC_F16>(t);
-}
-
-// 64 columns x 4 row lanes; a slice's rows in four interleaved float sums, then those
-template <int DT>
-__global__ void __launch_bounds__(256) k_col_sums(const void* x, int64_t rows, int64_t cols, int64_t stride, int64_t per,
-                                                  float* part) {
-  __shared__ float red[4][64];
-  const int cl = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + cl;
-  const int64_t rb = (int64_t)blockIdx.y * per, re = rb + per < rows ? rb + per : rows;
-  float t[4] = {0.f, 0.f, 0.f, 0.f};
-  if (c < cols) {
-    auto at = [&](int64_t r) {
-      return DT == NC_F32 ? reinterpret_cast<const float*>(x)[r * stride + c]
-                          : elem_f32<DT>(reinterpret_cast<const uint16_t*>(x)[r * stride + c]);
-    };
-    int64_t r = rb + w;
-    for (; r + 12 < re; r += 16) {
+  typedef float floatv __attribute__((ext_vector_type(V)));
+  floatv t = 0.f;
+  const float* p = a.part[w] + e;
+  for (int k = 0; k < a.parts[w]; ++k, p += n) t += *reinterpret_cast<const floatv*>(p);
+  if (DT == NC_F32) {
+    *reinterpret_cast<floatv*>(reinterpret_cast<float*>(a.out[w]) + e) = t;
+  } else {
+    typedef uint16_t shortv __attribute__((ext_vector_type(V)));
+    shortv o;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) t[u] += at(r + 4 * u);
-    }
-    for (; r < re; r += 4) t[0] += at(r);
+    for (int j = 0; j < V; ++j) o[j] = f32_elem<DT>(t[j]);
+    *reinterpret_cast<shortv*>(reinterpret_cast<uint16_t*>(a.out[w]) + e) = o;
   }
-  red[w][cl] = (t[0] + t[1]) + (t[2] + t[3]);
-  __syncthreads();
-  if (w == 0 && c < cols) part[blockIdx.y * cols + c] = (red[0][cl] + red[1][cl]) + (red[2][cl] + red[3][cl]);
 }
 
 // ---- launchers ---------------------------------------------------------------------------------------
@@ -319,11 +254,27 @@ static bool vec_rows(const void* p, int64_t stride, int dtype) {
 
 template <int DT, bool VEC>
 static int encode_rows(const CodeCtx& c, hipStream_t s) {
+  // A wave a row needs no barrier (16384 x 4096 bfloat16: 49 us; 79 us with 1024 threads a row); few rows get
+  // 256 threads each for a shorter way through a row.  Short rows go several to a wave, so that enough
+  // loads are in flight.
   const int64_t k = c.code_stride;
-  const dim3 waves(blocks_of(c.rows, 4)), rows((unsigned)c.rows);
-  if (k <= 512) hipLaunchKernelGGL((k_encode_rows<DT, VEC, 64, 1>), waves, dim3(256), 0, s, c);
-  else if (k <= 1024) hipLaunchKernelGGL((k_encode_rows<DT, VEC, 64, 2>), waves, dim3(256), 0, s, c);
-  else if (k <= 8192) hipLaunchKernelGGL((k_encode_rows<DT, VEC, 1024, 1>), rows, dim3(1024), 0, s, c);
+  const bool few = c.rows < 512;
+  const dim3 waves(blocks_of(c.rows, 4)), rows((unsigned)c.rows), b(256);
+  if (k <= 128) {
+    if (few) hipLaunchKernelGGL((k_encode_short_rows<DT, VEC, 16, 1>), dim3(blocks_of(c.rows, 16)), b, 0, s, c);
+    else hipLaunchKernelGGL((k_encode_short_rows<DT, VEC, 16, 4>), dim3(blocks_of(c.rows, 64)), b, 0, s, c);
+  } else if (k <= 256) {
+    if (few) hipLaunchKernelGGL((k_encode_short_rows<DT, VEC, 32, 1>), dim3(blocks_of(c.rows, 8)), b, 0, s, c);
+    else hipLaunchKernelGGL((k_encode_short_rows<DT, VEC, 32, 4>), dim3(blocks_of(c.rows, 32)), b, 0, s, c);
+  } else if (k <= 512) {
+    if (few) hipLaunchKernelGGL((k_encode_short_rows<DT, VEC, 64, 1>), dim3(blocks_of(c.rows, 4)), b, 0, s, c);
+    else hipLaunchKernelGGL((k_encode_short_rows<DT, VEC, 64, 4>), dim3(blocks_of(c.rows, 16)), b, 0, s, c);
+  }
+  else if (k <= 1024 && !few) hipLaunchKernelGGL((k_encode_rows<DT, VEC, 64, 2>), waves, dim3(256), 0, s, c);
+  else if (k <= 2048 && few) hipLaunchKernelGGL((k_encode_rows<DT, VEC, 256, 1>), rows, dim3(256), 0, s, c);
+  else if (k <= 2048) hipLaunchKernelGGL((k_encode_rows<DT, VEC, 64, 4>), waves, dim3(256), 0, s, c);
+  else if (k <= 4096 && !few) hipLaunchKernelGGL((k_encode_rows<DT, VEC, 64, 8>), waves, dim3(256), 0, s, c);
+  else if (k <= 8192) hipLaunchKernelGGL((k_encode_rows<DT, VEC, 256, 4>), rows, dim3(256), 0, s, c);
   else hipLaunchKernelGGL((k_encode_rows<DT, VEC, 1024, 0>), rows, dim3(1024), 0, s, c);
   return (int)hipGetLastError();
 }
@@ -354,7 +305,7 @@ static int encode(const CodeCtx& c, hipStream_t s) {
 
 int launch_encode(const CodeCtx& c, hipStream_t s) {
   if (c.rows <= 0) return 0;
-  const bool v = vec_rows(c.x, c.x_stride, c.dtype);
+  const bool v = load8_vec(c.x, c.x_stride, c.cols, c.dtype);
   switch (c.dtype) {
     case NC_F32: return v ? encode<NC_F32, true>(c, s) : encode<NC_F32, false>(c, s);
     case NC_F16: return v ? encode<NC_F16, true>(c, s) : encode<NC_F16, false>(c, s);
@@ -398,24 +349,29 @@ int launch_transpose(const TransposeCtx& c, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
-int launch_sum_parts(const float* part, int64_t n, int32_t splits, void* out, int32_t dtype, hipStream_t s) {
-  if (n <= 0) return 0;
-  hipLaunchKernelGGL(k_sum_parts, dim3(blocks_of(n, 256)), dim3(256), 0, s, part, n, splits, out, dtype);
+template <int DT>
+static int sum_parts(const SumParts& a, hipStream_t s) {
+  int64_t n[2];
+  bool vec = true;
+  for (int w = 0; w < 2; ++w) {
+    n[w] = a.out[w] ? a.n[w] : 0;
+    vec = vec && n[w] % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.out[w]) | reinterpret_cast<uintptr_t>(a.part[w])) & 15) == 0;
+  }
+  const int per = vec ? 1024 : 256;
+  const unsigned first = blocks_of(n[0], per), all = first + blocks_of(n[1], per);
+  if (all == 0) return 0;
+  if (vec) hipLaunchKernelGGL((k_sum_parts<DT, 4>), dim3(all), dim3(256), 0, s, a, first);
+  else hipLaunchKernelGGL((k_sum_parts<DT, 1>), dim3(all), dim3(256), 0, s, a, first);
   return (int)hipGetLastError();
 }
 
-int launch_col_sums(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t stride, int32_t slices,
-                    float* part, hipStream_t s) {
-  if (cols <= 0 || slices <= 0) return 0;
-  const int64_t per = (rows + slices - 1) / slices;
-  const dim3 g(blocks_of(cols, 64), (unsigned)slices);
+int launch_sum_parts(const SumParts& a, int32_t dtype, hipStream_t s) {
   switch (dtype) {
-    case NC_F32: hipLaunchKernelGGL((k_col_sums<NC_F32>), g, dim3(256), 0, s, x, rows, cols, stride, per, part); break;
-    case NC_F16: hipLaunchKernelGGL((k_col_sums<NC_F16>), g, dim3(256), 0, s, x, rows, cols, stride, per, part); break;
-    case NC_BF16: hipLaunchKernelGGL((k_col_sums<NC_BF16>), g, dim3(256), 0, s, x, rows, cols, stride, per, part); break;
-    default: return (int)hipErrorInvalidValue;
+    case NC_F32: return sum_parts<NC_F32>(a, s);
+    case NC_F16: return sum_parts<NC_F16>(a, s);
+    case NC_BF16: return sum_parts<NC_BF16>(a, s);
   }
-  return (int)hipGetLastError();
+  return (int)hipErrorInvalidValue;
 }
 
 }  // namespace nc

@@ -1,18 +1,19 @@
 // nc_lowgemm.hip — the matrix products of the 8-bit layer operators on the gfx950 matrix cores.
 //
 // k_low_gemm    C[m][n] = sum_k A[m][k] B[n][k]: int8 codes (v_mfma_i32_16x16x64_i8, exact sums) or
-//               16-bit elements (v_mfma_f32_16x16x32_bf16 / _f16, float sums).  A float product is six
-//               products of bfloat16 planes (split3: x = x0 + x1 + x2): x0 y0 + x0 y1 + x1 y0 + x0 y2 +
-//               x1 y1 + x2 y0; what is left out is below 2^-25 of |x y|.
+//               16-bit elements (v_mfma_f32_16x16x32_bf16 / _f16, float sums).
+// k_low_gemm_f  the same for float A: six products of bfloat16 planes (split3: x = x0 + x1 + x2),
+//               x0 y0 + x0 y1 + x1 y0 + x0 y2 + x1 y1 + x2 y0; what is left out is below 2^-22 of |x y|,
+//               2^-24.5 on average.
+//               A is split while it is staged, and its 8-bit checkpoint written besides.
 // k_low_wgrad   dW[n][k] = sum_m dY[m][n] V[m][k], V the values of an 8-bit checkpoint, decoded while a
 //               tile is staged (a code times a power of two is exact in 16 bits), both operands
 //               read transposed from LDS (ds_read_b64_tr_b16).
+#include <atomic>
+
 #include "nc_lowbit.h"
 
 namespace nc {
-
-#define NC_GLOBAL(p) ((const __attribute__((address_space(1))) void*)(p))
-#define NC_LDS(p) ((__attribute__((address_space(3))) void*)(p))
 
 // every matrix result is read by vector instructions next: wait states for the longest of the
 // instructions used here (see mfma16_drain in nc_device.h for the shortest count that held)
@@ -22,11 +23,33 @@ __device__ __forceinline__ void matrix_drain() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// loads into LDS are counted as memory loads of the wave that issued them: each wave waits for its
-// own before the barrier
+// 16 bytes a lane from base + offset into LDS at `to` + 16 lane (wave-uniform).  Written as an
+// instruction of its own because the compiler, which cannot tell the two halves of the double buffer
+// apart, would wait for every such load before the next LDS read; it has no result register, and
+// the kernels wait for it (vmcnt) before the barrier after which its bytes are read.
+__device__ __forceinline__ void load_lds16(const void* base, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void load_lds4(const void* base, uint32_t offset, uint32_t to) {  // 4 bytes a lane
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+// waits until at most N of the wave's vector memory loads are in flight
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ void staged_barrier() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  wait_loads<0>();
   __syncthreads();
+}
+// a barrier for LDS alone: __syncthreads() would also wait for every store in flight
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 // workgroups to tiles: those that the hardware deals to one chiplet (w mod 8) take a run of
@@ -46,6 +69,7 @@ struct Mac;
 template <>
 struct Mac<LOW_I8> {
   typedef intx4 Acc;
+  typedef int Elem;
   static __device__ __forceinline__ Acc zero() { return intx4{0, 0, 0, 0}; }
   static __device__ __forceinline__ Acc mac(uint4 a, uint4 b, Acc c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(intx4, a), __builtin_bit_cast(intx4, b), c, 0, 0, 0);
@@ -54,6 +78,7 @@ struct Mac<LOW_I8> {
 template <>
 struct Mac<LOW_BF16> {
   typedef floatx4 Acc;
+  typedef float Elem;
   static __device__ __forceinline__ Acc zero() { return zero4(); }
   static __device__ __forceinline__ Acc mac(uint4 a, uint4 b, Acc c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -62,6 +87,7 @@ struct Mac<LOW_BF16> {
 template <>
 struct Mac<LOW_F16> {
   typedef floatx4 Acc;
+  typedef float Elem;
   static __device__ __forceinline__ Acc zero() { return zero4(); }
   static __device__ __forceinline__ Acc mac(uint4 a, uint4 b, Acc c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
@@ -74,39 +100,162 @@ __device__ __forceinline__ float load_bias(const void* b, int dtype, int64_t n) 
   return dtype == NC_BF16 ? elem_f32<NC_BF16>(e) : elem_f32<NC_F16>(e);
 }
 
-// 4 neighbouring outputs [m][n .. n + 3]
-__device__ __forceinline__ void store4(const LowGemm& g, int64_t m, int64_t n, const float (&v)[4]) {
-  const bool whole = n + 4 <= g.N;
-  if (g.out_dtype == NC_F32) {
+// 4 neighbouring outputs [m][n .. n + 3]; vec: rows and columns allow one store
+template <int DT>
+__device__ __forceinline__ void store4(const LowGemm& g, bool vec, int64_t m, int64_t n, const float (&v)[4]) {
+  if (DT == NC_F32) {
     float* p = reinterpret_cast<float*>(g.out) + m * g.ldc + n;
-    if (whole && (reinterpret_cast<uintptr_t>(p) & 15) == 0) *reinterpret_cast<float4*>(p) = float4{v[0], v[1], v[2], v[3]};
-    else
+    if (vec) {
+      *reinterpret_cast<float4*>(p) = float4{v[0], v[1], v[2], v[3]};
+    } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (n + j < g.N) p[j] = v[j];
+    }
   } else {
     uint16_t* p = reinterpret_cast<uint16_t*>(g.out) + m * g.ldc + n;
     uint16_t e[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) e[j] = g.out_dtype == NC_BF16 ? f32_elem<NC_BF16>(v[j]) : f32_elem<NC_F16>(v[j]);
-    if (whole && (reinterpret_cast<uintptr_t>(p) & 7) == 0)
+    for (int j = 0; j < 4; ++j) e[j] = f32_elem<DT>(v[j]);
+    if (vec) {
       *reinterpret_cast<uint2*>(p) = uint2{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16};
-    else
+    } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (n + j < g.N) p[j] = e[j];
+    }
   }
+}
+template <int DT>
+__device__ __forceinline__ bool store4_vec(const LowGemm& g) {
+  const int b = DT == NC_F32 ? 16 : 8;
+  return g.N % 4 == 0 && g.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(g.out) & (b - 1)) == 0;
+}
+
+// one column's result of a sum
+template <int MODE>
+__device__ __forceinline__ float finish(const LowGemm& g, float x, float scale, float bias, uint32_t code) {
+  if (MODE == LOW_I8) x = x * scale;
+  if (g.bias) x += bias;
+  if (g.relu) x = relu_keep_nan(x);
+  if (MODE != LOW_I8 && code == 0) x = 0.f;
+  return x;
+}
+
+// A wave's FM x FN blocks of sums at [m0][n0]: 16 rows at a time through its own piece of LDS (cw,
+// 16 (64 FN + 16) bytes), so that they leave in whole lines.  Everything that the epilogue reads is read
+// first: a store counts as a memory access in flight like a load, so a load behind stores waits for
+// them.  Rows and columns behind the last read the last's.
+template <int MODE, int DT, int FM, int FN, typename Acc>
+__device__ __forceinline__ void store_tile(const LowGemm& g, unsigned char* cw, int lane, const Acc (&acc)[FM][FN], int64_t m0,
+                                           int64_t n0) {
+  constexpr int CROW = 64 * FN + 16;               // bytes of a row, padded
+  constexpr int LPR = 4 * FN, RPI = 64 / LPR;      // lanes a row, rows at once
+  const int i = lane & 15, q = lane >> 4;
+  const int64_t n = n0 + 4 * (lane % LPR);
+  float* part = g.splits > 1 ? g.part + (int64_t)blockIdx.y * g.M * g.N : nullptr;
+  const bool vec = store4_vec<DT>(g);
+  float cs[4], cb[4];
+  float rs[MODE == LOW_I8 ? FM : 1][16 / RPI];
+  uint32_t mask[FM][16 / RPI];
+  if (!part) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t nn = n + j < g.N ? n + j : g.N - 1;
+      cs[j] = MODE == LOW_I8 ? g.col_scale[nn] : 1.f;
+      cb[j] = g.bias ? load_bias(g.bias, g.bias_dtype, nn) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < FM; ++u)
+#pragma unroll
+      for (int k = 0; k < 16 / RPI; ++k) {
+        const int64_t m = m0 + 16 * u + k * RPI + lane / LPR, mm = m < g.M ? m : g.M - 1;
+        if (MODE == LOW_I8) rs[u][k] = g.row_scale[mm];
+        else mask[u][k] = g.mask ? *reinterpret_cast<const uint32_t*>(g.mask + mm * g.ldm + (n < g.ldm ? n : 0)) : ~0u;
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < FM; ++u) {
+#pragma unroll
+    for (int v = 0; v < FN; ++v) *reinterpret_cast<Acc*>(cw + i * CROW + 64 * v + 16 * q) = acc[u][v];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int k = 0; k < 16 / RPI; ++k) {
+      const int r = k * RPI + lane / LPR;
+      const int64_t m = m0 + 16 * u + r;
+      const Acc c = *reinterpret_cast<const Acc*>(cw + r * CROW + 16 * (lane % LPR));
+      if (m >= g.M || n >= g.N) continue;
+      if (part) {
+        float* p = part + m * g.N + n;
+        if (g.N % 4 == 0) {
+          *reinterpret_cast<Acc*>(p) = c;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < g.N) reinterpret_cast<typename Mac<MODE>::Elem*>(p)[j] = c[j];
+        }
+      } else {
+        float o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          o[j] = finish<MODE>(g, (float)c[j], MODE == LOW_I8 ? rs[u][k] * cs[j] : 1.f, cb[j], (mask[u][k] >> (8 * j)) & 255u);
+        store4<DT>(g, vec, m, n, o);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// the parts of a cut sum, in order, and the epilogue: 4 neighbouring columns a thread
+template <int MODE, int DT>
+__global__ void __launch_bounds__(256) k_low_finish(const LowGemm g, int64_t quads) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= g.M * quads) return;
+  const int64_t m = id / quads, n = 4 * (id - m * quads);
+  float o[4], cs[4], cb[4];
+  const float rs = MODE == LOW_I8 ? g.row_scale[m] : 1.f;
+  const uint32_t mask = MODE != LOW_I8 && g.mask ? *reinterpret_cast<const uint32_t*>(g.mask + m * g.ldm + n) : ~0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t nn = n + j < g.N ? n + j : g.N - 1;
+    cs[j] = MODE == LOW_I8 ? g.col_scale[nn] * rs : 1.f;
+    cb[j] = g.bias ? load_bias(g.bias, g.bias_dtype, nn) : 0.f;
+  }
+  typedef Mac<MODE == LOW_I8 ? LOW_I8 : LOW_BF16> M;
+  typedef typename M::Acc Acc;
+  Acc t = M::zero();
+  const float* p = g.part + m * g.N + n;
+  for (int k = 0; k < g.splits; ++k, p += g.M * g.N) {
+    if (g.N % 4 == 0) {
+      t += *reinterpret_cast<const Acc*>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < g.N) t[j] += reinterpret_cast<const typename M::Elem*>(p)[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = finish<MODE>(g, (float)t[j], cs[j], cb[j], (mask >> (8 * j)) & 255u);
+  store4<DT>(g, store4_vec<DT>(g), m, n, o);
 }
 
 // BM x BN tile, WM x WN waves, each (BM / WM) x (BN / WN) in blocks of 16 x 16.  The instruction
 // takes B's rows as its first operand: lane (i, q) then holds, for row m = i of the block, the four
 // neighbouring columns n = 4 q + 0..3.
-template <int MODE, int BM, int BN, int WM, int WN>
+// A slice is worked off in phases of 4 x FN blocks; while a phase multiplies, the next one's operands
+// are read from LDS.  Before the last phase a barrier says that the slice is read and the next one
+// has arrived; the slice after that goes into the freed half then, a whole slice ahead of its use.
+template <int MODE, int DT, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int64_t mt, int64_t nt) {
   constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int STAGE = (BM + BN) * SLICE;
   constexpr int LA = BM / 8 / W, LB = BN / 8 / W;  // 8-row loads a wave
-  static_assert(BM % (8 * W) == 0 && BN % (8 * W) == 0, "whole loads a wave");
+  constexpr int NG = FM / 4, PH = 2 * NG;          // phases of a slice
+  constexpr int CROW = 64 * FN + 16;               // bytes of a row of the epilogue's block, padded
+  static_assert(BM % (8 * W) == 0 && BN % (8 * W) == 0 && FM % 4 == 0, "whole loads a wave, whole phases");
+  static_assert(W * 16 * CROW <= 2 * STAGE, "the epilogue's blocks fit the buffers");
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
@@ -129,22 +278,21 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
   }
   const uint8_t* A = g.A + m0 * g.lda;
   const uint8_t* B = g.B + n0 * g.ldb;
-  const int total = g.slices * g.segments;
-  auto stage = [&](int t) {
-    unsigned char* s = lds + (t & 1) * STAGE;
-    int sl = t, seg = 0;
-    while (sl >= g.slices) { sl -= g.slices; ++seg; }
-    // plane pairs, the largest product last: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
-    const int pa = g.segments > 1 ? (0x001012 >> (4 * seg)) & 3 : 0;
-    const int pb = g.segments > 1 ? (0x010210 >> (4 * seg)) & 3 : 0;
-    const uint8_t* a = A + pa * g.plane_a + (int64_t)sl * SLICE;
-    const uint8_t* b = B + pb * g.plane_b + (int64_t)sl * SLICE;
+  const int first = (int)((int64_t)g.slices * blockIdx.y / g.splits);  // this part's slices
+  const int total = (int)((int64_t)g.slices * (blockIdx.y + 1) / g.splits) - first;
+  const uint32_t lds0 = lds_address(lds);
+  const uint8_t* a_next = A + (int64_t)first * SLICE;  // of the next stage() call
+  const uint8_t* b_next = B + (int64_t)first * SLICE;
+  auto stage = [&](int half) {
+    const uint8_t* a = a_next;
+    const uint8_t* b = b_next;
+    a_next += SLICE;
+    b_next += SLICE;
+    const uint32_t s = lds0 + half * STAGE;
 #pragma unroll
-    for (int j = 0; j < LA; ++j)
-      __builtin_amdgcn_global_load_lds(NC_GLOBAL(a + oa[j]), NC_LDS(s + (wave * LA + j) * 1024), 16, 0, 0);
+    for (int j = 0; j < LA; ++j) load_lds16(a, oa[j], s + (wave * LA + j) * 1024);
 #pragma unroll
-    for (int j = 0; j < LB; ++j)
-      __builtin_amdgcn_global_load_lds(NC_GLOBAL(b + ob[j]), NC_LDS(s + BM * SLICE + (wave * LB + j) * 1024), 16, 0, 0);
+    for (int j = 0; j < LB; ++j) load_lds16(b, ob[j], s + BM * SLICE + (wave * LB + j) * 1024);
   };
   typename Mac<MODE>::Acc acc[FM][FN];
 #pragma unroll
@@ -152,68 +300,651 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 #pragma unroll
     for (int v = 0; v < FN; ++v) acc[u][v] = Mac<MODE>::zero();
   const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
-  const int c0 = 16 * swz(i, q), c1 = 16 * swz(i, 4 + q);  // wm, wn and 16 u leave the swizzle as it is
+  // wm, wn and 16 u leave the swizzle as it is
+  const unsigned char* fa = lds + (wm + i) * SLICE + 16 * swz(i, q);
+  const unsigned char* fb = lds + BM * SLICE + (wn + i) * SLICE + 16 * swz(i, q);
+  const int other = 16 * swz(i, 4 + q) - 16 * swz(i, q);  // to the slice's second half
+  uint4 a[2][4], b[2][FN];
+  auto read = [&](int half, int p) {  // phase p's operands of the slice in `half`
+    const int h = p / NG, gr = p % NG;
+    const unsigned char* pa = fa + half * STAGE + (h ? other : 0) + gr * 64 * SLICE;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) a[p & 1][u] = *reinterpret_cast<const uint4*>(pa + 16 * u * SLICE);
+    if (gr == 0) {
+      const unsigned char* pb = fb + half * STAGE + (h ? other : 0);
+#pragma unroll
+      for (int v = 0; v < FN; ++v) b[h][v] = *reinterpret_cast<const uint4*>(pb + 16 * v * SLICE);
+    }
+  };
   stage(0);
-  for (int t = 0; t < total; ++t) {
-    staged_barrier();  // slice t is in LDS, slice t - 1 is used up
-    if (t + 1 < total) stage(t + 1);
-    const unsigned char* As = lds + (t & 1) * STAGE;
-    const unsigned char* Bs = As + BM * SLICE;
+  if (total > 1) {
+    stage(1);
+    wait_loads<LA + LB>();
+  } else {
+    wait_loads<0>();
+  }
+  __syncthreads();
+  read(0, 0);
+  auto multiply = [&](int p) {
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint4 a[FM], b[FN];
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int u = 0; u < FM; ++u) a[u] = *reinterpret_cast<const uint4*>(As + (wm + 16 * u + i) * SLICE + (h ? c1 : c0));
+      for (int v = 0; v < FN; ++v) {
+        auto& c = acc[(p % NG) * 4 + u][v];
+        c = Mac<MODE>::mac(b[p / NG][v], a[p & 1][u], c);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int t = 0; t + 1 < total; ++t) {
 #pragma unroll
-      for (int v = 0; v < FN; ++v) b[v] = *reinterpret_cast<const uint4*>(Bs + (wn + 16 * v + i) * SLICE + (h ? c1 : c0));
-#pragma unroll
-      for (int u = 0; u < FM; ++u)
-#pragma unroll
-        for (int v = 0; v < FN; ++v) acc[u][v] = Mac<MODE>::mac(b[v], a[u], acc[u][v]);
+    for (int p = 0; p < PH; ++p) {
+      if (p + 1 < PH) {
+        read(t & 1, p + 1);
+      } else {
+        staged_barrier();
+        if (t + 2 < total) stage(t & 1);
+        read((t + 1) & 1, 0);
+      }
+      multiply(p);
     }
   }
-  matrix_drain();
 #pragma unroll
-  for (int u = 0; u < FM; ++u) {
-    const int64_t m = m0 + wm + 16 * u + i;
-    if (m >= g.M) continue;
-    const float rs = MODE == LOW_I8 ? g.row_scale[m] : 1.f;
+  for (int p = 0; p < PH; ++p) {  // the last slice
+    if (p + 1 < PH) read((total - 1) & 1, p + 1);
+    multiply(p);
+  }
+  matrix_drain();
+  __syncthreads();  // the last slice is read: its memory takes the results
+  store_tile<MODE, DT, FM, FN>(g, lds + wave * 16 * CROW, lane, acc, m0 + wm, n0 + wn);
+}
+
+// ---- float A ------------------------------------------------------------------------------------------
+// The same pipeline over slices of 32 columns.  Planes lie in LDS as rows of 64 bytes, 16-byte chunk c of
+// row r at c ^ F((r >> 2) & 3), F = (0, 2, 3, 1): conflict-free for ds_read_b128 (the third weight plane's
+// layout of nc_device.h).  A's floats go into a piece of LDS of their own, where each lane finds the 8
+// columns that it asked for; it splits them and writes the planes before a slice's last phases.  4
+// neighbouring lanes hold a group of 32 columns, so the workgroups of the first column tile write the
+// checkpoint's codes in passing.  The six products of a slice are its phases; their order keeps few
+// planes alive: a2 b0, a1 b0, a0 b0, a1 b1, a0 b1, a0 b2.
+// A layer's sums are short (8 slices for 256 inputs), so a workgroup goes through its tiles as one stream of
+// slices: the next tile's first slices are on their way while a tile ends, and its results leave from
+// registers and are not waited for.
+// RELU: of max(A, 0); MASK: the output is masked by codes and has no bias (each would take 16 registers).
+template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
+__global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, int32_t tiles, int32_t nt) {
+  constexpr int W = WM * WN, T = 64 * W, FM = BM / WM / 16, FN = BN / WN / 16;
+  constexpr int APL = BM * 64, BPL = BN * 64, STAGE = 3 * (APL + BPL);
+  constexpr int XA = BM * 4 / T;                   // chunks of A a thread
+  constexpr int LA = XA * (VEC ? 2 : 8);           // loads of A a wave
+  constexpr int LB = 3 * BPL / 1024 / W;           // 1-KB loads of B a wave
+  static_assert(BM * 4 % T == 0 && 3 * BPL % (1024 * W) == 0, "whole chunks a thread, whole loads a wave");
+  extern __shared__ __attribute__((aligned(256))) unsigned char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, q = lane >> 4;
+  const int first = (int)((int64_t)g.slices * blockIdx.y / g.splits);
+  const int total = (int)((int64_t)g.slices * (blockIdx.y + 1) / g.splits) - first;
+  const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int steps = mine * total;
+  const uint32_t lds0 = lds_address(lds);
+  unsigned char* raw = lds + 2 * STAGE + wave * (XA * 2048);  // this wave's floats
+  const int pads = (int)(g.code_stride / CODE_GROUP) - g.slices;  // code groups behind the last slice
+  auto tile_at = [&](int k, int64_t& m0, int64_t& n0) {
+    const uint32_t t = (uint32_t)chiplet_order(blockIdx.x + k * gridDim.x, tiles), tm = t / (uint32_t)nt;
+    m0 = (int64_t)tm * BM;
+    n0 = (int64_t)(t - tm * (uint32_t)nt) * BN;
+  };
+
+  // what is loaded next: tile lk, slice lt
+  int lk = 0, lt = 0;
+  int64_t lm0 = 0, ln0 = 0;
+  uint32_t oa[XA], ob[LB];
+  const uint8_t* a_next = nullptr;
+  const uint8_t* b_next = nullptr;
+  auto enter = [&]() {
+    tile_at(lk, lm0, ln0);
+#pragma unroll
+    for (int l = 0; l < XA; ++l) {
+      const int r = (l * T + (int)threadIdx.x) >> 2;
+      const int64_t rr = lm0 + r < g.M ? r : g.M - 1 - lm0;  // rows behind the last: its copies, not stored
+      oa[l] = (uint32_t)(rr * g.lda);
+    }
+#pragma unroll
+    for (int j = 0; j < LB; ++j) {
+      const int at = (wave * LB + j) * 16 + (lane >> 2), r = at % BN;  // a row of a plane
+      const int64_t rr = ln0 + r < g.N ? r : g.N - 1 - ln0;
+      ob[j] = (uint32_t)(rr * g.ldb) + hchunk3(r, lane & 3);
+    }
+    a_next = g.A + lm0 * g.lda;
+    b_next = g.B + ln0 * g.ldb + (int64_t)first * 64;
+    if (g.codes && ln0 == 0 && first == 0) {
+      for (int e = threadIdx.x; e < BM * pads; e += T) {
+        const int64_t m = lm0 + e / pads, gr = g.slices + e % pads;
+        if (m >= g.M) break;
+        uint4* c = reinterpret_cast<uint4*>(g.codes + m * g.code_stride + gr * CODE_GROUP);
+        c[0] = c[1] = uint4{0u, 0u, 0u, 0u};
+        g.steps[m * (g.code_stride / CODE_GROUP) + gr] = 1;
+      }
+    }
+  };
+  // what the floats in LDS are: tile and slice, and whether their codes are written
+  int64_t xm0 = 0;
+  int xt = 0;
+  bool xcode = false;
+  auto load = [&](int half) {
+    xm0 = lm0;
+    xt = first + lt;
+    xcode = g.codes && ln0 == 0;
+    const uint32_t to = lds0 + 2 * STAGE + wave * (XA * 2048);
+#pragma unroll
+    for (int l = 0; l < XA; ++l) {
+      const int c = 8 * (4 * xt + (int)(threadIdx.x & 3)), k = (int)g.K;
+      if (VEC) {
+        const uint32_t at = oa[l] + 4 * (uint32_t)(c < k ? c : k - 8);  // columns behind the last: others, cleared
+        load_lds16(a_next, at, to + l * 2048);
+        load_lds16(a_next, at + 16, to + l * 2048 + 1024);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          load_lds4(a_next, oa[l] + 4 * (uint32_t)(c + e < k ? c + e : k - 1), to + l * 2048 + e * 256);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < LB; ++j) {
+      const int pl = (wave * LB + j) * 16 / BN;
+      load_lds16(b_next + pl * g.plane_b, ob[j], lds0 + half * STAGE + 3 * APL + (wave * LB + j) * 1024);
+    }
+    b_next += 64;
+    if (++lt == total) {
+      lt = 0;
+      if (++lk < mine) enter();
+    }
+  };
+  auto store_a = [&](int half) {
+    unsigned char* s = lds + half * STAGE;
+#pragma unroll
+    for (int l = 0; l < XA; ++l) {
+      const int at = l * T + threadIdx.x, r = at >> 2, c = at & 3;
+      float x[8];
+      if (VEC) {
+        const float4 lo = *reinterpret_cast<const float4*>(raw + l * 2048 + 16 * lane);
+        const float4 hi = *reinterpret_cast<const float4*>(raw + l * 2048 + 1024 + 16 * lane);
+        x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
+        x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const float*>(raw + l * 2048 + e * 256 + 4 * lane);
+      }
+      clear8<VEC>((int64_t)xt * 4 + c, g.K, x);
+      if (xcode) {
+        int sb;
+        const uint2 w = group_codes<RELU>(x, sb);
+        if (xm0 + r < g.M) {
+          *reinterpret_cast<uint2*>(g.codes + xm0 * g.code_stride + (uint32_t)(r * (int)g.code_stride + 32 * xt + 8 * c)) = w;
+          const int sr = (int)(g.code_stride / CODE_GROUP);
+          if (c == 0) (g.steps + xm0 * sr)[(uint32_t)(r * sr + xt)] = (uint8_t)sb;
+        }
+      }
+      if (RELU)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = relu_keep_nan(x[e]);
+      uint4 p[3];
+      split3(x, p);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(s + k * APL + r * 64 + hchunk3(r, c)) = p[k];
+    }
+    xcode = false;  // a step behind the last one stores the same again, which nobody reads
+  };
+  floatx4 acc[FM][FN];
+#pragma unroll
+  for (int u = 0; u < FM; ++u)
+#pragma unroll
+    for (int v = 0; v < FN; ++v) acc[u][v] = zero4();
+  const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+  const unsigned char* fa = lds + (wm + i) * 64 + hchunk3(i, q);  // wm, wn and 16 u leave the chunk order as it is
+  const unsigned char* fb = lds + 3 * APL + (wn + i) * 64 + hchunk3(i, q);
+  uint4 a[3][FM], b[3][FN];
+  auto read_a = [&](int half, int p) {
+#pragma unroll
+    for (int u = 0; u < FM; ++u) a[p][u] = *reinterpret_cast<const uint4*>(fa + half * STAGE + p * APL + 16 * u * 64);
+  };
+  auto read_b = [&](int half, int p) {
+#pragma unroll
+    for (int v = 0; v < FN; ++v) b[p][v] = *reinterpret_cast<const uint4*>(fb + half * STAGE + p * BPL + 16 * v * 64);
+  };
+  auto multiply = [&](int pa, int pb) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < FM; ++u)
+#pragma unroll
+      for (int v = 0; v < FN; ++v) acc[u][v] = Mac<LOW_BF16>::mac(b[pb][v], a[pa][u], acc[u][v]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  enter();
+  load(0);
+  wait_loads<0>();
+  store_a(0);
+  lds_barrier();  // (a wave's floats are read before the wave asks for the next ones)
+  if (steps > 1) load(1);
+  staged_barrier();
+  read_a(0, 2);
+  read_b(0, 0);
+  const bool vec = store4_vec<NC_F32>(g) && (g.splits == 1 || g.N % 4 == 0);
+  constexpr int RESULTS = FM * FN;  // stores of a whole tile's results
+  int s = 0;
+  bool left = false;  // RESULTS stores were issued after the loads that the next slice waits for: they stay in flight
+  auto slice = [&](auto arrived) {
+    const int h = s & 1;
+    read_a(h, 1);
+    multiply(2, 0);
+    read_a(h, 0);
+    multiply(1, 0);
+    read_b(h, 1);
+    multiply(0, 0);
+    if (left) wait_loads<LB + RESULTS>();  // A's floats are here, asked for before B's slice
+    else wait_loads<LB>();
+    store_a(h ^ 1);
+    multiply(1, 1);
+    read_b(h, 2);
+    multiply(0, 1);
+    if (left) wait_loads<RESULTS>();
+    else wait_loads<0>();
+    lds_barrier();
+    left = false;
+    arrived();
+    if (s + 2 < steps) load(h);
+    read_a(h ^ 1, 2);
+    read_b(h ^ 1, 0);
+    multiply(0, 2);
+    ++s;
+  };
+  for (int k = 0; k < mine; ++k) {
+    for (int t = 0; t + 1 < total; ++t) slice([] {});
+    int64_t m0, n0;
+    tile_at(k, m0, n0);
+    float cb[FN][4];  // what the results need, a slice ahead
+    uint32_t mask[FM][FN];
 #pragma unroll
     for (int v = 0; v < FN; ++v) {
       const int64_t n = n0 + wn + 16 * v + 4 * q;
-      if (n >= g.N) continue;
-      float o[4];
+      if (!MASK)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = n + j < g.N;
-        float x = (float)acc[u][v][j];
-        if (MODE == LOW_I8) x = x * (rs * (in ? g.col_scale[n + j] : 0.f));
-        if (g.bias && in) x += load_bias(g.bias, g.bias_dtype, n + j);
-        if (g.relu) x = x > 0.f || x != x ? x : 0.f;
-        if (g.mask && in && g.mask[m * g.ldm + n + j] == 0) x = 0.f;
-        o[j] = x;
-      }
-      store4(g, m, n, o);
+        for (int j = 0; j < 4; ++j)
+          cb[v][j] = g.bias ? reinterpret_cast<const float*>(g.bias)[n + j < g.N ? n + j : g.N - 1] : 0.f;
+      if (MASK)
+#pragma unroll
+        for (int u = 0; u < FM; ++u) {
+          const int64_t m = m0 + wm + 16 * u + i, mm = m < g.M ? m : g.M - 1;
+          mask[u][v] = *reinterpret_cast<const uint32_t*>(g.mask + mm * g.ldm + (n < g.ldm ? n : 0));
+        }
     }
+    slice([&] {  // here by now: taken before the next loads, so that nothing is waited for between the stores
+#pragma unroll
+      for (int v = 0; v < FN; ++v) {
+        if (!MASK)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(cb[v][j]));
+        if (MASK)
+#pragma unroll
+          for (int u = 0; u < FM; ++u) asm volatile("" : "+v"(mask[u][v]));
+      }
+    });
+    matrix_drain();
+    float* part = g.splits > 1 ? g.part + (int64_t)blockIdx.y * g.M * g.N : nullptr;
+#pragma unroll
+    for (int u = 0; u < FM; ++u) {
+      const int64_t m = m0 + wm + 16 * u + i;
+#pragma unroll
+      for (int v = 0; v < FN; ++v) {
+        const int64_t n = n0 + wn + 16 * v + 4 * q;
+        floatx4 o = acc[u][v];
+        acc[u][v] = zero4();
+        if (!part) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[j] = MASK ? (((mask[u][v] >> (8 * j)) & 255u) ? o[j] : 0.f) : g.bias ? o[j] + cb[v][j] : o[j];
+        }
+        if (m >= g.M || n >= g.N) continue;
+        float* p = part ? part + m * g.N + n : reinterpret_cast<float*>(g.out) + m * g.ldc + n;
+        if (vec) {
+          *reinterpret_cast<floatx4*>(p) = o;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < g.N) p[j] = o[j];
+        }
+      }
+    }
+    // (a tile cut off by the matrix's end stores less)
+    left = vec && m0 + BM <= g.M && n0 + BN <= g.N;
   }
 }
 
-template <int MODE, int BM, int BN, int WM, int WN>
+// ---- launches ------------------------------------------------------------------------------------------
+// once for each kernel and device
+template <typename K>
+static int allow_lds(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (bytes <= 65536) return 0;
+  if (const int e = (int)hipGetDevice(&dev)) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return 0;
+  const int e = (int)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (!e) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+template <int MODE, int DT>
+static int finish_parts(const LowGemm& g, hipStream_t s) {
+  if (g.splits <= 1) return (int)hipGetLastError();
+  const int64_t quads = (g.N + 3) / 4, n = g.M * quads;
+  hipLaunchKernelGGL((k_low_finish<MODE, DT>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, g, quads);
+  return (int)hipGetLastError();
+}
+
+template <int MODE, int DT, int BM, int BN, int WM, int WN>
 static int run_low_gemm(const LowGemm& g, hipStream_t s) {
   const int64_t mt = (g.M + BM - 1) / BM, nt = (g.N + BN - 1) / BN;
   constexpr int lds = 2 * (BM + BN) * SLICE;
-  hipLaunchKernelGGL((k_low_gemm<MODE, BM, BN, WM, WN>), dim3((unsigned)(mt * nt)), dim3(64 * WM * WN), lds, s, g, mt, nt);
-  return (int)hipGetLastError();
+  auto kernel = k_low_gemm<MODE, DT, BM, BN, WM, WN>;
+  static std::atomic<uint64_t> done{0};
+  if (const int e = allow_lds(kernel, lds, done)) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(mt * nt), (unsigned)g.splits), dim3(64 * WM * WN), lds, s, g, mt, nt);
+  return finish_parts<MODE, DT>(g, s);
+}
+
+template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
+static int run_low_gemm_f(const LowGemm& g, hipStream_t s) {
+  const int64_t mt = (g.M + BM - 1) / BM, nt = (g.N + BN - 1) / BN, tiles = mt * nt;
+  constexpr int lds = 2 * 192 * (BM + BN) + 128 * BM, per_cu = 163840 / lds;  // resident workgroups
+  auto kernel = k_low_gemm_f<BM, BN, WM, WN, VEC, RELU, MASK>;
+  static std::atomic<uint64_t> done{0};
+  if (const int e = allow_lds(kernel, lds, done)) return e;
+  const int64_t fill = 256 * per_cu;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles < fill ? tiles : fill), (unsigned)g.splits), dim3(64 * WM * WN), lds, s, g,
+                     (int32_t)tiles, (int32_t)nt);
+  return finish_parts<LOW_F32, NC_F32>(g, s);
+}
+
+// Tiles and cuts.  256 compute units; a large tile reads less LDS for each product, a small one (or a cut
+// sum) fills the units when the output is small.
+enum LowTile { TILE_SMALL, TILE_MIDDLE, TILE_LARGE };
+static int64_t tiles_of(int64_t M, int64_t N, int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
+
+static LowTile low_tile(int mode, int64_t M, int64_t N) {
+  if (mode == LOW_F32) {
+    if (tiles_of(M, N, 128, 256) >= 192) return N > 128 ? TILE_LARGE : TILE_MIDDLE;
+    return tiles_of(M, N, 128, 128) >= 192 ? TILE_MIDDLE : TILE_SMALL;
+  }
+  if (tiles_of(M, N, 256, 256) >= 192) return TILE_LARGE;
+  return tiles_of(M, N, 128, 128) >= 192 ? TILE_MIDDLE : TILE_SMALL;
+}
+
+int low_gemm_splits(int mode, int64_t M, int64_t N, int64_t K) {
+  const LowTile t = low_tile(mode, M, N);
+  if (t != TILE_SMALL) return 1;
+  const int64_t slices = (K * (mode == LOW_I8 ? 1 : mode == LOW_F32 ? 4 : 2) + SLICE - 1) / SLICE;
+  const int64_t tiles = tiles_of(M, N, 64, 64);
+  int64_t want = 512 / (tiles > 0 ? tiles : 1);
+  if (want > slices / 8) want = slices / 8;  // parts of 8 slices at least
+  return (int)(want < 1 ? 1 : want);
+}
+
+template <int MODE, int DT>
+static int pick_low_gemm(const LowGemm& g, hipStream_t s) {
+  switch (low_tile(MODE, g.M, g.N)) {
+    case TILE_LARGE: return run_low_gemm<MODE, DT, 256, 256, 2, 4>(g, s);
+    case TILE_MIDDLE: return run_low_gemm<MODE, DT, 128, 128, 2, 2>(g, s);
+    default: return run_low_gemm<MODE, DT, 64, 64, 1, 4>(g, s);
+  }
+}
+
+template <bool VEC, bool RELU, bool MASK>
+static int pick_low_gemm_f(const LowGemm& g, hipStream_t s) {
+  switch (low_tile(LOW_F32, g.M, g.N)) {
+    case TILE_LARGE: return run_low_gemm_f<128, 256, 2, 4, VEC, RELU, MASK>(g, s);
+    case TILE_MIDDLE: return run_low_gemm_f<128, 128, 4, 2, VEC, RELU, MASK>(g, s);
+    default: return run_low_gemm_f<64, 64, 2, 2, VEC, RELU, MASK>(g, s);
+  }
 }
 
 int launch_low_gemm(const LowGemm& g, hipStream_t s) {
   if (g.M <= 0 || g.N <= 0) return 0;
   switch (g.mode) {
-    case LOW_I8: return run_low_gemm<LOW_I8, 128, 128, 2, 2>(g, s);
-    case LOW_BF16: return run_low_gemm<LOW_BF16, 128, 128, 2, 2>(g, s);
-    case LOW_F16: return run_low_gemm<LOW_F16, 128, 128, 2, 2>(g, s);
+    case LOW_I8:
+      if (g.out_dtype == NC_F32) return pick_low_gemm<LOW_I8, NC_F32>(g, s);
+      return g.out_dtype == NC_F16 ? pick_low_gemm<LOW_I8, NC_F16>(g, s) : pick_low_gemm<LOW_I8, NC_BF16>(g, s);
+    case LOW_BF16: return pick_low_gemm<LOW_BF16, NC_BF16>(g, s);
+    case LOW_F16: return pick_low_gemm<LOW_F16, NC_F16>(g, s);
+    case LOW_F32: {
+      const bool vec = load8_vec(g.A, g.lda / 4, g.K, NC_F32);
+      if (g.mask && (g.a_relu || g.bias || g.relu)) return (int)hipErrorInvalidValue;  // no call has both
+      if (vec) return g.mask ? pick_low_gemm_f<true, false, true>(g, s)
+                    : g.a_relu ? pick_low_gemm_f<true, true, false>(g, s) : pick_low_gemm_f<true, false, false>(g, s);
+      return g.mask ? pick_low_gemm_f<false, false, true>(g, s)
+             : g.a_relu ? pick_low_gemm_f<false, true, false>(g, s) : pick_low_gemm_f<false, false, false>(g, s);
+    }
   }
   return (int)hipErrorInvalidValue;
+}
+
+// ---- few rows, or few columns ------------------------------------------------------------------------------
+// The int8 product where a launch costs more than its work, or where the weight's bytes are all there is
+// to it.  4 waves; each streams 16 channels of the weight from memory into the instruction's first operand
+// (lane (i, q): channel i, 16 bytes at 16 q of every 64), 8 loads ahead; the second operand is up to 16 MT
+// rows of x codes.  WK = 4: the waves share 16 channels and a quarter of the sum each (few rows, long sums);
+// WK = 1: 16 channels each (short sums).
+// DX >= 0: x is encoded here, by every workgroup for itself, while the first weights are on their way: one
+// launch instead of two, worth it up to 8192 values a workgroup.
+constexpr int SMALL_PAD = 16;  // bytes behind a row of codes in LDS: rows start 4 banks apart
+
+template <int DX, bool VEC, int MT, int WK>
+__global__ void __launch_bounds__(256) k_low_small(const LowSmall p) {
+  const LowGemm& g = p.g;
+  constexpr int RB = 16 * MT;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // x codes; then the waves' sums
+  __shared__ float scale[RB];
+  __shared__ uint32_t red[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, q = lane >> 4;
+  const int kp = (int)g.ldb, row_bytes = kp + SMALL_PAD;
+  const int64_t n0 = (int64_t)blockIdx.x * (WK == 4 ? 16 : 64) + (WK == 4 ? 0 : 16 * wave);
+  const int64_t m0 = (int64_t)blockIdx.y * RB;
+  const int rows = (int)(g.M - m0 < RB ? g.M - m0 : RB);
+  const int ksteps = (int)((g.K + 63) / 64);  // code rows are padded to whole steps
+  const int k0 = WK == 4 ? ksteps * wave / 4 : 0, k1 = WK == 4 ? ksteps * (wave + 1) / 4 : ksteps;
+  const int64_t ch = n0 + i < g.N ? n0 + i : g.N - 1;
+  const uint8_t* wrow = g.B + ch * g.ldb + 16 * q;
+  constexpr int DEEP = 8;
+  uint4 w[DEEP];
+#pragma unroll
+  for (int d = 0; d < DEEP; ++d) {
+    const int k = k0 + d < k1 ? k0 + d : (k1 > 0 ? k1 - 1 : 0);
+    w[d] = *reinterpret_cast<const uint4*>(wrow + 64 * k);
+  }
+  if (DX >= 0) {
+    constexpr int C = 4;
+    const int chunks = kp / 8;
+    if (WK == 4 && rows < 4) {  // the workgroup takes a row: 256 C chunks
+      for (int r = 0; r < rows; ++r) {
+        float v[C][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < C; ++j) load8<DX, VEC>(p.x, (m0 + r) * p.x_stride, threadIdx.x + 256 * j, g.K, v[j]);
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          clear8<VEC>(threadIdx.x + 256 * j, g.K, v[j]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = max(top, mag_bits(v[j][e]));
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        if (lane == 0) red[wave] = top;
+        __syncthreads();
+        top = max(max(red[0], red[1]), max(red[2], red[3]));
+        __syncthreads();
+        const bool bad = top >= 0x7f800000u;
+        const float s = row_scale(top), rcp = 1.f / s;
+        if (threadIdx.x == 0) scale[r] = bad ? __builtin_nanf("") : s;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          const int c = threadIdx.x + 256 * j;
+          if (c < chunks) *reinterpret_cast<uint2*>(lds + r * row_bytes + 8 * c) = row_codes(v[j], bad, s, rcp);
+        }
+      }
+    } else if (WK == 4) {  // a wave takes a row: 64 C chunks
+      for (int r = wave; r < rows; r += 4) {
+        float v[C][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < C; ++j) load8<DX, VEC>(p.x, (m0 + r) * p.x_stride, lane + 64 * j, g.K, v[j]);
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          clear8<VEC>(lane + 64 * j, g.K, v[j]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = max(top, mag_bits(v[j][e]));
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        const bool bad = top >= 0x7f800000u;
+        const float s = row_scale(top), rcp = 1.f / s;
+        if (lane == 0) scale[r] = bad ? __builtin_nanf("") : s;
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (lane + 64 * j < chunks) *reinterpret_cast<uint2*>(lds + r * row_bytes + 8 * (lane + 64 * j)) = row_codes(v[j], bad, s, rcp);
+      }
+    } else {  // half a wave takes a row of up to 32 chunks, every eighth one, all loads first
+      const int c = lane & 31, r0 = 2 * wave + (lane >> 5);
+      float v[RB / 8][8];
+#pragma unroll
+      for (int j = 0; j < RB / 8; ++j) {
+        const int r = r0 + 8 * j < rows ? r0 + 8 * j : rows - 1;
+        load8<DX, VEC>(p.x, (m0 + r) * p.x_stride, c, g.K, v[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < RB / 8; ++j) {
+        const int r = r0 + 8 * j;
+        uint32_t top = 0;
+        clear8<VEC>(c, g.K, v[j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, mag_bits(v[j][e]));
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        const bool bad = top >= 0x7f800000u;
+        const float s = row_scale(top), rcp = 1.f / s;
+        if (r < rows) {
+          if (c == 0) scale[r] = bad ? __builtin_nanf("") : s;
+          if (c < chunks) *reinterpret_cast<uint2*>(lds + r * row_bytes + 8 * c) = row_codes(v[j], bad, s, rcp);
+        }
+      }
+    }
+    __syncthreads();
+  } else if ((int)threadIdx.x < RB) {
+    scale[threadIdx.x] = g.row_scale[m0 + ((int)threadIdx.x < rows ? (int)threadIdx.x : rows - 1)];
+  }
+  // x's operands: rows behind the last are others (LDS holds no more than `rows`), not stored
+  const uint8_t* xrow[MT];
+#pragma unroll
+  for (int u = 0; u < MT; ++u) {
+    const int r = 16 * u + i < rows ? 16 * u + i : rows - 1;
+    xrow[u] = DX >= 0 ? lds + r * row_bytes + 16 * q : g.A + (m0 + r) * g.lda + 16 * q;
+  }
+  intx4 acc[MT];
+#pragma unroll
+  for (int u = 0; u < MT; ++u) acc[u] = intx4{0, 0, 0, 0};
+  for (int k = k0; k < k1; k += DEEP) {
+    uint4 x[DX >= 0 ? 1 : DEEP][MT];
+    if (DX < 0) {
+#pragma unroll
+      for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) x[DX >= 0 ? 0 : d][u] = *reinterpret_cast<const uint4*>(xrow[u] + 64 * (k + d < k1 ? k + d : k1 - 1));
+    }
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {
+      const uint4 wd = w[d];
+      if (k + DEEP < k1) w[d] = *reinterpret_cast<const uint4*>(wrow + 64 * (k + DEEP + d < k1 ? k + DEEP + d : k1 - 1));
+      if (k + d < k1) {
+#pragma unroll
+        for (int u = 0; u < MT; ++u) {
+          const uint4 xd = DX >= 0 ? *reinterpret_cast<const uint4*>(xrow[u] + 64 * (k + d)) : x[DX >= 0 ? 0 : d][u];
+          acc[u] = Mac<LOW_I8>::mac(wd, xd, acc[u]);
+        }
+      }
+    }
+  }
+  matrix_drain();
+  if (WK == 4) {  // the four sums of a block: wave u adds up block u of rows
+    __syncthreads();
+    intx4* part = reinterpret_cast<intx4*>(lds);
+#pragma unroll
+    for (int u = 0; u < MT; ++u) part[(wave * MT + u) * 64 + lane] = acc[u];
+    __syncthreads();
+    if (wave >= MT) return;
+    intx4 t = part[wave * 64 + lane];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) t += part[(k * MT + wave) * 64 + lane];
+    acc[0] = t;
+  } else if (DX < 0) {
+    __syncthreads();  // scale[]
+  }
+  const int64_t n = n0 + 4 * q;
+  if (n >= g.N) return;
+  float cs[4], cb[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t nn = n + j < g.N ? n + j : g.N - 1;
+    cs[j] = g.col_scale[nn];
+    cb[j] = g.bias ? load_bias(g.bias, g.bias_dtype, nn) : 0.f;
+  }
+#pragma unroll
+  for (int u = 0; u < (WK == 4 ? 1 : MT); ++u) {
+    const int r = 16 * (WK == 4 ? wave : u) + i;
+    if (r >= rows) continue;
+    float o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = finish<LOW_I8>(g, (float)acc[u][j], scale[r] * cs[j], cb[j], 1u);
+    if (g.out_dtype == NC_F32) store4<NC_F32>(g, store4_vec<NC_F32>(g), m0 + r, n, o);
+    else if (g.out_dtype == NC_F16) store4<NC_F16>(g, store4_vec<NC_F16>(g), m0 + r, n, o);
+    else store4<NC_BF16>(g, store4_vec<NC_BF16>(g), m0 + r, n, o);
+  }
+}
+
+// Which products it takes with x to encode: up to 3 rows of 8192, 16 of 2048, or short sums (256) of at
+// most 512 workgroups: beyond those every column tile's own encoding costs more than the launch that it
+// saves (bfloat16, us, here | encoded once: 777 x 93 x 1001 14.9 | 16.5, 777 x 256 x 4096 19.2 | 17.6).
+static bool short_sums(int64_t M, int64_t K) { return K <= 256 && M > 16; }
+bool low_small_encodes(int64_t M, int64_t N, int64_t K) {
+  if (short_sums(M, K)) return ((M + 63) / 64) * ((N + 63) / 64) <= 512;
+  return (M < 4 && K <= 8192) || (M <= 16 && K <= 2048);
+}
+
+template <int DX, bool VEC, int MT, int WK>
+static int run_low_small(const LowSmall& a, hipStream_t s) {
+  const int rb = 16 * MT, rows = (int)(a.g.M < rb ? a.g.M : rb);
+  int lds = DX >= 0 ? rows * (int)(a.g.ldb + SMALL_PAD) : 0;
+  if (WK == 4 && lds < 4 * MT * 1024) lds = 4 * MT * 1024;
+  const dim3 grid((unsigned)((a.g.N + (WK == 4 ? 15 : 63)) / (WK == 4 ? 16 : 64)), (unsigned)((a.g.M + rb - 1) / rb));
+  hipLaunchKernelGGL((k_low_small<DX, VEC, MT, WK>), grid, dim3(256), lds, s, a);
+  return (int)hipGetLastError();
+}
+template <int DX, bool VEC>
+static int encode_low_small(const LowSmall& a, hipStream_t s) {
+  if (short_sums(a.g.M, a.g.K)) return run_low_small<DX, VEC, 4, 1>(a, s);
+  return run_low_small<DX, VEC, 1, 4>(a, s);
+}
+
+int launch_low_small(const LowSmall& a, hipStream_t s) {
+  if (a.g.M <= 0 || a.g.N <= 0) return 0;
+  const bool vec = a.x_dtype >= 0 && load8_vec(a.x, a.x_stride, a.g.K, a.x_dtype);
+  switch (a.x_dtype) {
+    case NC_F32: return vec ? encode_low_small<NC_F32, true>(a, s) : encode_low_small<NC_F32, false>(a, s);
+    case NC_F16: return vec ? encode_low_small<NC_F16, true>(a, s) : encode_low_small<NC_F16, false>(a, s);
+    case NC_BF16: return vec ? encode_low_small<NC_BF16, true>(a, s) : encode_low_small<NC_BF16, false>(a, s);
+  }
+  if (a.g.M <= 16) return run_low_small<-1, false, 1, 4>(a, s);
+  if (a.g.M <= 32) return run_low_small<-1, false, 2, 4>(a, s);
+  return run_low_small<-1, false, 4, 4>(a, s);
 }
 
 // ---- weight gradient -----------------------------------------------------------------------------------
@@ -223,11 +954,9 @@ int launch_low_gemm(const LowGemm& g, hipStream_t s) {
 // make the 8 sum indices of a lane's operand: m = 4 q + e and 16 + 4 q + e, the same for both operands.
 // Rows of BN (BK) elements are cut into 32-byte units; unit u of row m lies at u ^ (m & 7): the 8 rows
 // that 32 lanes read together then cover all 64 banks.
-__device__ const uint4 g_zero_row[2] = {};  // what rows behind the last one read
-
-__device__ __forceinline__ shortx4 tr_read(const unsigned char* p) {
+__device__ __forceinline__ uint2 tr_read(uint32_t at) {
   typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)p);
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)at));
 }
 
 // 16 codes of one row and group -> 16 elements of 16 bits; step is a power of two: exact
@@ -242,15 +971,15 @@ __device__ __forceinline__ void decode16(uint4 c, float step, uint4& lo, uint4& 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float f = (float)((b >> (8 * e)) & 255u);
-      v[e] = RELU ? __builtin_fmaxf(__builtin_fmaf(f, step, -step), 0.f) : __builtin_fmaf(f, step, -128.f * step);
-      if (step != step) v[e] = step;  // a NaN group (fmax would drop it)
+      v[e] = __builtin_fmaf(f, step, RELU ? -step : -128.f * step);
+      if (RELU) v[e] = relu_keep_nan(v[e]);
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       if (F16) {
         o[2 * j + e] = f32_elem<NC_F16>(v[2 * e]) | (uint32_t)f32_elem<NC_F16>(v[2 * e + 1]) << 16;
       } else {  // exact in bfloat16: the upper halves
-        o[2 * j + e] = __builtin_bit_cast(uint32_t, v[2 * e]) >> 16 | (__builtin_bit_cast(uint32_t, v[2 * e + 1]) & 0xffff0000u);
+        o[2 * j + e] = upper_halves(v[2 * e], v[2 * e + 1]);
       }
     }
   }
@@ -258,68 +987,172 @@ __device__ __forceinline__ void decode16(uint4 c, float step, uint4& lo, uint4& 
   hi = uint4{o[4], o[5], o[6], o[7]};
 }
 
-template <int NP, bool F16, bool RELU, int BN, int BK, int MS, int WN, int WK>
+constexpr int SUM_ROWS = 512;  // rows that one workgroup adds up for the bias gradient
+
+// sums of the columns [n0, n0 + BN) of dY over rows [rb, re): a thread takes 8 columns of every R-th row, and
+// the R sums of a column are added in order
+template <int DT, int BN, int T>
+__device__ __forceinline__ void put_col_sums(const LowWgrad& g, int64_t n0, int64_t piece, const float (&t)[8], float* red) {
+  constexpr int C8 = BN / 8, R = T / C8;
+  const int c = threadIdx.x % C8, w = threadIdx.x / C8;
+  __syncthreads();  // the buffers are read
+#pragma unroll
+  for (int e = 0; e < 8; ++e) red[w * BN + 8 * c + e] = t[e];
+  __syncthreads();
+  for (int e = threadIdx.x; e < BN; e += T) {
+    float sum = 0.f;
+    for (int k = 0; k < R; ++k) sum += red[k * BN + e];
+    if (n0 + e >= g.N) continue;
+    if (!g.db) g.sums[piece * g.N + n0 + e] = sum;
+    else if (DT == NC_F32) reinterpret_cast<float*>(g.db)[n0 + e] = sum;
+    else reinterpret_cast<uint16_t*>(g.db)[n0 + e] = f32_elem<DT>(sum);
+  }
+}
+template <int DT, int BN, int T, bool VEC>
+__device__ __forceinline__ void col_sums(const LowWgrad& g, int64_t n0, int64_t rb, int64_t re, int64_t piece, float* red) {
+  constexpr int C8 = BN / 8, R = T / C8;
+  const int64_t c = n0 / 8 + threadIdx.x % C8;
+  const int64_t cols = VEC ? (g.N + 7) / 8 * 8 : g.N;  // 16-bit rows are padded to 64 columns
+  float t[8] = {};
+  int64_t r = rb + threadIdx.x / C8;
+  for (; r + 3 * R < re; r += 4 * R) {
+    float v[4][8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) load8<DT, VEC>(g.dy, (r + u * R) * g.ldy, c, cols, v[u]);  // (columns behind the last: not stored)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] += (v[0][e] + v[1][e]) + (v[2][e] + v[3][e]);
+  }
+  for (; r < re; r += R) {
+    float v[8];
+    load8<DT, VEC>(g.dy, r * g.ldy, c, cols, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] += v[e];
+  }
+  put_col_sums<DT, BN, T>(g, n0, piece, t, red);
+}
+
+// The pipeline is k_low_gemm's: phases of 4 x FK blocks, the next phase's operands read from LDS while
+// one multiplies; before a stage's last phase the barrier that frees its half.  dY goes into LDS by itself,
+// codes through registers: loaded with dY a stage ahead, decoded and written before the stage's
+// last phase but one.
+// NP = 3: dY is float, split into its planes on the way like A in k_low_gemm_f.  Workgroups with
+// blockIdx.y behind the last column tile add up their rows of dY instead (the bias gradient).
+template <int NP, int DT, bool RELU, int BN, int BK, int MS, int WN, int WK, bool VEC>
 __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
   constexpr int W = WN * WK, T = 64 * W;
   constexpr int FN = BN / WN / 16, FK = BK / WK / 16;
   constexpr int YROW = 2 * BN, XROW = 2 * BK;               // bytes of a staged row
   constexpr int YSTAGE = MS * YROW, XSTAGE = MS * XROW, STAGE = NP * YSTAGE + XSTAGE;
-  constexpr int YL = NP * YSTAGE / 1024 / W;                // 1-KB loads a wave
+  constexpr bool F16 = DT == NC_F16;
+  constexpr int YL = NP == 3 ? 0 : YSTAGE / 1024 / W;       // 1-KB loads a wave
+  constexpr int YF = NP == 3 ? MS * BN / 8 / T : 0;         // 8-column chunks a thread
   constexpr int XL = MS * BK / 16 / T;                      // 16-code loads a thread
-  static_assert(NP * YSTAGE % (1024 * W) == 0 && MS * BK % (16 * T) == 0 && YL > 0 && XL > 0, "whole loads");
+  constexpr int NG = FN / 4, NH = MS / 32, PH = NH * NP * NG;
+  static_assert(YSTAGE % (1024 * W) == 0 && MS * BK % (16 * T) == 0 && YL + YF > 0 && XL > 0, "whole loads");
+  static_assert(NP == 1 || MS * BN % (8 * T) == 0, "whole chunks");
   static_assert(BN >= 128 && BK >= 128, "rows of at least 8 units of 32 bytes");
+  static_assert((NG == 1 || (NG == 2 && FN == 8)) && YROW % 256 == 0 && XROW % 256 == 0, "the second group is 128 bytes away");
+  static_assert(FN % 4 == 0 && PH >= 2 && (NH == 1 || NH == 2), "phases");
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q = lane >> 4, j16 = lane & 15;
   const int64_t n0 = (int64_t)blockIdx.x * BN, k0 = (int64_t)blockIdx.y * BK;
-  const int64_t rb = (int64_t)blockIdx.z * g.rows_per;
-  const int64_t re = rb + g.rows_per < g.M ? rb + g.rows_per : g.M;
+  int64_t rb = (int64_t)blockIdx.z * g.rows_per;
+  int64_t re = rb + g.rows_per < g.M ? rb + g.rows_per : g.M;
   const int64_t ychunks = (g.N + 7) / 8, xchunks = g.code_stride / 16, steps_row = g.code_stride / CODE_GROUP;
   const int total = (int)((re - rb + MS - 1) / MS);
+  const uint32_t lds0 = lds_address(lds);
+  const int kt = g.want_dw ? (int)((g.K + BK - 1) / BK) : 0;
+  if ((int)blockIdx.y >= kt) {  // (the whole workgroup) a piece of the split's rows
+    const int piece = blockIdx.y - kt;
+    rb += piece * (int64_t)SUM_ROWS;
+    re = rb + SUM_ROWS < re ? rb + SUM_ROWS : re;
+    col_sums<DT, BN, T, VEC>(g, n0, rb, re, (int64_t)blockIdx.z * g.pieces + piece, reinterpret_cast<float*>(lds));
+    return;
+  }
 
-  auto stage_y = [&](int t) {
-    unsigned char* s = lds + (t & 1) * STAGE;
+  float yf[YF > 0 ? YF : 1][8], ysum[8] = {};  // float dY: its columns' sums in passing (T is a multiple of BN / 8)
+  const bool summing = YF > 0 && g.want_db && blockIdx.y == 0;
+  uint32_t yo[YL > 0 ? YL : 1];  // 16-bit dY: byte offsets from the stage's first row
+  int yrow[YL > 0 ? YL : 1];
 #pragma unroll
-    for (int l = 0; l < YL; ++l) {
-      const int at = (wave * YL + l) * 64 + lane;  // 16-byte position in the planes' tiles
-      const int p = at / (YSTAGE / 16), in = at % (YSTAGE / 16);
-      const int row = in / (YROW / 16), pos = in % (YROW / 16);
-      int64_t c = n0 / 8 + (pos ^ ((row & 7) << 1));
-      c = c < ychunks ? c : ychunks - 1;  // columns behind the last: not stored
-      const int64_t m = rb + (int64_t)t * MS + row;
-      const void* src = m < re ? (const void*)(g.dy + p * g.plane + m * g.ldy + 8 * c) : (const void*)g_zero_row;
-      __builtin_amdgcn_global_load_lds(NC_GLOBAL(src), NC_LDS(s + (wave * YL + l) * 1024), 16, 0, 0);
+  for (int l = 0; l < YL; ++l) {
+    const int at = (wave * YL + l) * 64 + lane;  // 16-byte position in the tile
+    yrow[l] = at / (YROW / 16);
+    int64_t c = n0 / 8 + ((at % (YROW / 16)) ^ ((yrow[l] & 7) << 1));
+    c = c < ychunks ? c : ychunks - 1;  // columns behind the last: not stored
+    yo[l] = (uint32_t)(yrow[l] * 2 * g.ldy + 16 * c);
+  }
+  uint32_t xo[XL], so[XL];  // codes and steps
+#pragma unroll
+  for (int l = 0; l < XL; ++l) {
+    const int at = l * T + threadIdx.x, row = at / (BK / 16);
+    int64_t c = k0 / 16 + at % (BK / 16);
+    c = c < xchunks ? c : xchunks - 1;
+    xo[l] = (uint32_t)(row * g.code_stride + 16 * c);
+    so[l] = (uint32_t)(row * steps_row + (c >> 1));
+  }
+  auto stage_y = [&](int t) {
+#pragma unroll
+    for (int l = 0; l < YF; ++l) {
+      const int at = l * T + threadIdx.x, row = at / (BN / 8);
+      const int64_t m = rb + (int64_t)t * MS + row, mm = m < re ? m : re - 1;
+      load8<NC_F32, VEC>(g.dy, mm * g.ldy, n0 / 8 + at % (BN / 8), g.N, yf[l]);
+    }
+    if (YL > 0) {
+      const uint8_t* base = reinterpret_cast<const uint8_t*>(g.dy) + 2 * (rb + (int64_t)t * MS) * g.ldy;
+      const int last = (int)(re - rb - (int64_t)t * MS) - 1;  // rows behind the last: its copies, against zeros
+#pragma unroll
+      for (int l = 0; l < YL; ++l) {
+        const uint32_t o = last >= MS - 1 || yrow[l] <= last ? yo[l] : yo[l] - (uint32_t)(yrow[l] - last) * (uint32_t)(2 * g.ldy);
+        load_lds16(base, o, lds0 + (t & 1) * STAGE + (wave * YL + l) * 1024);
+      }
     }
   };
   uint4 xc[XL];
   uint32_t xs[XL];
   auto load_x = [&](int t) {
+    const uint8_t* codes = g.codes + (rb + (int64_t)t * MS) * g.code_stride;
+    const uint8_t* steps = g.steps + (rb + (int64_t)t * MS) * steps_row;
+    const int last = (int)(re - rb - (int64_t)t * MS) - 1;
 #pragma unroll
     for (int l = 0; l < XL; ++l) {
-      const int at = l * T + threadIdx.x, row = at / (BK / 16);
-      int64_t c = k0 / 16 + at % (BK / 16);
-      c = c < xchunks ? c : xchunks - 1;
-      const int64_t m = rb + (int64_t)t * MS + row;
-      if (m < re) {
-        xc[l] = *reinterpret_cast<const uint4*>(g.codes + m * g.code_stride + 16 * c);
-        xs[l] = g.steps[m * steps_row + (c >> 1)];
-      } else {
-        xc[l] = uint4{0u, 0u, 0u, 0u};
-        xs[l] = 1u;
-      }
+      const int row = (l * T + (int)threadIdx.x) / (BK / 16);
+      const uint32_t back = row <= last ? 0u : (uint32_t)(row - last);
+      xc[l] = *reinterpret_cast<const uint4*>(codes + (xo[l] - back * (uint32_t)g.code_stride));
+      xs[l] = steps[so[l] - back * (uint32_t)steps_row];
     }
   };
-  auto store_x = [&](int t) {
+  auto store_xy = [&](int t) {
     unsigned char* s = lds + (t & 1) * STAGE + NP * YSTAGE;
 #pragma unroll
     for (int l = 0; l < XL; ++l) {
       const int at = l * T + threadIdx.x, row = at / (BK / 16), u = at % (BK / 16);
+      __builtin_amdgcn_sched_barrier(0);  // one chunk's temporaries at a time
+      const bool in = rb + (int64_t)t * MS + row < re;
       const float step = xs[l] == 255u ? __builtin_nanf("") : __builtin_bit_cast(float, xs[l] << 23);
       uint4 lo, hi;
       decode16<F16, RELU>(xc[l], step, lo, hi);
+      if (!in) lo = hi = uint4{0u, 0u, 0u, 0u};
       uint4* d = reinterpret_cast<uint4*>(s + row * XROW + 32 * (u ^ (row & 7)));
       d[0] = lo;
       d[1] = hi;
+    }
+#pragma unroll
+    for (int l = 0; l < YF; ++l) {
+      const int at = l * T + threadIdx.x, row = at / (BN / 8), c = at % (BN / 8);
+      const bool in = rb + (int64_t)t * MS + row < re;
+      if (!in)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) yf[l][e] = 0.f;
+      if (summing)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ysum[e] += yf[l][e];
+      uint4 p[3];
+      split3(yf[l], p);
+      unsigned char* y = lds + (t & 1) * STAGE + row * YROW + 16 * (c ^ ((row & 7) << 1));
+#pragma unroll
+      for (int k = 0; k < NP; ++k) *reinterpret_cast<uint4*>(y + k * YSTAGE) = p[k];
     }
   };
 
@@ -329,94 +1162,178 @@ __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
 #pragma unroll
     for (int v = 0; v < FK; ++v) acc[u][v] = zero4();
   const int wn = (wave / WK) * (BN / WN), wk = (wave % WK) * (BK / WK);
-  const int tr = 4 * q + (j16 >> 2), tc = 8 * (j16 & 3);  // row and byte in the 32-byte unit of a lane's transposed read
+  // a lane's transposed reads: row tr of a step, 8 bytes tc of a 32-byte unit; the addresses are kept for the
+  // first group of units and recomputed from them at each read, so that they take few registers
+  const int tr = 4 * q + (j16 >> 2), tc = 8 * (j16 & 3);
+  uint32_t ya[4], xa[FK];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) ya[u] = lds0 + tr * YROW + 32 * ((wn / 16 + u) ^ (tr & 7)) + tc;
+#pragma unroll
+  for (int v = 0; v < FK; ++v) xa[v] = lds0 + NP * YSTAGE + tr * XROW + 32 * ((wk / 16 + v) ^ (tr & 7)) + tc;
+  uint4 a[2][4], b[2][FK];
+  auto pair = [](uint32_t at, int next) {
+    asm volatile("" : "+v"(at));
+    const uint2 x0 = tr_read(at), x1 = tr_read(at + next);
+    return uint4{x0.x, x0.y, x1.x, x1.y};
+  };
+  // phase p = (half h, plane, group of 4 n blocks); the smallest plane first
+  auto read = [&](int t, int p, int to_a, int to_b) {
+    const int h = p / (NP * NG), pl = NP - 1 - (p / NG) % NP, gr = p % NG;
+    const uint32_t s = (t & 1) * STAGE;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)  // the second group's units: 4 more, of 32 bytes, in a row cut into 8
+      a[to_a][u] = pair((ya[u] ^ (128u * gr)) + (s + pl * YSTAGE + 32 * h * YROW), 16 * YROW);
+    if (p % (NP * NG) == 0) {
+#pragma unroll
+      for (int v = 0; v < FK; ++v) b[to_b][v] = pair(xa[v] + (s + 32 * h * XROW), 16 * XROW);
+    }
+  };
+  auto multiply = [&](int p) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int v = 0; v < FK; ++v) {
+        auto& c = acc[(p % NG) * 4 + u][v];
+        c = Mac<F16 ? LOW_F16 : LOW_BF16>::mac(b[p / (NP * NG)][v], a[p & 1][u], c);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  };
   if (total > 0) {
     stage_y(0);
     load_x(0);
-    store_x(0);
-  }
-  for (int t = 0; t < total; ++t) {
+    store_xy(0);
+    if (total > 1) {
+      load_x(1);
+      stage_y(1);
+    }
     staged_barrier();
-    if (t + 1 < total) {
-      stage_y(t + 1);
-      load_x(t + 1);
-    }
-    const unsigned char* Y = lds + (t & 1) * STAGE;
-    const unsigned char* X = Y + NP * YSTAGE;
+    read(0, 0, 0, 0);
+    for (int t = 0; t + 1 < total; ++t) {
 #pragma unroll
-    for (int ms = 0; ms < MS; ms += 32) {
-      uint4 b[FK];
-#pragma unroll
-      for (int v = 0; v < FK; ++v) {
-        const unsigned char* p = X + (ms + tr) * XROW + 32 * ((wk / 16 + v) ^ (tr & 7)) + tc;
-        const shortx4 x0 = tr_read(p), x1 = tr_read(p + 16 * XROW);
-        b[v] = uint4{__builtin_bit_cast(uint2, x0).x, __builtin_bit_cast(uint2, x0).y, __builtin_bit_cast(uint2, x1).x,
-                     __builtin_bit_cast(uint2, x1).y};
-      }
-#pragma unroll
-      for (int pl = NP - 1; pl >= 0; --pl) {
-#pragma unroll
-        for (int u = 0; u < FN; ++u) {
-          const unsigned char* p = Y + pl * YSTAGE + (ms + tr) * YROW + 32 * ((wn / 16 + u) ^ (tr & 7)) + tc;
-          const shortx4 y0 = tr_read(p), y1 = tr_read(p + 16 * YROW);
-          const uint4 a = uint4{__builtin_bit_cast(uint2, y0).x, __builtin_bit_cast(uint2, y0).y,
-                                __builtin_bit_cast(uint2, y1).x, __builtin_bit_cast(uint2, y1).y};
-#pragma unroll
-          for (int v = 0; v < FK; ++v) acc[u][v] = Mac<F16 ? LOW_F16 : LOW_BF16>::mac(b[v], a, acc[u][v]);
+      for (int p = 0; p < PH; ++p) {
+        if (p + 1 < PH) {
+          if (p == PH - 2) store_xy(t + 1);
+          read(t, p + 1, (p + 1) & 1, (p + 1) / (NP * NG));
+        } else {
+          staged_barrier();
+          if (t + 2 < total) {
+            load_x(t + 2);
+            stage_y(t + 2);
+          }
+          read(t + 1, 0, PH & 1, NH == 1 ? 1 : 0);
         }
+        multiply(p);
       }
+      if (PH & 1)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) a[0][u] = a[1][u];
+      if (NH == 1)
+#pragma unroll
+        for (int v = 0; v < FK; ++v) b[0][v] = b[1][v];
     }
-    if (t + 1 < total) store_x(t + 1);  // the other half of LDS: last read before this pass's barrier
+    read(total - 1, 0, 0, 0);  // again: kept across the loop's end, the operands would not fit the registers
+#pragma unroll
+    for (int p = 0; p < PH; ++p) {
+      if (p + 1 < PH) read(total - 1, p + 1, (p + 1) & 1, (p + 1) / (NP * NG));
+      multiply(p);
+    }
   }
   matrix_drain();
-  float* part = g.part + (int64_t)blockIdx.z * g.N * g.K;
   const int i = j16;
+  float* part = g.part + (int64_t)blockIdx.z * g.N * g.K;
+  const bool vec = g.K % 4 == 0 && (reinterpret_cast<uintptr_t>(g.dw) & (DT == NC_F32 ? 15 : 7)) == 0;
 #pragma unroll
   for (int u = 0; u < FN; ++u) {
     const int64_t n = n0 + wn + 16 * u + i;
-    if (n >= g.N) continue;
 #pragma unroll
     for (int v = 0; v < FK; ++v) {
-      const int64_t k = k0 + wk + 16 * v + 4 * q;
-      float* p = part + n * g.K + k;
-      if (k + 4 <= g.K && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        *reinterpret_cast<floatx4*>(p) = acc[u][v];
-      } else {
+      const int64_t k = k0 + wk + 16 * v + 4 * q, at = n * g.K + k;
+      if (n >= g.N || k >= g.K) continue;
+      const floatx4 c = acc[u][v];
+      if (!g.dw || DT == NC_F32) {
+        float* p = (g.dw ? reinterpret_cast<float*>(g.dw) : part) + at;
+        if (vec) {
+          *reinterpret_cast<floatx4*>(p) = c;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (k + e < g.K) p[e] = acc[u][v][e];
+          for (int e = 0; e < 4; ++e)
+            if (k + e < g.K) p[e] = c[e];
+        }
+      } else {
+        uint16_t* p = reinterpret_cast<uint16_t*>(g.dw) + at;
+        uint16_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = f32_elem<DT>(c[e]);
+        if (vec) {
+          *reinterpret_cast<uint2*>(p) = uint2{o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16};
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (k + e < g.K) p[e] = o[e];
+        }
       }
     }
   }
+  if (summing) put_col_sums<DT, BN, T>(g, n0, blockIdx.z, ysum, reinterpret_cast<float*>(lds));
 }
 
-constexpr int WG_N = 128, WG_K = 128;
+// tiles of 256 columns (float: 128 of dY, whose three planes take the room) where there are more than 128
+static bool wgrad_wide(int dtype, int64_t N, int64_t K) {
+  return (N > 128 || dtype == NC_F32) && K > 128;
+}
 
-void low_wgrad_splits(int64_t M, int64_t N, int64_t K, int32_t& splits, int64_t& rows_per) {
-  const int64_t tiles = ((N + WG_N - 1) / WG_N) * ((K + WG_K - 1) / WG_K);
-  int64_t want = (512 + tiles - 1) / tiles, most = (M + 255) / 256;
+void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, int32_t& splits, int32_t& pieces, int64_t& rows_per) {
+  const bool wide = wgrad_wide(dtype, N, K);
+  const int64_t tn = wide && dtype != NC_F32 ? 256 : 128, tk = wide ? 256 : 128;
+  const int64_t tiles = tiles_of(N, K, (int)tn, (int)tk);
+  int64_t want = (wide ? 256 : 512) / tiles, most = (M + 127) / 128;
   if (want > most) want = most;
   if (want < 1) want = 1;
   rows_per = round_up((M + want - 1) / want, 64);
   if (rows_per < 64) rows_per = 64;
   splits = (int32_t)((M + rows_per - 1) / rows_per);
   if (splits < 1) splits = 1;
+  pieces = (int32_t)((rows_per + SUM_ROWS - 1) / SUM_ROWS);
 }
 
-template <int NP, bool F16, bool RELU>
+template <int NP, int DT, bool RELU, int TN, int TK, int MS, int WN, int WK, bool VEC>
 static int run_low_wgrad(const LowWgrad& g, hipStream_t s) {
-  constexpr int MS = NP == 3 ? 32 : 64;
-  constexpr int lds = 2 * (NP * MS * 2 * WG_N + MS * 2 * WG_K);
-  const dim3 grid((unsigned)((g.N + WG_N - 1) / WG_N), (unsigned)((g.K + WG_K - 1) / WG_K), (unsigned)g.splits);
-  hipLaunchKernelGGL((k_low_wgrad<NP, F16, RELU, WG_N, WG_K, MS, 2, 2>), grid, dim3(256), lds, s, g);
+  constexpr int lds = 2 * (NP * MS * 2 * TN + MS * 2 * TK);
+  auto kernel = k_low_wgrad<NP, DT, RELU, TN, TK, MS, WN, WK, VEC>;
+  static std::atomic<uint64_t> done{0};
+  if (const int e = allow_lds(kernel, lds, done)) return e;
+  const unsigned kt = g.want_dw ? (unsigned)((g.K + TK - 1) / TK) : 0u;
+  const dim3 grid((unsigned)((g.N + TN - 1) / TN), kt + (g.want_db && !(NP == 3 && kt) ? (unsigned)g.pieces : 0u),
+                  (unsigned)g.splits);
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * WN * WK), lds, s, g);
   return (int)hipGetLastError();
 }
 
+template <int DT, bool RELU>
+static int pick_low_wgrad(const LowWgrad& g, hipStream_t s) {
+  if (wgrad_wide(DT, g.N, g.K)) return run_low_wgrad<1, DT, RELU, 256, 256, 64, 2, 4, true>(g, s);
+  return run_low_wgrad<1, DT, RELU, 128, 128, 64, 2, 2, true>(g, s);
+}
+
+template <bool RELU, bool VEC>
+static int pick_low_wgrad_f(const LowWgrad& g, hipStream_t s) {
+  if (wgrad_wide(NC_F32, g.N, g.K)) return run_low_wgrad<3, NC_F32, RELU, 128, 256, 64, 2, 4, VEC>(g, s);
+  return run_low_wgrad<3, NC_F32, RELU, 128, 128, 32, 2, 2, VEC>(g, s);
+}
+
 int launch_low_wgrad(const LowWgrad& g, hipStream_t s) {
-  if (g.N <= 0 || g.K <= 0) return 0;
-  if (g.planes == 3) return g.relu ? run_low_wgrad<3, false, true>(g, s) : run_low_wgrad<3, false, false>(g, s);
-  if (g.f16) return g.relu ? run_low_wgrad<1, true, true>(g, s) : run_low_wgrad<1, true, false>(g, s);
-  return g.relu ? run_low_wgrad<1, false, true>(g, s) : run_low_wgrad<1, false, false>(g, s);
+  if (g.N <= 0 || g.K <= 0 || (!g.want_dw && !g.want_db)) return 0;
+  switch (g.dtype) {
+    case NC_F16: return g.relu ? pick_low_wgrad<NC_F16, true>(g, s) : pick_low_wgrad<NC_F16, false>(g, s);
+    case NC_BF16: return g.relu ? pick_low_wgrad<NC_BF16, true>(g, s) : pick_low_wgrad<NC_BF16, false>(g, s);
+    case NC_F32: {
+      const bool vec = load8_vec(g.dy, g.ldy, g.N, NC_F32);
+      if (vec) return g.relu ? pick_low_wgrad_f<true, true>(g, s) : pick_low_wgrad_f<false, true>(g, s);
+      return g.relu ? pick_low_wgrad_f<true, false>(g, s) : pick_low_wgrad_f<false, false>(g, s);
+    }
+  }
+  return (int)hipErrorInvalidValue;
 }
 
 }  // namespace nc

@@ -160,6 +160,7 @@ class NcImapPointsArgs(ctypes.Structure):
 NC_F32, NC_F16, NC_BF16 = 0, 1, 2
 NC_CODES_ROW, NC_CODES_GROUP, NC_CODES_RELU = 0, 1, 2
 NC_MAX_INPUTS = 131072
+NC_MAX_STRIDE = 1 << 22
 
 
 class NcCodesArgs(ctypes.Structure):

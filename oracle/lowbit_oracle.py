@@ -12,12 +12,13 @@ GROUP = 32
 
 
 def row_codes(x):
-    """(codes float64 [M, K], scales float32 [M]): s = max(fl32(amax / 127), 2^-126), q the integer
+    """(codes float64 [M, K], scales float32 [M]): s = max(fl32(amax fl32(1 / 127)), 2^-126), q the integer
     nearest to x / s.  The float64 quotient of two float32 numbers is within 2^-53 of the exact
     one, which is a half-integer or at least 2^-49 (relative) from it: no code can differ."""
     x = x.double()
     top = x.abs().amax(1)
-    s = (top / 127).to(torch.float32).clamp_min(torch.finfo(torch.float32).tiny)
+    inv = torch.tensor(1 / 127, dtype=torch.float32).double()  # (the product is exact in float64)
+    s = (top * inv).to(torch.float32).clamp_min(torch.finfo(torch.float32).tiny)
     q = torch.round(x / s.double()[:, None]).clamp(-127, 127)
     bad = ~torch.isfinite(top)
     q[bad] = 0

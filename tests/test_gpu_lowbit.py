@@ -95,7 +95,7 @@ def test_group_codes(m, k, dtype, relu):
 
 def test_codes_next_to_ties_and_at_the_ends():
     """Quotients on and one ulp beside a half, zero rows, the least and the largest numbers."""
-    s = 3.0 / 127
+    s = (torch.tensor(3.0) * torch.tensor(1 / 127, dtype=F32)).item()
     k = torch.arange(-126, 126)
     mid = ((k.double() + 0.5) * torch.tensor(s, dtype=F32).double()).float()
     up, dn = torch.nextafter(mid, torch.full_like(mid, 9.)), torch.nextafter(mid, torch.full_like(mid, -9.))
@@ -178,7 +178,9 @@ def test_quantized_linear_types(m, k, n, dtype, out_dtype, bias):
     product_case(m, k, n, dtype, out_dtype, bias, False, m + n)
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 8192, 2048), (3, 16384, 256), (1024, 768, 1536), (2100, 512, 640), (64, 4096, 4096)])
+@pytest.mark.parametrize("m,k,n", [(1, 8192, 2048), (3, 16384, 256), (1024, 768, 1536), (2100, 512, 640), (64, 4096, 4096),
+                                   (16, 2048, 300), (17, 256, 4100), (700, 250, 517), (300, 2049, 1027), (90, 8200, 33),
+                                   (6000, 96, 2050)])
 def test_quantized_linear_larger(m, k, n):
     product_case(m, k, n, BF16, BF16, F32, True, m)
 
@@ -275,7 +277,8 @@ def test_layer(m, k, n, dtype, relu):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m,k,n", [(5000, 93, 256), (3001, 256, 256), (1024, 1024, 768), (640, 512, 2048)])
+@pytest.mark.parametrize("m,k,n", [(5000, 93, 256), (3001, 256, 256), (1024, 1024, 768), (640, 512, 2048), (70, 1100, 55),
+                                   (64, 55, 4616), (150, 2047, 1033), (1, 4096, 96), (33000, 40, 300), (9000, 300, 130)])
 def test_layer_larger(m, k, n, dtype):
     layer_case(m, k, n, dtype, True, m, bias=m % 2 == 0)
 

@@ -112,7 +112,7 @@ def test_layer_args_validated(lib):
 
     for kw, msg in ((dict(dtype=5), b"dtype"), (dict(rows=-2), b"rows"), (dict(rows=1 << 31), b"2^31"),
                     (dict(inputs=0), b"inputs"), (dict(outputs=L.NC_MAX_INPUTS + 1), b"131072"),
-                    (dict(x_stride=-1), b"stride"), (dict(dy_stride=-1), b"stride")):
+                    (dict(x_stride=-1), b"stride"), (dict(dy_stride=-1), b"stride"), (dict(x_stride=(1 << 22) + 1), b"2^22")):
         a = args(**kw)
         for back in (0, 1):
             assert lib.nc_layer_workspace_bytes(ctypes.byref(a), back) == 0, kw
