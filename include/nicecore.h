@@ -521,6 +521,10 @@ int nc_points_backward(const nc_points_args* args, void* workspace, size_t works
  * (Renderer.py:87).  Replaces Renderer.render_batch_ray (Renderer.py:95-262) with
  * nice=False and Renderer.eval_points (:36-93, decoders(pi, c_grid=None)). */
 #define NC_IMAP_HIDDEN 256
+/* nc_imap_* flag with NC_SAVE_FOR_BACKWARD (ABI v12): the backward keeps the layers' inputs as 8-bit
+ * checkpoints (nc_layer_*) instead of float32: 4.1 KB of workspace a point instead of 9.5 KB.  Outputs, ray
+ * and bias gradients are those of float32 layers; the weight gradients see the checkpoints' values. */
+#define NC_CODED_ACTIVATIONS 256
 typedef struct nc_imap_params {
   const float* fourier_B; /* [3, 93] embedder._B */
   const float* lin_w[4];  /* pts_linears[l].weight: [256, 93], [256, 256] x 3 */
@@ -532,7 +536,7 @@ typedef struct nc_imap_params {
 
 typedef struct nc_imap_render_args {
   int32_t abi_version;   /* NC_ABI_VERSION */
-  int32_t flags;         /* NC_SAVE_FOR_BACKWARD */
+  int32_t flags;         /* NC_SAVE_FOR_BACKWARD | NC_CODED_ACTIVATIONS */
   int64_t n_rays;
   int32_t n_strat;       /* N_samples (configs/imap.yaml:107); N_surface is 0 for iMAP* */
   int32_t n_extra;       /* importance depths merged into the samples (second pass) */
@@ -558,7 +562,7 @@ typedef struct nc_imap_render_args {
 
 typedef struct nc_imap_points_args {
   int32_t abi_version;
-  int32_t flags;         /* NC_SAVE_FOR_BACKWARD */
+  int32_t flags;         /* NC_SAVE_FOR_BACKWARD | NC_CODED_ACTIVATIONS */
   int64_t n_points;
   const double* pts;     /* [P,3] float64 */
   nc_imap_params dec;
@@ -577,8 +581,12 @@ int nc_imap_points_backward(const nc_imap_points_args* args, void* workspace, si
 /* Byte offset inside the workspace of the saved hidden activations h_layer = relu(z)
  * (layer 0..3, [n_points][256] float32, point-major) that nc_imap_points_forward wrote:
  * read-only introspection (the tests score weight gradients against a float64 truth
- * evaluated on the same ReLU branches).  Returns -1 for a bad layer or arguments. */
+ * evaluated on the same ReLU branches).  Returns -1 for a bad layer or arguments, and with
+ * NC_CODED_ACTIVATIONS, which saves no such activations. */
 int64_t nc_imap_points_activation_offset(const nc_imap_points_args* args, int layer);
+/* out[p][0..92] = sin(p.float() @ B), out[p][93..95] = 0: the scene MLP's Fourier features
+ * (decoder.py:26-30) of n_points float64 points, as rows of 96 float32. (ABI v12) */
+int nc_imap_features(const double* pts, int64_t n_points, const float* fourier_B, float* out, void* stream);
 
 /* ---- 8-bit layer operators (ABI v12) ---------------------------------------------
  * Codes are kept in rows of code_stride bytes, a multiple of 128 and at least the number of
@@ -655,7 +663,8 @@ typedef struct nc_layer_args {
   int64_t code_stride;
   const void* dy;      /* backward: [rows][dy_stride] */
   int64_t dy_stride;
-  void* dx;            /* [rows][inputs] */
+  void* dx;            /* [rows][dx_stride] */
+  int64_t dx_stride;
   void* dw;            /* [outputs][inputs] */
   void* db;            /* [outputs] */
 } nc_layer_args;

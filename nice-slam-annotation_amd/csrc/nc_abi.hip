@@ -1231,10 +1231,36 @@ struct ImapWs {
   size_t dmax = 0, z = 0, pts = 0, pf = 0, emb = 0, h = 0, raw = 0, occ = 0, rgb = 0;
   size_t gocc = 0, grgb = 0, dout = 0, dz = 0, demb = 0, dx = 0, dpts = 0, gnorm = 0, wt = 0, total = 0;
   size_t wimg = 0, wflag = 0, wtimg = 0, wtflag = 0;  // split-f16 weight images (k_imap_wimage)
+  // NC_CODED_ACTIVATIONS: checkpoints of the features and h_0..h_3; two activations that the layers write in
+  // turn (forward: z, backward: dz; `demb` holds the features in the forward); the layers' own scratch
+  bool coded = false;
+  size_t code[5] = {}, step[5] = {}, turn[2] = {}, layer = 0, layer_bytes = 0;
 };
 
-void imap_layout(int64_t N, int64_t P, bool rays, bool bwd, ImapWs& w) {
+constexpr int64_t EMB_CODES = 128;  // code_stride of the 93 features
+// layer l (0..3 hidden, 4 output) of the coded MLP
+nc_layer_args imap_layer(int l, int64_t P) {
+  nc_layer_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.abi_version = NC_ABI_VERSION;
+  a.dtype = NC_F32;
+  a.relu = l > 0;
+  a.rows = P;
+  a.inputs = l == 0 ? EMB : IH;
+  a.outputs = l == 4 ? 4 : IH;
+  a.x_stride = l == 0 ? EMBP : IH;
+  a.w_stride = a.inputs;
+  a.y_stride = a.outputs;
+  a.code_stride = l == 0 ? EMB_CODES : IH;
+  a.dy_stride = a.outputs;
+  a.dx_stride = a.x_stride;
+  return a;
+}
+
+void imap_layout(int64_t N, int64_t P, bool rays, bool bwd, bool coded, ImapWs& w) {
   size_t o = 0;
+  coded = coded && bwd;
+  w.coded = coded;
   auto take = [&](size_t& f, size_t bytes) { f = o; o = align256(o + bytes); };
   if (rays) {
     take(w.dmax, 4);
@@ -1242,10 +1268,23 @@ void imap_layout(int64_t N, int64_t P, bool rays, bool bwd, ImapWs& w) {
   }
   take(w.pts, rays ? (size_t)P * 24 : 0);
   take(w.pf, (size_t)P * 16);
-  take(w.emb, (size_t)P * EMBP * 4);
-  take(w.h, (size_t)4 * P * IH * 4);
-  take(w.wimg, (size_t)3 * IH * imap_wimage_row(IH));  // W_1..3 images, forward B
-  take(w.wflag, 16);
+  if (coded) {
+    for (int l = 0; l < 5; ++l) {
+      const nc_layer_args a = imap_layer(l, P);
+      take(w.code[l], (size_t)P * a.code_stride);
+      take(w.step[l], (size_t)P * (a.code_stride / CODE_GROUP));
+      const size_t f = nc_layer_workspace_bytes(&a, 0), b = nc_layer_workspace_bytes(&a, 1);
+      w.layer_bytes = f > w.layer_bytes ? f : w.layer_bytes;
+      w.layer_bytes = b > w.layer_bytes ? b : w.layer_bytes;
+    }
+    for (int k = 0; k < 2; ++k) take(w.turn[k], (size_t)P * IH * 4);
+    take(w.layer, w.layer_bytes);
+  } else {
+    take(w.emb, (size_t)P * EMBP * 4);
+    take(w.h, (size_t)4 * P * IH * 4);
+    take(w.wimg, (size_t)3 * IH * imap_wimage_row(IH));  // W_1..3 images, forward B
+    take(w.wflag, 16);
+  }
   take(w.raw, (size_t)P * 16);
   if (rays) {
     take(w.occ, (size_t)P * 4);
@@ -1258,13 +1297,15 @@ void imap_layout(int64_t N, int64_t P, bool rays, bool bwd, ImapWs& w) {
       take(w.gnorm, (size_t)N * 4);
       take(w.dout, (size_t)P * 16);
     }
-    take(w.dz, (size_t)4 * P * IH * 4);
     take(w.demb, (size_t)P * EMBP * 4);
     take(w.dx, (size_t)P * EMBP * 4);
     take(w.dpts, (size_t)P * 24);
-    take(w.wt, (size_t)(3 * IH + EMB) * IH * 4);  // W_1..3^T, W_0^T: the dX GEMMs' k-contiguous B
-    take(w.wtimg, (size_t)(3 * IH + EMB) * imap_wimage_row(IH));  // and their split-f16 images
-    take(w.wtflag, 16);
+    if (!coded) {
+      take(w.dz, (size_t)4 * P * IH * 4);
+      take(w.wt, (size_t)(3 * IH + EMB) * IH * 4);  // W_1..3^T, W_0^T: the dX GEMMs' k-contiguous B
+      take(w.wtimg, (size_t)(3 * IH + EMB) * imap_wimage_row(IH));  // and their split-f16 images
+      take(w.wtflag, 16);
+    }
   }
   w.total = o;
 }
@@ -1297,8 +1338,64 @@ int run_gemm(const ImapGemm& g, bool a_km, bool b_kn, hipStream_t s) {
   return check_hip(timed(KID_IMAP_GEMM, s, [&] { return launch_imap_gemm(g, a_km, b_kn, s); }), "k_imap_gemm");
 }
 
+// the same MLP as a chain of checkpointed layers: z_0 = emb W_0^T + b_0, z_l = relu(z_{l-1}) W_l^T + b_l,
+// raw = relu(z_3) W_out^T + b_out; layer l keeps its input's codes
+int imap_coded_forward(const nc_imap_params& d, int64_t P, void* ws, const ImapWs& w, float* raw, hipStream_t s) {
+  float* emb = at<float>(ws, w.demb);
+  if (int e = check_hip(timed(KID_IMAP_FOURIER, s, [&] { return launch_imap_embed(at<float4>(ws, w.pf), d.fourier_B, P, emb, s); }),
+                        "k_imap_embed"))
+    return e;
+  const float* x = emb;
+  for (int l = 0; l < 5; ++l) {
+    nc_layer_args a = imap_layer(l, P);
+    a.x = x;
+    a.w = l == 4 ? d.out_w : d.lin_w[l];
+    a.bias = l == 4 ? d.out_b : d.lin_b[l];
+    a.y = l == 4 ? raw : at<float>(ws, w.turn[l & 1]);
+    a.codes = at<uint8_t>(ws, w.code[l]);
+    a.steps = at<uint8_t>(ws, w.step[l]);
+    if (int e = nc_layer_forward(&a, at<void>(ws, w.layer), w.layer_bytes, s)) return e;
+    x = static_cast<const float*>(a.y);
+  }
+  return 0;
+}
+
+int imap_coded_backward(const nc_imap_params& d, int64_t P, void* ws, const ImapWs& w, const float* dout, double* dpts,
+                        hipStream_t s) {
+  const ImapOff off;
+  float* demb = at<float>(ws, w.demb);
+  float* dx = d.grad ? at<float>(ws, w.dx) : nullptr;
+  const float* dy = dout;
+  for (int l = 4; l >= 0; --l) {
+    nc_layer_args a = imap_layer(l, P);
+    a.dy = dy;
+    a.w = l == 4 ? d.out_w : d.lin_w[l];
+    a.codes = at<uint8_t>(ws, w.code[l]);
+    a.steps = at<uint8_t>(ws, w.step[l]);
+    if (l > 0) a.dx = at<float>(ws, w.turn[l & 1]);
+    else if (dpts || dx) a.dx = demb;
+    if (d.grad) {
+      a.dw = d.grad + (l == 4 ? off.wo : off.w[l]);
+      a.db = d.grad + (l == 4 ? off.bo : off.b[l]);
+    }
+    if (int e = nc_layer_backward(&a, at<void>(ws, w.layer), w.layer_bytes, s)) return e;
+    dy = static_cast<const float*>(a.dx);
+  }
+  if (!dpts && !dx) return 0;
+  const float4* pf = at<float4>(ws, w.pf);
+  if (int e = check_hip(timed(KID_IMAP_FOURIER, s, [&] { return launch_imap_fourier_bwd(pf, d.fourier_B, P, demb, dx, dpts, s); }),
+                        "k_imap_fourier_bwd"))
+    return e;
+  if (!d.grad) return 0;
+  if (int e = check_hip(launch_imap_zero(reinterpret_cast<uint32_t*>(d.grad + off.B), 3 * EMB, s), "k_imap_zero")) return e;
+  ImapGemm g = gemm(reinterpret_cast<const float*>(pf), 4, dx, EMBP, d.grad + off.B, EMB, 3, EMB, P);  // dB = pf^T dx
+  g.atomic = 1;
+  return run_gemm(g, true, true, s);
+}
+
 // forward MLP over P points whose p.float() is in ws.pf: emb, h_0..h_3, raw
 int imap_mlp_forward(const nc_imap_params& d, int64_t P, void* ws, const ImapWs& w, float* raw, hipStream_t s) {
+  if (w.coded) return imap_coded_forward(d, P, ws, w, raw, s);
   const float4* pf = at<float4>(ws, w.pf);
   float* emb = at<float>(ws, w.emb);
   float* h = at<float>(ws, w.h);
@@ -1344,6 +1441,7 @@ int imap_mlp_forward(const nc_imap_params& d, int64_t P, void* ws, const ImapWs&
 // weight gradients (overwritten into d.grad) when d.grad != NULL
 int imap_mlp_backward(const nc_imap_params& d, int64_t P, void* ws, const ImapWs& w, const float* dout, double* dpts,
                       hipStream_t s) {
+  if (w.coded) return imap_coded_backward(d, P, ws, w, dout, dpts, s);
   const float4* pf = at<float4>(ws, w.pf);
   const float* emb = at<float>(ws, w.emb);
   const float* h = at<float>(ws, w.h);
@@ -1402,7 +1500,7 @@ int imap_mlp_backward(const nc_imap_params& d, int64_t P, void* ws, const ImapWs
   }
   if (!d.grad) return 0;
   const ImapOff off;
-  if (int e = check_hip(hipMemsetAsync(d.grad, 0, (size_t)off.total * 4, s), "grad memset")) return e;
+  if (int e = check_hip(launch_imap_zero(reinterpret_cast<uint32_t*>(d.grad), off.total, s), "k_imap_zero")) return e;
   float* G = d.grad;
   auto dw = [&](const float* A, int64_t lda, int64_t M, const float* B, int64_t ldb, int64_t N, float* C) {
     ImapGemm g = gemm(A, lda, B, ldb, C, N, M, N, P);
@@ -1424,14 +1522,14 @@ int imap_render_prepare(const nc_imap_render_args* a, ImapWs& w, int64_t& P, int
   if (!a) return fail(-1, "nicecore: args is NULL");
   if (a->abi_version != NC_ABI_VERSION) return fail(-2, "nicecore: ABI version mismatch");
   if (a->n_rays < 0) return fail(-1, "nicecore: n_rays < 0");
-  if (a->flags & ~NC_SAVE_FOR_BACKWARD) return fail(-1, "nicecore: unknown flags");
+  if (a->flags & ~(NC_SAVE_FOR_BACKWARD | NC_CODED_ACTIVATIONS)) return fail(-1, "nicecore: unknown flags");
   if (a->n_extra < 0 || (a->n_extra > 0 && !a->z_extra && a->n_rays > 0))
     return fail(-1, "nicecore: n_extra > 0 needs z_extra");
   if (a->n_strat < 1 || a->n_strat + a->n_extra > NC_MAX_SAMPLES)
     return fail(-1, "nicecore: need 1 <= N_samples, N_samples + n_extra <= 64");
   S = a->n_strat + a->n_extra;
   P = a->n_rays * S;
-  imap_layout(a->n_rays, P, true, (a->flags & NC_SAVE_FOR_BACKWARD) != 0, w);
+  imap_layout(a->n_rays, P, true, (a->flags & NC_SAVE_FOR_BACKWARD) != 0, (a->flags & NC_CODED_ACTIVATIONS) != 0, w);
   return 0;
 }
 
@@ -1483,8 +1581,8 @@ int imap_points_prepare(const nc_imap_points_args* a, ImapWs& w) {
   if (!a) return fail(-1, "nicecore: args is NULL");
   if (a->abi_version != NC_ABI_VERSION) return fail(-2, "nicecore: ABI version mismatch");
   if (a->n_points < 0) return fail(-1, "nicecore: n_points < 0");
-  if (a->flags & ~NC_SAVE_FOR_BACKWARD) return fail(-1, "nicecore: unknown flags");
-  imap_layout(0, a->n_points, false, (a->flags & NC_SAVE_FOR_BACKWARD) != 0, w);
+  if (a->flags & ~(NC_SAVE_FOR_BACKWARD | NC_CODED_ACTIVATIONS)) return fail(-1, "nicecore: unknown flags");
+  imap_layout(0, a->n_points, false, (a->flags & NC_SAVE_FOR_BACKWARD) != 0, (a->flags & NC_CODED_ACTIVATIONS) != 0, w);
   return 0;
 }
 
@@ -1558,8 +1656,18 @@ int nc_imap_render_backward(const nc_imap_render_args* a, void* ws, size_t ws_by
 
 int64_t nc_imap_points_activation_offset(const nc_imap_points_args* a, int layer) {
   ImapWs w;
-  if (layer < 0 || layer > 3 || imap_points_prepare(a, w)) return -1;
+  if (layer < 0 || layer > 3 || imap_points_prepare(a, w) || w.coded) return -1;
   return (int64_t)(w.h + (size_t)layer * a->n_points * IH * 4);
+}
+
+int nc_imap_features(const double* pts, int64_t n_points, const float* fourier_B, float* out, void* stream) {
+  if (n_points < 0) return fail(-1, "nicecore: n_points < 0");
+  if (n_points == 0) return 0;
+  if (!pts || !fourier_B || !out) return fail(-1, "nicecore: NULL pts, fourier_B or output");
+  if (n_points > INT32_MAX) return fail(-1, "nicecore: n_points must be below 2^31");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return check_hip(timed(KID_IMAP_FOURIER, s, [&] { return launch_imap_features(pts, fourier_B, n_points, out, s); }),
+                   "k_imap_features");
 }
 
 size_t nc_imap_points_workspace_bytes(const nc_imap_points_args* a) {
@@ -1714,7 +1822,8 @@ int layer_check(const nc_layer_args* a) {
   if (a->abi_version != NC_ABI_VERSION) return fail(-2, "nicecore: ABI version mismatch");
   if (!dtype_ok(a->dtype)) return fail(-1, "nicecore: unknown dtype");
   if (int e = check_matrix(a->rows, a->inputs, a->outputs)) return e;
-  if (a->x_stride < 0 || a->w_stride < 0 || a->dy_stride < 0 || a->y_stride < 0) return fail(-1, "nicecore: negative row stride");
+  if (a->x_stride < 0 || a->w_stride < 0 || a->dy_stride < 0 || a->y_stride < 0 || a->dx_stride < 0)
+    return fail(-1, "nicecore: negative row stride");
   if (a->x_stride > NC_MAX_STRIDE || a->dy_stride > NC_MAX_STRIDE) return fail(-1, "nicecore: row strides must not exceed 2^22 elements");
   return 0;
 }
@@ -1951,7 +2060,7 @@ int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* s
     if (int e = check_hip(timed(KID_CODES, s, [&] { return launch_transpose(t, s); }), "transpose")) return e;
     LowGemm g = layer_gemm(a->dtype, a->dy, nullptr, w, ws, a->rows, a->inputs, a->outputs);
     g.out = a->dx;
-    g.ldc = a->inputs;
+    g.ldc = a->dx_stride;
     if (a->relu) {
       g.mask = a->codes;
       g.ldm = a->code_stride;

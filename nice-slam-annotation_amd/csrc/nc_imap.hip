@@ -532,6 +532,26 @@ __global__ void k_imap_pf(const double* pts, int64_t P, float4* pf) {
   pf[p] = float4{(float)pts[p * 3 + 0], (float)pts[p * 3 + 1], (float)pts[p * 3 + 2], 0.f};
 }
 
+// k_imap_pf and k_imap_embed in one: the features of float64 points
+__global__ void k_imap_features(const double* pts, const float* B, int64_t P, float* emb) {
+  const int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (e >= P * EMBP) return;
+  const int64_t p = e / EMBP;
+  const int j = (int)(e - p * EMBP);
+  float v = 0.f;
+  if (j < EMB) {
+    const float fx = (float)pts[p * 3], fy = (float)pts[p * 3 + 1], fz = (float)pts[p * 3 + 2];
+    v = sinf(__builtin_fmaf(fz, B[2 * EMB + j], __builtin_fmaf(fy, B[EMB + j], fx * B[j])));
+  }
+  emb[e] = v;
+}
+
+// a fill that a graph may capture (memset nodes have given wrong results on later replays)
+__global__ void k_imap_zero(uint32_t* p, int64_t n) {
+  const int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (e < n) p[e] = 0u;
+}
+
 static inline unsigned blocks_of(int64_t n, int b) { return (unsigned)((n + b - 1) / b); }
 
 // the split-f16 kernel takes the layer GEMMs whose operands are both k-contiguous
@@ -619,7 +639,7 @@ int launch_imap_out_bwd(const float* dout, const float* wo, const float* h3, int
 
 int launch_imap_wimage(const ImapWImage& w, int n, hipStream_t s) {
   if (n <= 0) return 0;
-  if (int e = (int)hipMemsetAsync(w.flag, 0, 4 * sizeof(uint32_t), s)) return e;
+  if (int e = launch_imap_zero(w.flag, 4, s)) return e;
   int64_t most = 0;
   for (int z = 0; z < n; ++z) {
     const int64_t c = (int64_t)w.N[z] * ((w.K[z] + 31) / 32) * 4;
@@ -664,6 +684,18 @@ int launch_imap_split(const float* raw, int64_t P, float* occ, float* rgb, hipSt
 int launch_imap_dout(const float* gocc, const float* grgb, int64_t P, float* dout, hipStream_t s) {
   if (P <= 0) return 0;
   hipLaunchKernelGGL(k_imap_dout, dim3(blocks_of(P, 256)), dim3(256), 0, s, gocc, grgb, P, dout);
+  return (int)hipGetLastError();
+}
+
+int launch_imap_features(const double* pts, const float* B, int64_t P, float* emb, hipStream_t s) {
+  if (P <= 0) return 0;
+  hipLaunchKernelGGL(k_imap_features, dim3(blocks_of(P * EMBP, 256)), dim3(256), 0, s, pts, B, P, emb);
+  return (int)hipGetLastError();
+}
+
+int launch_imap_zero(uint32_t* p, int64_t n, hipStream_t s) {
+  if (n <= 0) return 0;
+  hipLaunchKernelGGL(k_imap_zero, dim3(blocks_of(n, 256)), dim3(256), 0, s, p, n);
   return (int)hipGetLastError();
 }
 

@@ -259,6 +259,8 @@ int launch_imap_colsum(const float* X, int64_t P, int ld, int ncols, float* out,
 int launch_imap_split(const float* raw, int64_t P, float* occ, float* rgb, hipStream_t s);
 int launch_imap_dout(const float* gocc, const float* grgb, int64_t P, float* dout, hipStream_t s);
 int launch_imap_pf(const double* pts, int64_t P, float4* pf, hipStream_t s);
+int launch_imap_features(const double* pts, const float* B, int64_t P, float* emb, hipStream_t s);
+int launch_imap_zero(uint32_t* p, int64_t n, hipStream_t s);
 
 struct ParamReduceCtx {
   int32_t n_jobs;

@@ -17,6 +17,7 @@ NC_SAVE_FOR_BACKWARD = 1
 NC_DETERMINISTIC = 2
 NC_SAVE_POINT_JACOBIAN = 4
 NC_DEFER_PARAM_GRADS = 8
+NC_CODED_ACTIVATIONS = 256
 
 
 def NC_NO_WEIGHT_GRAD(kind: int) -> int:
@@ -182,7 +183,7 @@ class NcLayerArgs(ctypes.Structure):
                 ("rows", c_int64), ("inputs", c_int64), ("outputs", c_int64), ("x", c_void_p), ("x_stride", c_int64),
                 ("w", c_void_p), ("w_stride", c_int64), ("bias", c_void_p), ("y", c_void_p), ("y_stride", c_int64),
                 ("codes", c_void_p), ("steps", c_void_p), ("code_stride", c_int64),
-                ("dy", c_void_p), ("dy_stride", c_int64), ("dx", c_void_p), ("dw", c_void_p), ("db", c_void_p)]
+                ("dy", c_void_p), ("dy_stride", c_int64), ("dx", c_void_p), ("dx_stride", c_int64), ("dw", c_void_p), ("db", c_void_p)]
 
 
 NC_ADAM_DENSE = 0
@@ -228,6 +229,7 @@ EXPORTS = {
     "nc_layer_workspace_bytes": (c_size_t, [POINTER(NcLayerArgs), c_int]),
     "nc_layer_forward": (c_int, [POINTER(NcLayerArgs), c_void_p, c_size_t, c_void_p]),
     "nc_layer_backward": (c_int, [POINTER(NcLayerArgs), c_void_p, c_size_t, c_void_p]),
+    "nc_imap_features": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
     "nc_sparse_merge_temp_bytes": (c_size_t, [c_int64, c_int64]),
     "nc_sparse_rows_merge": (c_int, [POINTER(NcSparseRows), POINTER(NcSparseRows), c_void_p, c_void_p,
                                      c_int32, c_int64, c_void_p, c_size_t, c_void_p]),

@@ -87,6 +87,11 @@ class MLP(nn.Module):
         self.sample_mode = sample_mode
         self.leaky = leaky
 
+    def quantize(self):
+        """This iMAP* MLP in 8 bits for queries without gradients (imap.QuantizedMLP)."""
+        from .imap import QuantizedMLP
+        return QuantizedMLP(self)
+
     def forward(self, p, c_grid=None):
         """MLP.forward (decoder.py:190-219) for the iMAP* scene MLP (c_dim = 0, hidden 256,
         4 blocks, no skip: get_model(nice=False)) on the HIP kernels (nicecore.imap).  The

@@ -50,6 +50,15 @@ def imap_params(module) -> list:
     return ps
 
 
+ACTIVATIONS = {None: 0, "float32": 0, "int8": L.NC_CODED_ACTIVATIONS}
+
+
+def _activation_flag(activations) -> int:
+    if activations not in ACTIVATIONS:
+        raise L.NiceCoreError(f"activations must be 'float32' or 'int8', got {activations!r}")
+    return ACTIVATIONS[activations] if torch.is_grad_enabled() else 0  # (no backward, nothing to keep)
+
+
 def _fill_params(d: L.NcImapParams, params, device):
     for p in params:
         if p.device != device or p.dtype != torch.float32 or not p.is_contiguous():
@@ -87,7 +96,7 @@ class ImapRenderFn(torch.autograd.Function):
         a = L.NcImapRenderArgs()
         a.abi_version = L.NC_ABI_VERSION
         need = ctx.needs_input_grad
-        a.flags = L.NC_SAVE_FOR_BACKWARD if any(need[1:3] + need[4:]) else 0
+        a.flags = L.NC_SAVE_FOR_BACKWARD | spec.get("coded", 0) if any(need[1:3] + need[4:]) else 0
         a.n_rays, a.n_strat = N, spec["n_strat"]
         a.rays_o, a.rays_d = rays_o.data_ptr(), rays_d.data_ptr()
         for k, row in enumerate(spec["bound"]):
@@ -159,20 +168,21 @@ class ImapRenderFn(torch.autograd.Function):
 
 
 class ImapEvalFn(torch.autograd.Function):
-    """Inputs (p, *params) -> raw [P,4] float32 (no bound mask)."""
+    """Inputs (coded, p, *params) -> raw [P,4] float32 (no bound mask); ``coded``: the flag of
+    _activation_flag."""
 
     @staticmethod
-    def forward(ctx, p, *params):
+    def forward(ctx, coded, p, *params):
         lib = L.load()
         device = p.device
         if device.type != "cuda":
             raise L.NiceCoreError("nicecore evaluates on a HIP device; points are on " + str(device))
-        _refuse_nondeterministic(any(ctx.needs_input_grad[1:]))
+        _refuse_nondeterministic(any(ctx.needs_input_grad[2:]))
         pts = p.detach().reshape(-1, 3).double().contiguous()
         P = pts.shape[0]
         a = L.NcImapPointsArgs()
         a.abi_version = L.NC_ABI_VERSION
-        a.flags = L.NC_SAVE_FOR_BACKWARD if any(ctx.needs_input_grad) else 0
+        a.flags = L.NC_SAVE_FOR_BACKWARD | coded if any(ctx.needs_input_grad) else 0
         a.n_points, a.pts = P, pts.data_ptr()
         _fill_params(a.dec, params, device)
         raw = torch.empty(P, 4, device=device, dtype=torch.float32)
@@ -195,10 +205,10 @@ class ImapEvalFn(torch.autograd.Function):
         device = pts.device
         gr = g_raw.detach().float().contiguous()
         a.g_raw = gr.data_ptr()
-        g_pts = torch.empty_like(pts) if need[0] else None
+        g_pts = torch.empty_like(pts) if need[1] else None
         a.g_pts = g_pts.data_ptr() if g_pts is not None else None
         flat = None
-        if any(need[1:]):
+        if any(need[2:]):
             flat = torch.zeros(lib.nc_imap_param_count(), device=device, dtype=torch.float32)
             a.dec.grad = flat.data_ptr()
         if a.n_points > 0:
@@ -207,24 +217,75 @@ class ImapEvalFn(torch.autograd.Function):
                     "nc_imap_points_backward")
         a.dec.grad = None
         gp = g_pts.to(ctx.p_dtype).reshape(ctx.p_shape) if g_pts is not None else None
-        return (gp, *_param_grads(flat, params, need[1:]))
+        return (None, gp, *_param_grads(flat, params, need[2:]))
 
 
-def eval_points(module, p):
-    """MLP.forward(p, c_grid=None) of the iMAP* MLP: raw [P,4]."""
-    return ImapEvalFn.apply(p, *imap_params(module))
+def eval_points(module, p, activations=None):
+    """MLP.forward(p, c_grid=None) of the iMAP* MLP: raw [P,4].  ``activations``: see render_rays.
+    ``module`` may be a QuantizedMLP (no gradient)."""
+    if isinstance(module, QuantizedMLP):
+        return module(p)
+    return ImapEvalFn.apply(_activation_flag(activations), p, *imap_params(module))
 
 
-def render_rays(module, rays_o, rays_d, bound, gt_depth=None, n_strat=32, n_importance=0, depth_max=None):
+class QuantizedMLP:
+    """The iMAP* MLP held in 8 bits, for queries without gradients (meshing, rendering points): every
+    layer's weight as quantize_rows codes (nicecore.lowbit), made once from ``module``'s current
+    parameters, and every layer a quantized_linear with the ReLU in its epilogue.  Takes the
+    module's place in eval_points and Renderer.eval_points.  Hidden activations are bfloat16."""
+
+    def __init__(self, module):
+        from .lowbit import quantize_rows
+        ps = [p.detach() for p in imap_params(module)]
+        for p in ps:
+            if p.device.type != "cuda" or p.dtype != torch.float32:
+                raise L.NiceCoreError("iMAP* parameters must be float32 on a HIP device")
+        self.fourier_B = ps[0].contiguous().clone()
+        w0 = torch.nn.functional.pad(ps[1], (0, 3))  # the features come as rows of 96, three of them 0
+        self.weights = [quantize_rows(w) for w in (w0, ps[3], ps[5], ps[7], ps[9])]
+        self.biases = [b.clone() for b in (ps[2], ps[4], ps[6], ps[8], ps[10])]
+        self.device = ps[0].device
+
+    def features(self, p):
+        """sin(p.float() @ B) (decoder.py:26-30) as [P, 96] float32, the last three columns 0."""
+        from .lowbit import _on
+        if p.device != self.device:
+            raise L.NiceCoreError(f"points are on {p.device}, the quantised MLP on {self.device}")
+        if p.requires_grad and torch.is_grad_enabled():
+            raise L.NiceCoreError("a QuantizedMLP has no gradient: call it under torch.no_grad() or with p.detach()")
+        pts = p.detach().reshape(-1, 3).double().contiguous()
+        out = torch.empty(pts.shape[0], 96, device=self.device, dtype=torch.float32)
+        with _on(self.device):
+            L.check(L.load().nc_imap_features(pts.data_ptr(), pts.shape[0], self.fourier_B.data_ptr(), out.data_ptr(),
+                                              L.raw_stream(self.device)), "nc_imap_features")
+        return out
+
+    def __call__(self, p):
+        from .lowbit import quantized_linear
+        h = self.features(p)
+        with torch.no_grad():
+            for l, (w, b) in enumerate(zip(self.weights, self.biases)):
+                last = l == 4
+                h = quantized_linear(h, w, b, relu=not last, out_dtype=torch.float32 if last else torch.bfloat16)
+        return h
+
+
+def render_rays(module, rays_o, rays_d, bound, gt_depth=None, n_strat=32, n_importance=0, depth_max=None,
+                activations=None):
     """Renderer.render_batch_ray with nice=False, occupancy=False, N_surface=0, lindisp=False,
     perturb=0 (configs/imap.yaml:106-111); N_importance > 0 runs the forward-only first pass,
-    sample_pdf (det=True) and the differentiable second pass (Renderer.py:239-259)."""
+    sample_pdf (det=True) and the differentiable second pass (Renderer.py:239-259).
+
+    ``activations``: what the backward keeps of the layers' inputs, 'float32' (default) or 'int8':
+    8-bit checkpoints (nicecore.lowbit.checkpointed_linear), 4.1 KB of workspace a point instead of
+    9.5 KB; the weight gradients then see the checkpoints' values."""
     from .ops import sample_pdf
     from .render_fn import _bound_rows
     if n_strat + n_importance > L.NC_MAX_SAMPLES:
         raise L.NiceCoreError("nicecore supports N_samples + N_importance <= 64")
     params = imap_params(module)
-    spec = {"n_strat": n_strat, "bound": _bound_rows(bound), "depth_max": depth_max}
+    spec = {"n_strat": n_strat, "bound": _bound_rows(bound), "depth_max": depth_max,
+            "coded": _activation_flag(activations)}
     if n_importance > 0:
         N = rays_o.shape[0]
         z = torch.empty(N, n_strat, device=rays_o.device, dtype=torch.float64)

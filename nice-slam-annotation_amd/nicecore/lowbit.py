@@ -262,8 +262,8 @@ class _CheckpointedLinear(torch.autograd.Function):
             ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
             with _on(dev):
                 L.check(lib.nc_layer_forward(ref, ws.data_ptr(), nbytes, L.raw_stream(dev)), "nc_layer_forward")
-        ctx.save_for_backward(weight if need[0] else None, kept)
-        ctx.args, ctx.shape, ctx.dtype = a, x.shape, x.dtype
+        ctx.save_for_backward(weight if need[0] else None)  # (checked for changes in place)
+        ctx.kept, ctx.args, ctx.shape, ctx.dtype = kept, a, x.shape, x.dtype
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], outputs)
 
     @staticmethod
@@ -272,8 +272,8 @@ class _CheckpointedLinear(torch.autograd.Function):
             return None, None, None, None
         if torch.is_grad_enabled():
             raise L.NiceCoreError("checkpointed_linear has no second derivative (backward with create_graph=True)")
-        weight, kept = ctx.saved_tensors
-        a, dtype = ctx.args, ctx.dtype
+        weight, = ctx.saved_tensors
+        kept, a, dtype = ctx.kept, ctx.args, ctx.dtype
         rows, inputs, outputs, stride = a.rows, a.inputs, a.outputs, a.code_stride
         need = ctx.needs_input_grad
         dev = dy.device
@@ -289,7 +289,8 @@ class _CheckpointedLinear(torch.autograd.Function):
             codes = kept.data_ptr()
         b = L.NcLayerArgs(L.NC_ABI_VERSION, a.dtype, a.relu, 0, rows, inputs, outputs, None, 0, w_ptr, w_stride, None, None, 0,
                           codes, codes + rows * stride if codes else None, stride, dy2.data_ptr(), dy_stride,
-                          *(t.data_ptr() if t is not None else None for t in (dx, dw, db)))
+                          dx.data_ptr() if need[0] else None, inputs, dw.data_ptr() if need[1] else None,
+                          db.data_ptr() if need[2] else None)
         lib, ref = L.load(), ctypes.byref(b)
         nbytes = lib.nc_layer_workspace_bytes(ref, 1)
         if nbytes == 0:
@@ -308,4 +309,6 @@ def checkpointed_linear(x, weight, bias=None, relu=False):
     bytes a channel):  dx = (dy W) [x > 0 if relu]  and  db  are those of the full layer, dW = dy^T a8
     sees the checkpoint's values.  All tensors have one dtype; sums are held in float32, and a
     float32 product is accurate to float32.  A chain of such layers trains an MLP."""
+    if not torch.is_grad_enabled():  # no backward, no checkpoint (a Function sees the inputs' own requires_grad)
+        x, weight, bias = (t.detach() if isinstance(t, torch.Tensor) else t for t in (x, weight, bias))
     return _CheckpointedLinear.apply(x, weight, bias, bool(relu))

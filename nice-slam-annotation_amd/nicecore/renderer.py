@@ -44,6 +44,9 @@ class Renderer(object):
         # extension: how the decoder parameters get their .grad ("autograd" | "direct",
         # render_fn.param_inputs); absent from the reference configs = the default
         self.param_grads = r.get('param_grads')
+        # extension, iMAP* only: what a backward keeps of the layers' inputs ("float32" | "int8",
+        # imap.render_rays); absent = float32
+        self.activations = r.get('activations')
         self.scale = cfg['scale']
         self.occupancy = cfg['occupancy']
         self.nice = slam.nice
@@ -54,6 +57,8 @@ class Renderer(object):
     def _check_supported(self):
         if not self.nice and (self.lindisp or self.perturb > 0.):
             raise NotImplementedError("nicecore's iMAP* path implements lindisp=False, perturb=0 (configs/imap.yaml)")
+        if self.nice and self.activations not in (None, "float32"):
+            raise NotImplementedError("activations='int8' is the iMAP* MLP's; NICE decoders keep float32 records")
         if self.nice != self.occupancy:
             raise NotImplementedError(
                 "nicecore renders NICE decoders with occupancy=True (configs/nice_slam.yaml) and the "
@@ -72,7 +77,7 @@ class Renderer(object):
         out = None
         s = 0
         for pi in torch.split(p, self.points_batch_size):
-            r = _eval_points(decoders, pi, c, stage) if self.nice else _imap.eval_points(decoders, pi)
+            r = _eval_points(decoders, pi, c, stage) if self.nice else _imap.eval_points(decoders, pi, self.activations)
             if out is None:
                 out = torch.empty(p.shape[0], 4, dtype=r.dtype, device=r.device)
             out[s:s + pi.shape[0]] = r
@@ -100,7 +105,7 @@ class Renderer(object):
             if ray_mask is not None:
                 raise NotImplementedError("ray_mask is the NICE callers' bbox pre-filter (Tracker.py:99, Mapper.py:580)")
             return _imap.render_rays(decoders, rays_o, rays_d, self.bound, gt_depth, self.N_samples,
-                                     self.N_importance, depth_max)
+                                     self.N_importance, depth_max, activations=self.activations)
         return render_rays(decoders, c, rays_o, rays_d, self.bound, stage, gt_depth,
                            self.N_samples, self.N_surface, depth_max, sparse_grads=sparse_grads,
                            n_importance=self.N_importance, perturb=self.perturb, lindisp=self.lindisp,

@@ -93,9 +93,9 @@ def test_qlinear_args_validated(lib):
         assert lib.nc_quantized_linear_workspace_bytes(ctypes.byref(a)) == 0, kw
         assert msg in lib.nc_last_error(), (kw, lib.nc_last_error())
         assert lib.nc_quantized_linear(ctypes.byref(a), 256, 1 << 30, None) == -1
-    a = args()
+    a = args(rows=100, inputs=300, code_stride=384)  # (few rows are encoded within the product)
     n = lib.nc_quantized_linear_workspace_bytes(ctypes.byref(a))
-    assert n >= 4 * 128 + 16
+    assert n >= 100 * 384 + 400
     assert lib.nc_quantized_linear(ctypes.byref(a), 256, n - 1, None) == -1 and b"workspace" in lib.nc_last_error()
     assert lib.nc_quantized_linear(ctypes.byref(a), None, n, None) == -1
     assert lib.nc_quantized_linear(ctypes.byref(args(out=0)), 256, n, None) == -1 and b"NULL" in lib.nc_last_error()
@@ -105,14 +105,14 @@ def test_qlinear_args_validated(lib):
 def test_layer_args_validated(lib):
     def args(**kw):
         a = L.NcLayerArgs(abi_version=L.NC_ABI_VERSION, rows=4, inputs=100, outputs=8, x=16, x_stride=100, w=16, w_stride=100,
-                          y=16, y_stride=8, codes=32, steps=16, code_stride=128, dy=16, dy_stride=8, dx=16, dw=16, db=16)
+                          y=16, y_stride=8, codes=32, steps=16, code_stride=128, dy=16, dy_stride=8, dx=16, dx_stride=100, dw=16, db=16)
         for k, v in kw.items():
             setattr(a, k, v)
         return a
 
     for kw, msg in ((dict(dtype=5), b"dtype"), (dict(rows=-2), b"rows"), (dict(rows=1 << 31), b"2^31"),
                     (dict(inputs=0), b"inputs"), (dict(outputs=L.NC_MAX_INPUTS + 1), b"131072"),
-                    (dict(x_stride=-1), b"stride"), (dict(dy_stride=-1), b"stride"), (dict(x_stride=(1 << 22) + 1), b"2^22")):
+                    (dict(x_stride=-1), b"stride"), (dict(dy_stride=-1), b"stride"), (dict(x_stride=(1 << 22) + 1), b"2^22"), (dict(dx_stride=-1), b"stride")):
         a = args(**kw)
         for back in (0, 1):
             assert lib.nc_layer_workspace_bytes(ctypes.byref(a), back) == 0, kw
@@ -143,3 +143,29 @@ def test_oracle_codes():
     assert byte.item() == 128 and v.tolist() == [[128.0, 0.0, 2.0, -4.0]]
     q, byte, v = LO.group_codes(torch.tensor([[254.0, 0.25, 1.5, -3.0]]), True)
     assert byte.item() == 127 and q.tolist() == [[255.0, 1.0, 3.0, 0.0]] and v.tolist() == [[254.0, 0.0, 2.0, 0.0]]
+
+
+def test_imap_flags_validated(lib):
+    """The iMAP* entries with 8-bit checkpoints: less than half the workspace; other flags are refused."""
+    def points(flags, n=1000):
+        a = L.NcImapPointsArgs(abi_version=L.NC_ABI_VERSION, flags=flags, n_points=n)
+        return lib.nc_imap_points_workspace_bytes(ctypes.byref(a)), a
+    full, _ = points(L.NC_SAVE_FOR_BACKWARD, 200000)
+    coded, a = points(L.NC_SAVE_FOR_BACKWARD | L.NC_CODED_ACTIVATIONS, 200000)
+    assert 0 < coded < full / 2
+    assert lib.nc_imap_points_activation_offset(ctypes.byref(a), 0) == -1
+    assert points(L.NC_CODED_ACTIVATIONS)[0] == points(0)[0]  # nothing to keep
+    assert points(L.NC_DETERMINISTIC)[0] == 0
+    assert lib.nc_imap_features(None, -1, None, None, None) == -1
+    assert lib.nc_imap_features(None, 5, None, None, None) == -1 and b"NULL" in lib.nc_last_error()
+    assert lib.nc_imap_features(None, 0, None, None, None) == 0
+
+
+def test_activation_names_are_checked():
+    from nicecore import decoder as D
+    from nicecore import imap
+    m = D.build_imap(seed=0)
+    with pytest.raises(L.NiceCoreError, match="activations"):
+        imap.eval_points(m, torch.zeros(4, 3), activations="fp8")
+    with pytest.raises(L.NiceCoreError, match="HIP device"):
+        m.quantize()

@@ -32,6 +32,8 @@ def main():
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--mode", default="mapper", choices=["mapper", "tracker"])
     ap.add_argument("--cpu-rays", type=int, default=0)
+    ap.add_argument("--activations", default="float32", choices=["float32", "int8"],
+                    help="what the backward keeps of the layers' inputs")
     args = ap.parse_args()
     from nicecore import _lib as L
     from nicecore import decoder as D
@@ -41,7 +43,8 @@ def main():
     m = D.build_imap(seed=0).cuda()
     with torch.no_grad():
         m.output_linear.bias[3] = 3.0
-    cfg = {"rendering": {"lindisp": False, "perturb": 0.0, "N_samples": 32, "N_surface": 0, "N_importance": 12},
+    cfg = {"rendering": {"lindisp": False, "perturb": 0.0, "N_samples": 32, "N_surface": 0, "N_importance": 12,
+                         "activations": args.activations},
            "scale": 1, "occupancy": False}
     slam = types.SimpleNamespace(nice=False, bound=sc.bound, H=sc.H, W=sc.W, fx=sc.fx, fy=sc.fy, cx=sc.cx, cy=sc.cy)
     r = Renderer(cfg, None, slam)
@@ -66,7 +69,8 @@ def main():
     for _ in range(args.warmup):
         step()
     torch.cuda.synchronize()
-    with L.KernelTimer(["k_imap_gemm", "k_imap_fourier", "k_ray_setup", "k_composite_fwd",
+    torch.cuda.reset_peak_memory_stats()
+    with L.KernelTimer(["k_codes", "k_low_gemm", "k_low_wgrad", "k_imap_gemm", "k_imap_fourier", "k_ray_setup", "k_composite_fwd",
                         "k_composite_bwd", "k_ray_grads", "k_sample_pdf"]) as kt:
         step()
     torch.cuda.synchronize()
@@ -82,11 +86,12 @@ def main():
     # forward over both passes; backward dX (+ dW in mapper mode) over the second pass
     flops = 2 * macs * (P1 + P) + 2 * macs * P * (1 if tracker else 2)
     out = {"workload": f"iMAP* {args.mode} iteration, room0 bound, {args.rays} rays x (32 + 12 importance), "
-                       f"MLP 93-256x4-4 f32", "ms_per_step": round(dt * 1e3, 4),
+                       f"MLP 93-256x4-4 f32, activations kept as {args.activations}",
+           "peak_memory_mb": round(torch.cuda.max_memory_allocated() / 1e6, 1), "ms_per_step": round(dt * 1e3, 4),
            "rays_per_s": round(args.rays / dt, 1),
            "kernels_ms": {k: round(v[0], 4) for k, v in kt.result.items()},
            "gemm_launches": kt.result.get("k_imap_gemm", (0, 0))[1],
-           "gemm_tflops": round(flops / (gemm_ms * 1e-3) / 1e12, 2) if gemm_ms else None,
+           "gemm_tflops": round(flops / (gemm_ms * 1e-3) / 1e12, 2) if gemm_ms and args.activations == "float32" else None,
            "mfma_peak_tflops": F32_MFMA_PEAK_TFLOPS}
     if out["gemm_tflops"]:
         out["gemm_frac"] = round(out["gemm_tflops"] / F32_MFMA_PEAK_TFLOPS, 3)
