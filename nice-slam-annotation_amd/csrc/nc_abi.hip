@@ -1789,7 +1789,8 @@ Operand operand_a(int dtype, const void* p, int64_t rows, int64_t cols, int64_t 
 
 struct LayerWs {
   Operand a, b;            // the forward's x and W, the backward's dY and W^T
-  size_t gemm_part = 0, part = 0, sums = 0, total = 0;
+  size_t gemm_part = 0, part = 0, sums = 0, values = 0, total = 0;
+  bool decodes = false;    // dW: the codes' values are written out first
   int32_t gemm_splits = 1, splits = 0, pieces = 0;
   int64_t rows_per = 0;
 };
@@ -1810,6 +1811,9 @@ void layer_layout(const nc_layer_args* a, bool backward, LayerWs& w) {
     o = align256(o + (size_t)w.splits * (size_t)a->outputs * (size_t)a->inputs * 4);
     w.sums = o;
     o = align256(o + (size_t)w.splits * (size_t)w.pieces * (size_t)a->outputs * 4);
+    w.decodes = low_wgrad_decodes(a->dtype, a->rows, a->outputs, a->inputs);
+    w.values = o;
+    if (w.decodes) o = align256(o + (size_t)round_up(a->rows, 64) * (size_t)round_up(a->inputs, CODE_ALIGN) * 2);
   }
   w.gemm_splits = low_gemm_splits(layer_mode(a->dtype), a->rows, n, k);
   w.gemm_part = o;
@@ -2086,6 +2090,21 @@ int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* s
     g.want_db = a->db != nullptr;
     g.pieces = a->dtype == NC_F32 && a->dw ? 1 : w.pieces;
     const int32_t db_parts = w.splits * g.pieces;
+    if (w.decodes && a->dw) {
+      CodeCtx c;
+      std::memset(&c, 0, sizeof(c));
+      c.dtype = a->dtype;
+      c.format = a->relu ? NC_CODES_RELU : NC_CODES_GROUP;
+      c.rows = a->rows;
+      c.zero_rows = round_up(a->rows, 64) - a->rows;
+      c.cols = c.x_stride = a->code_stride;
+      c.codes = a->codes;
+      c.code_stride = a->code_stride;
+      c.scales = a->steps;
+      c.values = at<uint16_t>(ws, w.values);
+      if (int e = check_hip(timed(KID_CODES, s, [&] { return launch_decode(c, s); }), "decode")) return e;
+      g.x = at<uint16_t>(ws, w.values);
+    }
     if (w.splits == 1) g.dw = a->dw;
     if (db_parts == 1) g.db = a->db;
     g.splits = w.splits;

@@ -43,6 +43,7 @@ struct CodeCtx {
   int64_t code_stride;
   void* scales;            // ROW: float [rows]; else uint8 [rows][code_stride / 32]
   void* values;            // decode: [rows][x_stride]
+  int64_t zero_rows;       // decode: rows of zeros behind them
   // encode of the layer's input: what the matrix kernel reads besides
   int32_t relu;            // max(x, 0) in the 16-bit copy / planes
   uint16_t* copy;          // 16-bit x: [rows][copy_stride]; float x: three bfloat16 planes of that
@@ -112,6 +113,7 @@ struct LowWgrad {
   const uint8_t* codes;
   const uint8_t* steps;
   int64_t code_stride;
+  const uint16_t* x;       // the codes' values, [round_up(M, 64)][code_stride], zeros behind row M; or NULL
   int64_t M, N, K;
   float* part;             // [splits][N][K]
   float* sums;             // [splits][pieces][N]: the columns' sums of dY (float with want_dw: pieces = 1)
@@ -123,6 +125,7 @@ struct LowWgrad {
   int64_t rows_per;        // rows of a split, a multiple of 64
 };
 int launch_low_wgrad(const LowWgrad& g, hipStream_t s);
+bool low_wgrad_decodes(int dtype, int64_t M, int64_t N, int64_t K);  // whether it takes x
 void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, int32_t& splits, int32_t& pieces, int64_t& rows_per);
 
 // out[e] = sum_s part[s][e], in order, as dtype, for two matrices in one launch; out = NULL: none
@@ -147,7 +150,7 @@ __device__ __forceinline__ uint16_t f32_elem(float x) {  // round to nearest eve
   return DT == NC_BF16 ? f32_bf16(x) : __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-__device__ __forceinline__ float relu_keep_nan(float x) { return x < 0.f ? 0.f : x; }
+__device__ __forceinline__ float relu_keep_nan(float x) { return x <= 0.f ? 0.f : x; }  // (of -0: +0)
 
 // x = x0 + x1 + x2, exactly, in bfloat16: each plane is what is left cut to its upper half (8 significant
 // bits, 24 in all; the third is whole by then).  Of 8 values: a plane is 4 words.  An infinity or NaN
@@ -215,10 +218,11 @@ inline bool load8_vec(const void* p, int64_t stride, int64_t cols, int dtype) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * (dtype == NC_F32 ? 4 : 2)) % 16 == 0 && cols % 8 == 0;
 }
 
-__device__ __forceinline__ uint2 pack8(const int (&q)[8]) {
+// the low bytes of 8 words
+__device__ __forceinline__ uint2 pack8(const uint32_t (&q)[8]) {
   uint2 r;
-  r.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | (uint32_t)(q[3] & 255) << 24;
-  r.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | (uint32_t)(q[7] & 255) << 24;
+  r.x = __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400u) | __builtin_amdgcn_perm(q[3], q[2], 0x04000c0cu);
+  r.y = __builtin_amdgcn_perm(q[5], q[4], 0x0c0c0400u) | __builtin_amdgcn_perm(q[7], q[6], 0x04000c0cu);
   return r;
 }
 
@@ -241,35 +245,36 @@ __device__ __forceinline__ float row_scale(uint32_t top) {
   return __builtin_fmaxf(__builtin_bit_cast(float, top) * (1.f / 127.f), 0x1p-126f);
 }
 __device__ __forceinline__ uint2 row_codes(const float (&v)[8], bool bad, float s, float rcp) {
-  int q[8];
+  uint32_t q[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) q[e] = bad ? 0 : row_code(v[e], s, rcp);
+  for (int e = 0; e < 8; ++e) q[e] = bad ? 0u : (uint32_t)row_code(v[e], s, rcp);
   return pack8(q);
 }
 
 // the codes of 8 columns and the step byte of their group, whose other columns the three lanes beside
-// (lane ^ 1, 2, 3) hold
+// (lane ^ 1, 2, 3) hold; RELU: the columns are max(x, 0) already.
+// v inv + 1.5 2^23 rounds v / step to an integer, ties to even, in the float's low bits.  The bounds are for
+// an amax near the largest float, which no step reaches, and for NaN, of which the median takes the lower.
 template <bool RELU>
 __device__ __forceinline__ uint2 group_codes(const float (&v)[8], int& sb) {
   uint32_t top = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {  // RELU: x <= 0 counts as 0 (a NaN does not)
-    const uint32_t m = mag_bits(v[e]);
-    top = max(top, RELU && v[e] <= 0.f ? 0u : m);
-  }
+  for (int e = 0; e < 8; ++e) top = max(top, RELU ? __builtin_bit_cast(uint32_t, v[e]) : mag_bits(v[e]));
   top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true));  // lane ^ 1
   top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4e, 0xf, 0xf, true));  // lane ^ 2
   sb = step_byte(top, RELU);
-  const float inv = __builtin_bit_cast(float, (uint32_t)(254 - min(sb, 253)) << 23);
-  int q[8];
+  const float inv = sb == 255 ? 0.f : __builtin_bit_cast(float, (uint32_t)(254 - sb) << 23);
+  constexpr float ONE = 12582912.f;
+  uint32_t q[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float t = __builtin_rintf(v[e] * inv);
-    const float c = __builtin_fminf(__builtin_fmaxf(t, RELU ? 0.f : -127.f), RELU ? 254.f : 127.f);
-    const int k = sb == 255 ? 0 : (int)c;
-    q[e] = RELU ? (v[e] <= 0.f ? 0 : 1 + k) : k;
+    const float t = __builtin_amdgcn_fmed3f(__builtin_fmaf(v[e], inv, ONE), RELU ? ONE : ONE - 127.f, ONE + (RELU ? 254.f : 127.f));
+    const uint32_t k = __builtin_bit_cast(uint32_t, t);
+    q[e] = RELU ? (v[e] <= 0.f ? 0u : k + 1u) : k;
   }
-  return pack8(q);
+  uint2 w = pack8(q);
+  if (!RELU && sb == 255) w = uint2{0u, 0u};
+  return w;
 }
 
 }  // namespace nc

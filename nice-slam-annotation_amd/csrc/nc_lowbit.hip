@@ -4,6 +4,8 @@
 // columns (16 or 32 bytes in, 8 bytes of codes out).
 #include "nc_lowbit.h"
 
+#include <type_traits>
+
 namespace nc {
 
 static inline unsigned blocks_of(int64_t n, int b) { return (unsigned)((n + b - 1) / b); }
@@ -144,6 +146,10 @@ __global__ void __launch_bounds__(256) k_encode_groups(const CodeCtx a, int64_t 
   load8<DT, VEC>(a.x, r * a.x_stride, c, a.cols, v);
   clear8<VEC>(c, a.cols, v);
   constexpr bool RELU = FMT == NC_CODES_RELU;
+  if (RELU || a.relu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = relu_keep_nan(v[e]);
+  }
   if (FMT >= 0) {
     int sb;
     const uint2 w = group_codes<RELU>(v, sb);
@@ -153,10 +159,6 @@ __global__ void __launch_bounds__(256) k_encode_groups(const CodeCtx a, int64_t 
     }
   }
   if (OUT > 0 && 8 * c < a.copy_stride) {
-    if (a.relu) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = relu_keep_nan(v[e]);
-    }
     if (OUT == 1) {
       store8<DT == NC_F32 ? NC_BF16 : DT, true>(a.copy, r * a.copy_stride, c, a.copy_stride, v);  // exact: v is of that type
     } else {
@@ -173,6 +175,11 @@ __global__ void __launch_bounds__(256) k_decode(const CodeCtx a, int64_t row_chu
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= total) return;
   const int64_t r = id / row_chunks, c = id - r * row_chunks;
+  if (r >= a.rows) {
+    const float zero[8] = {};
+    store8<DT, VEC>(a.values, r * a.x_stride, c, a.cols, zero);
+    return;
+  }
   const uint2 w = *reinterpret_cast<const uint2*>(a.codes + r * a.code_stride + 8 * c);
   float s;
   if (a.format == NC_CODES_ROW) {
@@ -192,34 +199,49 @@ __global__ void __launch_bounds__(256) k_decode(const CodeCtx a, int64_t row_chu
 }
 
 // ---- transpose into padded 16-bit rows: 64 x 64 tiles through LDS -------------------------------------
-template <int DT>
+// A lane loads 16 bytes of its row (VEC; else element by element) and writes them down a column of the tile:
+// a wave's 64 lanes are a column's 64 elements, side by side in LDS.  Then 8 lanes write a row of the
+// result, 16 bytes each (float: to each plane).
+template <int DT, bool VEC>
 __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
-  __shared__ float tile[64][65];
+  using E = typename std::conditional<DT == NC_F32, float, uint16_t>::type;
+  constexpr int EC = 16 / sizeof(E), CH = 64 / EC / 4;  // elements a chunk, chunks a thread
+  __shared__ __attribute__((aligned(16))) E tile[64][64 + EC];
   const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int rr = e >> 6, cc = e & 63;
-    const int64_t r = r0 + rr, c = c0 + cc;
-    float v = 0.f;
-    if (r < a.rows && c < a.cols)
-      v = DT == NC_F32 ? reinterpret_cast<const float*>(a.src)[r * a.src_stride + c]
-                       : elem_f32<DT>(reinterpret_cast<const uint16_t*>(a.src)[r * a.src_stride + c]);
-    tile[rr][cc] = v;
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int cc = e >> 6, rr = e & 63;
-    const int64_t r = r0 + rr, c = c0 + cc;
-    if (c >= a.cols) continue;  // r < dst_stride: whole tiles of 64
-    uint16_t* d = a.dst + c * a.dst_stride + r;
-    float x = tile[rr][cc];
-    if (DT == NC_F32) {  // split3, one value
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool in = r0 + lane < a.rows;
+  const E* src = reinterpret_cast<const E*>(a.src) + (in ? r0 + lane : a.rows - 1) * a.src_stride;
+  E v[CH][EC];
 #pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        d[k * a.plane] = (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16);
-        x = x - cut_bf16(x);
-      }
+  for (int j = 0; j < CH; ++j) {
+    const int64_t c = c0 + EC * (wave + 4 * j);
+    if (VEC) {  // columns behind the last: others, not stored
+      *reinterpret_cast<uint4*>(v[j]) = *reinterpret_cast<const uint4*>(src + (c < a.cols ? c : a.cols - EC));
     } else {
-      d[0] = f32_elem<DT>(x);
+#pragma unroll
+      for (int e = 0; e < EC; ++e) v[j][e] = src[c + e < a.cols ? c + e : a.cols - 1];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < CH; ++j)
+#pragma unroll
+    for (int e = 0; e < EC; ++e) tile[EC * (wave + 4 * j) + e][lane] = in ? v[j][e] : E(0);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int at = j * 256 + threadIdx.x, cc = at >> 3, r8 = 8 * (at & 7);
+    if (c0 + cc >= a.cols) continue;  // r0 + r8 < dst_stride: whole tiles of 64
+    uint16_t* d = a.dst + (c0 + cc) * a.dst_stride + r0 + r8;
+    if constexpr (DT == NC_F32) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = tile[cc][r8 + e];
+      uint4 p[3];
+      split3(x, p);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(d + k * a.plane) = p[k];
+    } else {
+      *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(&tile[cc][r8]);
     }
   }
 }
@@ -283,7 +305,7 @@ template <int DT, bool VEC, int FMT>
 static int encode_groups(const CodeCtx& c, hipStream_t s) {
   int64_t width = FMT >= 0 ? c.code_stride : 0;
   if (c.copy && c.copy_stride > width) width = c.copy_stride;
-  const int64_t rc = width / 8, total = rc * c.rows;
+  const int64_t rc = width / 8, total = rc * (c.rows + c.zero_rows);
   const dim3 g(blocks_of(total, 256));
   if (!c.copy) {
     if (FMT >= 0) hipLaunchKernelGGL((k_encode_groups<DT, VEC, FMT, 0>), g, dim3(256), 0, s, c, rc, total);
@@ -317,7 +339,7 @@ int launch_encode(const CodeCtx& c, hipStream_t s) {
 int launch_decode(const CodeCtx& c, hipStream_t s) {
   if (c.rows <= 0) return 0;
   const bool v = vec_rows(c.values, c.x_stride, c.dtype);
-  const int64_t rc = (c.cols + 7) / 8, total = rc * c.rows;
+  const int64_t rc = (c.cols + 7) / 8, total = rc * (c.rows + c.zero_rows);
   const dim3 g(blocks_of(total, 256)), b(256);
   switch (c.dtype) {
     case NC_F32:
@@ -337,16 +359,22 @@ int launch_decode(const CodeCtx& c, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
+template <int DT>
+static int transpose(const TransposeCtx& c, hipStream_t s) {
+  const dim3 g(blocks_of(c.dst_stride, 64), blocks_of(c.cols, 64));
+  if (load8_vec(c.src, c.src_stride, c.cols, c.dtype)) hipLaunchKernelGGL((k_transpose<DT, true>), g, dim3(256), 0, s, c);
+  else hipLaunchKernelGGL((k_transpose<DT, false>), g, dim3(256), 0, s, c);
+  return (int)hipGetLastError();
+}
+
 int launch_transpose(const TransposeCtx& c, hipStream_t s) {
   if (c.rows <= 0 || c.cols <= 0) return 0;
-  const dim3 g(blocks_of(c.dst_stride, 64), blocks_of(c.cols, 64));
   switch (c.dtype) {
-    case NC_F32: hipLaunchKernelGGL((k_transpose<NC_F32>), g, dim3(256), 0, s, c); break;
-    case NC_F16: hipLaunchKernelGGL((k_transpose<NC_F16>), g, dim3(256), 0, s, c); break;
-    case NC_BF16: hipLaunchKernelGGL((k_transpose<NC_BF16>), g, dim3(256), 0, s, c); break;
-    default: return (int)hipErrorInvalidValue;
+    case NC_F32: return transpose<NC_F32>(c, s);
+    case NC_F16: return transpose<NC_F16>(c, s);
+    case NC_BF16: return transpose<NC_BF16>(c, s);
   }
-  return (int)hipGetLastError();
+  return (int)hipErrorInvalidValue;
 }
 
 template <int DT>

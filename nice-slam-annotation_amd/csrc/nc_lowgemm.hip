@@ -476,6 +476,9 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
         for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const float*>(raw + l * 2048 + e * 256 + 4 * lane);
       }
       clear8<VEC>((int64_t)xt * 4 + c, g.K, x);
+      if (RELU)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = relu_keep_nan(x[e]);
       if (xcode) {
         int sb;
         const uint2 w = group_codes<RELU>(x, sb);
@@ -485,9 +488,6 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
           if (c == 0) (g.steps + xm0 * sr)[(uint32_t)(r * sr + xt)] = (uint8_t)sb;
         }
       }
-      if (RELU)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = relu_keep_nan(x[e]);
       uint4 p[3];
       split3(x, p);
 #pragma unroll
@@ -1037,7 +1037,9 @@ __device__ __forceinline__ void col_sums(const LowWgrad& g, int64_t n0, int64_t 
 // last phase but one.
 // NP = 3: dY is float, split into its planes on the way like A in k_low_gemm_f.  Workgroups with
 // blockIdx.y behind the last column tile add up their rows of dY instead (the bias gradient).
-template <int NP, int DT, bool RELU, int BN, int BK, int MS, int WN, int WK, bool VEC>
+// CODED = false: the codes' values lie in memory already, with zeros behind the last row, and go into LDS by
+// themselves too.
+template <int NP, int DT, bool RELU, bool CODED, int BN, int BK, int MS, int WN, int WK, bool VEC>
 __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
   constexpr int W = WN * WK, T = 64 * W;
   constexpr int FN = BN / WN / 16, FK = BK / WK / 16;
@@ -1046,9 +1048,10 @@ __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
   constexpr bool F16 = DT == NC_F16;
   constexpr int YL = NP == 3 ? 0 : YSTAGE / 1024 / W;       // 1-KB loads a wave
   constexpr int YF = NP == 3 ? MS * BN / 8 / T : 0;         // 8-column chunks a thread
-  constexpr int XL = MS * BK / 16 / T;                      // 16-code loads a thread
+  constexpr int XL = CODED ? MS * BK / 16 / T : 0;          // 16-code loads a thread
+  constexpr int XD = CODED ? 0 : XSTAGE / 1024 / W;         // 1-KB loads of values a wave
   constexpr int NG = FN / 4, NH = MS / 32, PH = NH * NP * NG;
-  static_assert(YSTAGE % (1024 * W) == 0 && MS * BK % (16 * T) == 0 && YL + YF > 0 && XL > 0, "whole loads");
+  static_assert(YSTAGE % (1024 * W) == 0 && MS * BK % (16 * T) == 0 && XSTAGE % (1024 * W) == 0 && YL + YF > 0, "whole loads");
   static_assert(NP == 1 || MS * BN % (8 * T) == 0, "whole chunks");
   static_assert(BN >= 128 && BK >= 128, "rows of at least 8 units of 32 bytes");
   static_assert((NG == 1 || (NG == 2 && FN == 8)) && YROW % 256 == 0 && XROW % 256 == 0, "the second group is 128 bytes away");
@@ -1083,7 +1086,15 @@ __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
     c = c < ychunks ? c : ychunks - 1;  // columns behind the last: not stored
     yo[l] = (uint32_t)(yrow[l] * 2 * g.ldy + 16 * c);
   }
-  uint32_t xo[XL], so[XL];  // codes and steps
+  uint32_t xd[XD > 0 ? XD : 1];
+#pragma unroll
+  for (int l = 0; l < XD; ++l) {
+    const int at = (wave * XD + l) * 64 + lane, row = at / (XROW / 16);
+    int64_t c = k0 / 8 + ((at % (XROW / 16)) ^ ((row & 7) << 1));
+    c = c < 2 * xchunks ? c : 2 * xchunks - 1;  // columns behind the last: not stored
+    xd[l] = (uint32_t)(row * 2 * g.code_stride + 16 * c);
+  }
+  uint32_t xo[XL > 0 ? XL : 1], so[XL > 0 ? XL : 1];  // codes and steps
 #pragma unroll
   for (int l = 0; l < XL; ++l) {
     const int at = l * T + threadIdx.x, row = at / (BK / 16);
@@ -1108,9 +1119,14 @@ __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
         load_lds16(base, o, lds0 + (t & 1) * STAGE + (wave * YL + l) * 1024);
       }
     }
+    if (XD > 0) {
+      const uint8_t* base = reinterpret_cast<const uint8_t*>(g.x) + 2 * (rb + (int64_t)t * MS) * g.code_stride;
+#pragma unroll
+      for (int l = 0; l < XD; ++l) load_lds16(base, xd[l], lds0 + (t & 1) * STAGE + NP * YSTAGE + (wave * XD + l) * 1024);
+    }
   };
-  uint4 xc[XL];
-  uint32_t xs[XL];
+  uint4 xc[XL > 0 ? XL : 1];
+  uint32_t xs[XL > 0 ? XL : 1];
   auto load_x = [&](int t) {
     const uint8_t* codes = g.codes + (rb + (int64_t)t * MS) * g.code_stride;
     const uint8_t* steps = g.steps + (rb + (int64_t)t * MS) * steps_row;
@@ -1283,6 +1299,14 @@ static bool wgrad_wide(int dtype, int64_t N, int64_t K) {
   return (N > 128 || dtype == NC_F32) && K > 128;
 }
 
+// Every tile column of dY decodes the codes anew.  Written out once (4 bytes moved for each) they cost
+// 0.6-1 ps each, and save 0.3-0.4 ps for each tile column: M x K x N 8192 x 4096 x 4096, whole step, 820 us
+// without, 766 with; 8192 x 2048 x 2048 247, 241; 65536 x 1024 x 1024 771, 694; 8192 x 4096 x 1024 293, 297;
+// 4096 x 1024 x 1024 135, 145.
+bool low_wgrad_decodes(int dtype, int64_t M, int64_t N, int64_t K) {
+  return dtype != NC_F32 && wgrad_wide(dtype, N, K) && (N >= 2048 || (N >= 1024 && M >= 65536));
+}
+
 void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, int32_t& splits, int32_t& pieces, int64_t& rows_per) {
   const bool wide = wgrad_wide(dtype, N, K);
   const int64_t tn = wide && dtype != NC_F32 ? 256 : 128, tk = wide ? 256 : 128;
@@ -1297,10 +1321,10 @@ void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, int32_t& split
   pieces = (int32_t)((rows_per + SUM_ROWS - 1) / SUM_ROWS);
 }
 
-template <int NP, int DT, bool RELU, int TN, int TK, int MS, int WN, int WK, bool VEC>
+template <int NP, int DT, bool RELU, bool CODED, int TN, int TK, int MS, int WN, int WK, bool VEC>
 static int run_low_wgrad(const LowWgrad& g, hipStream_t s) {
   constexpr int lds = 2 * (NP * MS * 2 * TN + MS * 2 * TK);
-  auto kernel = k_low_wgrad<NP, DT, RELU, TN, TK, MS, WN, WK, VEC>;
+  auto kernel = k_low_wgrad<NP, DT, RELU, CODED, TN, TK, MS, WN, WK, VEC>;
   static std::atomic<uint64_t> done{0};
   if (const int e = allow_lds(kernel, lds, done)) return e;
   const unsigned kt = g.want_dw ? (unsigned)((g.K + TK - 1) / TK) : 0u;
@@ -1312,21 +1336,25 @@ static int run_low_wgrad(const LowWgrad& g, hipStream_t s) {
 
 template <int DT, bool RELU>
 static int pick_low_wgrad(const LowWgrad& g, hipStream_t s) {
-  if (wgrad_wide(DT, g.N, g.K)) return run_low_wgrad<1, DT, RELU, 256, 256, 64, 2, 4, true>(g, s);
-  return run_low_wgrad<1, DT, RELU, 128, 128, 64, 2, 2, true>(g, s);
+  if (wgrad_wide(DT, g.N, g.K)) return run_low_wgrad<1, DT, RELU, true, 256, 256, 64, 2, 4, true>(g, s);
+  return run_low_wgrad<1, DT, RELU, true, 128, 128, 64, 2, 2, true>(g, s);
 }
 
 template <bool RELU, bool VEC>
 static int pick_low_wgrad_f(const LowWgrad& g, hipStream_t s) {
-  if (wgrad_wide(NC_F32, g.N, g.K)) return run_low_wgrad<3, NC_F32, RELU, 128, 256, 64, 2, 4, VEC>(g, s);
-  return run_low_wgrad<3, NC_F32, RELU, 128, 128, 32, 2, 2, VEC>(g, s);
+  if (wgrad_wide(NC_F32, g.N, g.K)) return run_low_wgrad<3, NC_F32, RELU, true, 128, 256, 64, 2, 4, VEC>(g, s);
+  return run_low_wgrad<3, NC_F32, RELU, true, 128, 128, 32, 2, 2, VEC>(g, s);
 }
 
 int launch_low_wgrad(const LowWgrad& g, hipStream_t s) {
   if (g.N <= 0 || g.K <= 0 || (!g.want_dw && !g.want_db)) return 0;
   switch (g.dtype) {
-    case NC_F16: return g.relu ? pick_low_wgrad<NC_F16, true>(g, s) : pick_low_wgrad<NC_F16, false>(g, s);
-    case NC_BF16: return g.relu ? pick_low_wgrad<NC_BF16, true>(g, s) : pick_low_wgrad<NC_BF16, false>(g, s);
+    case NC_F16:
+      if (g.x) return run_low_wgrad<1, NC_F16, false, false, 256, 256, 64, 2, 4, true>(g, s);
+      return g.relu ? pick_low_wgrad<NC_F16, true>(g, s) : pick_low_wgrad<NC_F16, false>(g, s);
+    case NC_BF16:
+      if (g.x) return run_low_wgrad<1, NC_BF16, false, false, 256, 256, 64, 2, 4, true>(g, s);
+      return g.relu ? pick_low_wgrad<NC_BF16, true>(g, s) : pick_low_wgrad<NC_BF16, false>(g, s);
     case NC_F32: {
       const bool vec = load8_vec(g.dy, g.ldy, g.N, NC_F32);
       if (vec) return g.relu ? pick_low_wgrad_f<true, true>(g, s) : pick_low_wgrad_f<false, true>(g, s);
