@@ -1806,11 +1806,12 @@ void layer_layout(const nc_layer_args* a, bool backward, LayerWs& w) {
   } else {
     w.a = operand_a(a->dtype, a->dy, a->rows, k, a->dy_stride, false, o);
     w.b = operand(a->dtype, nullptr, n, k, 0, true, o);
-    low_wgrad_splits(a->dtype, a->rows, a->outputs, a->inputs, w.splits, w.pieces, w.rows_per);
+    low_wgrad_splits(a->dtype, a->rows, a->outputs, a->inputs, a->dw != nullptr, w.splits, w.pieces, w.rows_per);
     w.part = o;
     o = align256(o + (size_t)w.splits * (size_t)a->outputs * (size_t)a->inputs * 4);
     w.sums = o;
-    o = align256(o + (size_t)w.splits * (size_t)w.pieces * (size_t)a->outputs * 4);
+    const int64_t pieces = std::max((w.rows_per + 511) / 512, (a->inputs + 127) / 128);  // with dW or without
+    o = align256(o + (size_t)w.splits * (size_t)pieces * (size_t)a->outputs * 4);
     w.decodes = low_wgrad_decodes(a->dtype, a->rows, a->outputs, a->inputs);
     w.values = o;
     if (w.decodes) o = align256(o + (size_t)round_up(a->rows, 64) * (size_t)round_up(a->inputs, CODE_ALIGN) * 2);
@@ -2088,7 +2089,7 @@ int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* s
     g.sums = at<float>(ws, w.sums);
     g.want_dw = a->dw != nullptr;
     g.want_db = a->db != nullptr;
-    g.pieces = a->dtype == NC_F32 && a->dw ? 1 : w.pieces;
+    g.pieces = w.pieces;
     const int32_t db_parts = w.splits * g.pieces;
     if (w.decodes && a->dw) {
       CodeCtx c;

@@ -116,7 +116,7 @@ struct LowWgrad {
   const uint16_t* x;       // the codes' values, [round_up(M, 64)][code_stride], zeros behind row M; or NULL
   int64_t M, N, K;
   float* part;             // [splits][N][K]
-  float* sums;             // [splits][pieces][N]: the columns' sums of dY (float with want_dw: pieces = 1)
+  float* sums;             // [splits][pieces][N]: the columns' sums of dY
   int32_t pieces;
   void* dw;                // splits = 1: dW itself, of dtype; else NULL
   void* db;                // one part: the sums themselves; else NULL
@@ -126,7 +126,8 @@ struct LowWgrad {
 };
 int launch_low_wgrad(const LowWgrad& g, hipStream_t s);
 bool low_wgrad_decodes(int dtype, int64_t M, int64_t N, int64_t K);  // whether it takes x
-void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, int32_t& splits, int32_t& pieces, int64_t& rows_per);
+void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, bool want_dw, int32_t& splits, int32_t& pieces,
+                      int64_t& rows_per);
 
 // out[e] = sum_s part[s][e], in order, as dtype, for two matrices in one launch; out = NULL: none
 struct SumParts {

@@ -256,7 +256,15 @@ __global__ void __launch_bounds__(256) k_sum_parts(const SumParts a, unsigned fi
   typedef float floatv __attribute__((ext_vector_type(V)));
   floatv t = 0.f;
   const float* p = a.part[w] + e;
-  for (int k = 0; k < a.parts[w]; ++k, p += n) t += *reinterpret_cast<const floatv*>(p);
+  int k = a.parts[w];
+  for (; k >= 8; k -= 8, p += 8 * n) {  // 8 loads in flight, added in order
+    floatv v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const floatv*>(p + j * n);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t += v[j];
+  }
+  for (; k > 0; --k, p += n) t += *reinterpret_cast<const floatv*>(p);
   if (DT == NC_F32) {
     *reinterpret_cast<floatv*>(reinterpret_cast<float*>(a.out[w]) + e) = t;
   } else {

@@ -9,6 +9,8 @@
 // k_low_wgrad   dW[n][k] = sum_m dY[m][n] V[m][k], V the values of an 8-bit checkpoint, decoded while a
 //               tile is staged (a code times a power of two is exact in 16 bits), both operands
 //               read transposed from LDS (ds_read_b64_tr_b16).
+#include <cmath>
+
 #include <atomic>
 
 #include "nc_lowbit.h"
@@ -1035,12 +1037,12 @@ __device__ __forceinline__ void col_sums(const LowWgrad& g, int64_t n0, int64_t 
 // one multiplies; before a stage's last phase the barrier that frees its half.  dY goes into LDS by itself,
 // codes through registers: loaded with dY a stage ahead, decoded and written before the stage's
 // last phase but one.
-// NP = 3: dY is float, split into its planes on the way like A in k_low_gemm_f.  Workgroups with
-// blockIdx.y behind the last column tile add up their rows of dY instead (the bias gradient).
+// NP = 3: dY is float, split into its planes on the way like A in k_low_gemm_f, and its columns are added up
+// in passing (the bias gradient).  Where dW is not asked for, the workgroups add up the columns alone.
 // CODED = false: the codes' values lie in memory already, with zeros behind the last row, and go into LDS by
 // themselves too.
 template <int NP, int DT, bool RELU, bool CODED, int BN, int BK, int MS, int WN, int WK, bool VEC>
-__global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
+__global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_eu(2))) k_low_wgrad(const LowWgrad g) {
   constexpr int W = WN * WK, T = 64 * W;
   constexpr int FN = BN / WN / 16, FK = BK / WK / 16;
   constexpr int YROW = 2 * BN, XROW = 2 * BK;               // bytes of a staged row
@@ -1065,9 +1067,9 @@ __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
   const int64_t ychunks = (g.N + 7) / 8, xchunks = g.code_stride / 16, steps_row = g.code_stride / CODE_GROUP;
   const int total = (int)((re - rb + MS - 1) / MS);
   const uint32_t lds0 = lds_address(lds);
-  const int kt = g.want_dw ? (int)((g.K + BK - 1) / BK) : 0;
-  if ((int)blockIdx.y >= kt) {  // (the whole workgroup) a piece of the split's rows
-    const int piece = blockIdx.y - kt;
+  const int kt = (int)gridDim.y;
+  if (!g.want_dw) {
+    const int piece = blockIdx.y;
     rb += piece * (int64_t)SUM_ROWS;
     re = rb + SUM_ROWS < re ? rb + SUM_ROWS : re;
     col_sums<DT, BN, T, VEC>(g, n0, rb, re, (int64_t)blockIdx.z * g.pieces + piece, reinterpret_cast<float*>(lds));
@@ -1178,6 +1180,13 @@ __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
 #pragma unroll
     for (int v = 0; v < FK; ++v) acc[u][v] = zero4();
   const int wn = (wave / WK) * (BN / WN), wk = (wave % WK) * (BK / WK);
+  // 16-bit dY: the bias gradient as products with ones, every kt-th stage by each tile column and every
+  // WK-th block of n by each wave
+  constexpr int FB = NP == 1 ? FN / WK : 1;
+  floatx4 bias[FB];
+#pragma unroll
+  for (int u = 0; u < FB; ++u) bias[u] = zero4();
+  int next_bias = NP == 1 && g.want_db ? (int)blockIdx.y : total;
   // a lane's transposed reads: row tr of a step, 8 bytes tc of a 32-byte unit; the addresses are kept for the
   // first group of units and recomputed from them at each read, so that they take few registers
   const int tr = 4 * q + (j16 >> 2), tc = 8 * (j16 & 3);
@@ -1215,6 +1224,27 @@ __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
       }
     __builtin_amdgcn_sched_barrier(0);
   };
+  auto add_bias = [&](int t, int p) {
+    if (NP != 1 || t != next_bias) return;
+    const int in = (int)(re - rb - (int64_t)t * MS) - 32 * (p / NG) - 4 * q;  // rows from this lane's first
+    constexpr uint32_t ONE = F16 ? 0x3c00u : 0x3f80u;
+    const uint4 w = {(in > 0 ? ONE : 0u) | (in > 1 ? ONE << 16 : 0u), (in > 2 ? ONE : 0u) | (in > 3 ? ONE << 16 : 0u),
+                     (in > 16 ? ONE : 0u) | (in > 17 ? ONE << 16 : 0u), (in > 18 ? ONE : 0u) | (in > 19 ? ONE << 16 : 0u)};
+#pragma unroll
+    for (int u0 = 0; u0 < 4; u0 += WK) {  // this wave's block of the WK, selected without a branch
+      uint4 y = a[p & 1][u0];
+#pragma unroll
+      for (int u = 1; u < WK; ++u) {
+        const bool mine = wave % WK == u;
+        const uint4 o = a[p & 1][u0 + u];
+        y = uint4{mine ? o.x : y.x, mine ? o.y : y.y, mine ? o.z : y.z, mine ? o.w : y.w};
+      }
+      constexpr int PER = 4 / WK > 0 ? 4 / WK : 1;  // blocks a group and wave
+      auto& c = bias[((p % NG) * PER + u0 / WK) % FB];
+      c = Mac<F16 ? LOW_F16 : LOW_BF16>::mac(w, y, c);
+    }
+    if (p == PH - 1) next_bias += kt;
+  };
   if (total > 0) {
     stage_y(0);
     load_x(0);
@@ -1240,6 +1270,7 @@ __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
           read(t + 1, 0, PH & 1, NH == 1 ? 1 : 0);
         }
         multiply(p);
+        add_bias(t, p);
       }
       if (PH & 1)
 #pragma unroll
@@ -1253,6 +1284,7 @@ __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
     for (int p = 0; p < PH; ++p) {
       if (p + 1 < PH) read(total - 1, p + 1, (p + 1) & 1, (p + 1) / (NP * NG));
       multiply(p);
+      add_bias(total - 1, p);
     }
   }
   matrix_drain();
@@ -1292,33 +1324,53 @@ __global__ void __launch_bounds__(64 * WN * WK) k_low_wgrad(const LowWgrad g) {
     }
   }
   if (summing) put_col_sums<DT, BN, T>(g, n0, blockIdx.z, ysum, reinterpret_cast<float*>(lds));
+  if (NP == 1 && g.want_db && q == 0) {  // all rows of the product with ones are alike
+#pragma unroll
+    for (int u = 0; u < FN; ++u) {
+      const int64_t n = n0 + wn + 16 * u + i;
+      if (u % WK != wave % WK || n >= g.N) continue;
+      const float sum = bias[u / WK < FB ? u / WK : 0][0];
+      if (!g.db) g.sums[((int64_t)blockIdx.z * kt + blockIdx.y) * g.N + n] = sum;
+      else reinterpret_cast<uint16_t*>(g.db)[n] = f32_elem<DT>(sum);
+    }
+  }
 }
 
-// tiles of 256 columns (float: 128 of dY, whose three planes take the room) where there are more than 128
-static bool wgrad_wide(int dtype, int64_t N, int64_t K) {
-  return (N > 128 || dtype == NC_F32) && K > 128;
+// Tiles: 256 x 256 (float: 128 of dY, whose three planes take the room, x 256) are 4/3 as fast in full, 128 x
+// 128 leave fewer partial sums when an output of few tiles has to be cut along the rows: M x K x N in us,
+// small and large tiles, bfloat16: 1237 x 517 x 1031 26, 41; 4096 x 256 x 256 21, 30; 4096 x 1024 x 1024 36, 38;
+// 4096 x 512 x 4096 52, 49; 8192 x 2048 x 2048 132, 90; 65536 x 1024 x 1024 302, 235.
+// Large tiles of 16-bit elements take the codes' values written out (4 bytes moved for a code, 0.6-1 ps):
+// decoding them in each tile column costs 0.3-0.4 ps a code and column, so small N stays with small tiles.
+// A whole step of 8192 x 4096 x 4096: 820 us decoding in the columns, 766 written out; 8192 x 4096 x 1024 293, 297.
+static bool wgrad_wide(int dtype, int64_t M, int64_t N, int64_t K) {
+  if (dtype == NC_F32) return K > 128;
+  const int64_t tiles = tiles_of(N, K, 256, 256);
+  return N >= 1024 && (tiles >= 32 || (tiles >= 16 && M >= 65536));
 }
+bool low_wgrad_decodes(int dtype, int64_t M, int64_t N, int64_t K) { return dtype != NC_F32 && wgrad_wide(dtype, M, N, K); }
 
-// Every tile column of dY decodes the codes anew.  Written out once (4 bytes moved for each) they cost
-// 0.6-1 ps each, and save 0.3-0.4 ps for each tile column: M x K x N 8192 x 4096 x 4096, whole step, 820 us
-// without, 766 with; 8192 x 2048 x 2048 247, 241; 65536 x 1024 x 1024 771, 694; 8192 x 4096 x 1024 293, 297;
-// 4096 x 1024 x 1024 135, 145.
-bool low_wgrad_decodes(int dtype, int64_t M, int64_t N, int64_t K) {
-  return dtype != NC_F32 && wgrad_wide(dtype, N, K) && (N >= 2048 || (N >= 1024 && M >= 65536));
-}
-
-void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, int32_t& splits, int32_t& pieces, int64_t& rows_per) {
-  const bool wide = wgrad_wide(dtype, N, K);
+// Cuts of the rows.  Large tiles: one workgroup a compute unit.  Small ones: a row costs a workgroup about
+// 20 ns and a cut 4 ps an element of dW to store and add, which sqrt(5000 M / (N K)) cuts balance (within 5 %
+// of the best of 1 to 64 from 200 x 256 x 256 to 65536 x 256 x 256).  Up to 256 rows stay whole, which
+// spares the launch that adds the parts.
+void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, bool want_dw, int32_t& splits, int32_t& pieces,
+                      int64_t& rows_per) {
+  const bool wide = wgrad_wide(dtype, M, N, K);
   const int64_t tn = wide && dtype != NC_F32 ? 256 : 128, tk = wide ? 256 : 128;
   const int64_t tiles = tiles_of(N, K, (int)tn, (int)tk);
-  int64_t want = (wide ? 256 : 512) / tiles, most = (M + 127) / 128;
+  int64_t want = (wide ? 256 : 512) / tiles, most = wide ? (M + 127) / 128 : (M + 63) / 64;
+  if (!wide) {
+    const int64_t balanced = (int64_t)(sqrt(5000. * (double)M / ((double)N * (double)K)) + 0.5);
+    if (want > balanced) want = balanced;
+  }
   if (want > most) want = most;
-  if (want < 1) want = 1;
+  if (want < 1 || M <= 256) want = 1;
   rows_per = round_up((M + want - 1) / want, 64);
   if (rows_per < 64) rows_per = 64;
   splits = (int32_t)((M + rows_per - 1) / rows_per);
   if (splits < 1) splits = 1;
-  pieces = (int32_t)((rows_per + SUM_ROWS - 1) / SUM_ROWS);
+  pieces = (int32_t)(!want_dw ? (rows_per + SUM_ROWS - 1) / SUM_ROWS : dtype == NC_F32 ? 1 : (K + tk - 1) / tk);
 }
 
 template <int NP, int DT, bool RELU, bool CODED, int TN, int TK, int MS, int WN, int WK, bool VEC>
@@ -1327,34 +1379,32 @@ static int run_low_wgrad(const LowWgrad& g, hipStream_t s) {
   auto kernel = k_low_wgrad<NP, DT, RELU, CODED, TN, TK, MS, WN, WK, VEC>;
   static std::atomic<uint64_t> done{0};
   if (const int e = allow_lds(kernel, lds, done)) return e;
-  const unsigned kt = g.want_dw ? (unsigned)((g.K + TK - 1) / TK) : 0u;
-  const dim3 grid((unsigned)((g.N + TN - 1) / TN), kt + (g.want_db && !(NP == 3 && kt) ? (unsigned)g.pieces : 0u),
-                  (unsigned)g.splits);
+  const dim3 grid((unsigned)((g.N + TN - 1) / TN), (unsigned)(g.want_dw ? (g.K + TK - 1) / TK : g.pieces), (unsigned)g.splits);
   hipLaunchKernelGGL(kernel, grid, dim3(64 * WN * WK), lds, s, g);
   return (int)hipGetLastError();
 }
 
-template <int DT, bool RELU>
+template <int DT>
 static int pick_low_wgrad(const LowWgrad& g, hipStream_t s) {
-  if (wgrad_wide(DT, g.N, g.K)) return run_low_wgrad<1, DT, RELU, true, 256, 256, 64, 2, 4, true>(g, s);
-  return run_low_wgrad<1, DT, RELU, true, 128, 128, 64, 2, 2, true>(g, s);
+  if (wgrad_wide(DT, g.M, g.N, g.K)) {
+    if (g.want_dw && !g.x) return (int)hipErrorInvalidValue;
+    return run_low_wgrad<1, DT, false, false, 256, 256, 64, 2, 4, true>(g, s);
+  }
+  if (g.relu) return run_low_wgrad<1, DT, true, true, 128, 128, 64, 2, 2, true>(g, s);
+  return run_low_wgrad<1, DT, false, true, 128, 128, 64, 2, 2, true>(g, s);
 }
 
 template <bool RELU, bool VEC>
 static int pick_low_wgrad_f(const LowWgrad& g, hipStream_t s) {
-  if (wgrad_wide(NC_F32, g.N, g.K)) return run_low_wgrad<3, NC_F32, RELU, true, 128, 256, 64, 2, 4, VEC>(g, s);
+  if (wgrad_wide(NC_F32, g.M, g.N, g.K)) return run_low_wgrad<3, NC_F32, RELU, true, 128, 256, 64, 2, 4, VEC>(g, s);
   return run_low_wgrad<3, NC_F32, RELU, true, 128, 128, 32, 2, 2, VEC>(g, s);
 }
 
 int launch_low_wgrad(const LowWgrad& g, hipStream_t s) {
   if (g.N <= 0 || g.K <= 0 || (!g.want_dw && !g.want_db)) return 0;
   switch (g.dtype) {
-    case NC_F16:
-      if (g.x) return run_low_wgrad<1, NC_F16, false, false, 256, 256, 64, 2, 4, true>(g, s);
-      return g.relu ? pick_low_wgrad<NC_F16, true>(g, s) : pick_low_wgrad<NC_F16, false>(g, s);
-    case NC_BF16:
-      if (g.x) return run_low_wgrad<1, NC_BF16, false, false, 256, 256, 64, 2, 4, true>(g, s);
-      return g.relu ? pick_low_wgrad<NC_BF16, true>(g, s) : pick_low_wgrad<NC_BF16, false>(g, s);
+    case NC_F16: return pick_low_wgrad<NC_F16>(g, s);
+    case NC_BF16: return pick_low_wgrad<NC_BF16>(g, s);
     case NC_F32: {
       const bool vec = load8_vec(g.dy, g.ldy, g.N, NC_F32);
       if (vec) return g.relu ? pick_low_wgrad_f<true, true>(g, s) : pick_low_wgrad_f<false, true>(g, s);
