@@ -9,9 +9,9 @@
 // k_low_wgrad   dW[n][k] = sum_m dY[m][n] V[m][k], V the values of an 8-bit checkpoint, decoded while a
 //               tile is staged (a code times a power of two is exact in 16 bits), both operands
 //               read transposed from LDS (ds_read_b64_tr_b16).
-#include <cmath>
-
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "nc_lowbit.h"
 
@@ -229,15 +229,24 @@ __global__ void __launch_bounds__(256) k_low_finish(const LowGemm g, int64_t qua
   typedef typename M::Acc Acc;
   Acc t = M::zero();
   const float* p = g.part + m * g.N + n;
-  for (int k = 0; k < g.splits; ++k, p += g.M * g.N) {
-    if (g.N % 4 == 0) {
-      t += *reinterpret_cast<const Acc*>(p);
-    } else {
+  const bool whole = g.N % 4 == 0;
+  auto part = [&](int k) {
+    const typename M::Elem* e = reinterpret_cast<const typename M::Elem*>(p + k * (g.M * g.N));
+    if (whole) return *reinterpret_cast<const Acc*>(e);
+    Acc v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < g.N) t[j] += reinterpret_cast<const typename M::Elem*>(p)[j];
-    }
+    for (int j = 0; j < 4; ++j) v[j] = e[n + j < g.N ? j : 0];  // columns behind the last: not stored
+    return v;
+  };
+  int k = 0;
+  for (; k + 4 <= g.splits; k += 4) {  // 4 loads in flight, added in order
+    const Acc a = part(k), b = part(k + 1), c = part(k + 2), d = part(k + 3);
+    t += a;
+    t += b;
+    t += c;
+    t += d;
   }
+  for (; k < g.splits; ++k) t += part(k);
 #pragma unroll
   for (int j = 0; j < 4; ++j) o[j] = finish<MODE>(g, (float)t[j], cs[j], cb[j], (mask >> (8 * j)) & 255u);
   store4<DT>(g, store4_vec<DT>(g), m, n, o);
@@ -668,33 +677,46 @@ static int run_low_gemm_f(const LowGemm& g, hipStream_t s) {
   return finish_parts<LOW_F32, NC_F32>(g, s);
 }
 
-// Tiles and cuts.  256 compute units; a large tile reads less LDS for each product, a small one (or a cut
-// sum) fills the units when the output is small.
+// Tiles and cuts of the sum.  256 compute units; a large tile reads less LDS for each product, a small one (or
+// a cut sum) fills the units when the output is small.  M x K x N in us (S, M, L: tiles; x4: cuts):
+//   float     8192 x 1024 x 1024 S 135, M 100, L 91;  4096 x 1024 x 1024 S 67, M 54, L 103;  2048 x 1024 x 1024 S 37,
+//             M 50;  2048 x 4096 x 1024 S 129, M x2 106, L x4 101;  8192 x 8192 x 256 S 278, L x4 189;  65536 x 1024 x 64
+//             S 85, M 103
+//   bfloat16  8192 x 1024 x 1024 S 32, M 28, L 37;  4096 x 1024 x 1024 S 19, M 22;  1024 x 4096 x 4096 S 61, M 58;
+//             1000 x 1000 x 1000 S 14, S x2 17;  200 x 4096 x 256 S x12 12, x4 13
+//   int8      8192 x 1024 x 1024 S 22, M 20, L 27;  4096 x 1024 x 1024 S 14, M 16;  65536 x 1024 x 64 S 17, M 20, L 27
 enum LowTile { TILE_SMALL, TILE_MIDDLE, TILE_LARGE };
+struct LowCut {
+  LowTile tile;
+  int splits;
+};
 static int64_t tiles_of(int64_t M, int64_t N, int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
 
-static LowTile low_tile(int mode, int64_t M, int64_t N) {
+static LowCut low_cut(int mode, int64_t M, int64_t N, int64_t K) {
+  const int64_t slices = (K * (mode == LOW_I8 ? 1 : mode == LOW_F32 ? 4 : 2) + SLICE - 1) / SLICE;
+  const int64_t middle = N > 64 ? tiles_of(M, N, 128, 128) : 0;
   if (mode == LOW_F32) {
-    if (tiles_of(M, N, 128, 256) >= 192) return N > 128 ? TILE_LARGE : TILE_MIDDLE;
-    return tiles_of(M, N, 128, 128) >= 192 ? TILE_MIDDLE : TILE_SMALL;
+    const int64_t large = N > 128 ? tiles_of(M, N, 128, 256) : 0;
+    if (large >= 192) return {TILE_LARGE, 1};
+    if (middle >= 192) return {TILE_MIDDLE, 1};
+    if (large > 0) {
+      const int64_t cuts = std::min(256 / large, slices / 32);
+      if (large * cuts >= 192) return {TILE_LARGE, (int)cuts};
+    }
+  } else {
+    if (N > 128 && tiles_of(M, N, 256, 256) >= 192) return {TILE_LARGE, 1};
+    if (middle >= (slices >= 32 ? 192 : 320)) return {TILE_MIDDLE, 1};
   }
-  if (tiles_of(M, N, 256, 256) >= 192) return TILE_LARGE;
-  return tiles_of(M, N, 128, 128) >= 192 ? TILE_MIDDLE : TILE_SMALL;
+  if (slices < 32) return {TILE_SMALL, 1};
+  const int64_t cuts = std::min(512 / std::max<int64_t>(tiles_of(M, N, 64, 64), 1), slices / 8);  // 8 slices at least
+  return {TILE_SMALL, (int)std::max<int64_t>(cuts, 1)};
 }
 
-int low_gemm_splits(int mode, int64_t M, int64_t N, int64_t K) {
-  const LowTile t = low_tile(mode, M, N);
-  if (t != TILE_SMALL) return 1;
-  const int64_t slices = (K * (mode == LOW_I8 ? 1 : mode == LOW_F32 ? 4 : 2) + SLICE - 1) / SLICE;
-  const int64_t tiles = tiles_of(M, N, 64, 64);
-  int64_t want = 512 / (tiles > 0 ? tiles : 1);
-  if (want > slices / 8) want = slices / 8;  // parts of 8 slices at least
-  return (int)(want < 1 ? 1 : want);
-}
+int low_gemm_splits(int mode, int64_t M, int64_t N, int64_t K) { return low_cut(mode, M, N, K).splits; }
 
 template <int MODE, int DT>
 static int pick_low_gemm(const LowGemm& g, hipStream_t s) {
-  switch (low_tile(MODE, g.M, g.N)) {
+  switch (low_cut(MODE, g.M, g.N, g.K).tile) {
     case TILE_LARGE: return run_low_gemm<MODE, DT, 256, 256, 2, 4>(g, s);
     case TILE_MIDDLE: return run_low_gemm<MODE, DT, 128, 128, 2, 2>(g, s);
     default: return run_low_gemm<MODE, DT, 64, 64, 1, 4>(g, s);
@@ -703,7 +725,7 @@ static int pick_low_gemm(const LowGemm& g, hipStream_t s) {
 
 template <bool VEC, bool RELU, bool MASK>
 static int pick_low_gemm_f(const LowGemm& g, hipStream_t s) {
-  switch (low_tile(LOW_F32, g.M, g.N)) {
+  switch (low_cut(LOW_F32, g.M, g.N, g.K).tile) {
     case TILE_LARGE: return run_low_gemm_f<128, 256, 2, 4, VEC, RELU, MASK>(g, s);
     case TILE_MIDDLE: return run_low_gemm_f<128, 128, 4, 2, VEC, RELU, MASK>(g, s);
     default: return run_low_gemm_f<64, 64, 2, 2, VEC, RELU, MASK>(g, s);
