@@ -589,8 +589,9 @@ int64_t nc_imap_points_activation_offset(const nc_imap_points_args* args, int la
 int nc_imap_features(const double* pts, int64_t n_points, const float* fourier_B, float* out, void* stream);
 
 /* ---- 8-bit layer operators (ABI v12) ---------------------------------------------
- * Codes are kept in rows of code_stride bytes, a multiple of 128 and at least the number of
- * columns, 16-byte aligned; behind the last column the encoder writes codes of 0. */
+ * Codes are kept in rows of code_stride bytes, the number of columns rounded up to a multiple of 128,
+ * 16-byte aligned; behind the last column the encoder writes codes of 0.  rows < 2^31, rows x
+ * channels <= 2^34; rows of an input may overlap (a stride of 0 repeats one), those of an output not. */
 #define NC_F32 0
 #define NC_F16 1
 #define NC_BF16 2

@@ -11,6 +11,7 @@
 
 #include <cstdio>
 #include <cstdlib>
+#include <algorithm>
 #include <cstring>
 #include <string>
 #include <vector>
@@ -1714,7 +1715,7 @@ int64_t elem_size(int dtype) { return dtype == NC_F32 ? 4 : 2; }
 bool dtype_ok(int dtype) { return dtype == NC_F32 || dtype == NC_F16 || dtype == NC_BF16; }
 
 int check_codes(const void* codes, int64_t stride, int64_t cols) {
-  if (stride < cols || stride % CODE_ALIGN != 0) return fail(-1, "nicecore: code_stride must be a multiple of 128 that holds the columns");
+  if (stride != round_up(cols, CODE_ALIGN)) return fail(-1, "nicecore: code_stride must be the columns rounded up to a multiple of 128");
   if (reinterpret_cast<uintptr_t>(codes) & 15) return fail(-1, "nicecore: codes must be 16-byte aligned");
   return 0;
 }
@@ -1723,6 +1724,13 @@ int check_matrix(int64_t rows, int64_t inputs, int64_t outputs) {
   if (rows < 0 || inputs < 1 || outputs < 1) return fail(-1, "nicecore: need rows >= 0, inputs >= 1, outputs >= 1");
   if (inputs > NC_MAX_INPUTS || outputs > NC_MAX_INPUTS) return fail(-1, "nicecore: inputs and outputs must not exceed 131072");
   if (rows > INT32_MAX) return fail(-1, "nicecore: rows must be below 2^31");
+  // 8 columns a thread, 2^32 threads a launch
+  if (rows * round_up(std::max(inputs, outputs), CODE_ALIGN) > (int64_t(1) << 34)) return fail(-1, "nicecore: rows x channels must not exceed 2^34");
+  return 0;
+}
+// rows that a call writes must not overlap
+int check_written(const void* p, int64_t rows, int64_t cols, int64_t stride) {
+  if (p && rows > 1 && stride < cols) return fail(-1, "nicecore: rows of an output overlap (row stride below the columns)");
   return 0;
 }
 
@@ -1829,6 +1837,8 @@ int layer_check(const nc_layer_args* a) {
   if (int e = check_matrix(a->rows, a->inputs, a->outputs)) return e;
   if (a->x_stride < 0 || a->w_stride < 0 || a->dy_stride < 0 || a->y_stride < 0 || a->dx_stride < 0)
     return fail(-1, "nicecore: negative row stride");
+  if (int e = check_written(a->y, a->rows, a->outputs, a->y_stride)) return e;
+  if (int e = check_written(a->dx, a->rows, a->inputs, a->dx_stride)) return e;
   if (a->x_stride > NC_MAX_STRIDE || a->dy_stride > NC_MAX_STRIDE) return fail(-1, "nicecore: row strides must not exceed 2^22 elements");
   return 0;
 }
@@ -1884,6 +1894,7 @@ int qlinear_check(const nc_qlinear_args* a) {
     return fail(-1, "nicecore: unknown dtype");
   if (int e = check_matrix(a->rows, a->inputs, a->outputs)) return e;
   if (a->x_stride < 0 || a->out_stride < 0) return fail(-1, "nicecore: negative row stride");
+  if (int e = check_written(a->out, a->rows, a->outputs, a->out_stride)) return e;
   if (int e = check_codes(a->w_codes, a->code_stride, a->inputs)) return e;
   if (!a->x)
     if (int e = check_codes(a->x_codes, a->code_stride, a->inputs)) return e;
@@ -1924,6 +1935,7 @@ int nc_encode_rows(const nc_codes_args* a, void* stream) {
 
 int nc_decode_rows(const nc_codes_args* a, void* stream) {
   if (int e = check_codes_args(a)) return e;
+  if (int e = check_written(a->values, a->rows, a->cols, a->stride)) return e;
   if (a->rows == 0) return 0;
   if (!a->values || !a->codes || !a->scales) return fail(-1, "nicecore: NULL values, codes or scales");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);

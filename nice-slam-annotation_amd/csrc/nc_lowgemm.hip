@@ -1136,7 +1136,7 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
     }
     if (YL > 0) {
       const uint8_t* base = reinterpret_cast<const uint8_t*>(g.dy) + 2 * (rb + (int64_t)t * MS) * g.ldy;
-      const int last = (int)(re - rb - (int64_t)t * MS) - 1;  // rows behind the last: its copies, against zeros
+      const int last = (int)(re - rb - (int64_t)t * MS) - 1;  // rows behind the last: its copies, cleared later
 #pragma unroll
       for (int l = 0; l < YL; ++l) {
         const uint32_t o = last >= MS - 1 || yrow[l] <= last ? yo[l] : yo[l] - (uint32_t)(yrow[l] - last) * (uint32_t)(2 * g.ldy);
@@ -1248,10 +1248,8 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
   };
   auto add_bias = [&](int t, int p) {
     if (NP != 1 || t != next_bias) return;
-    const int in = (int)(re - rb - (int64_t)t * MS) - 32 * (p / NG) - 4 * q;  // rows from this lane's first
-    constexpr uint32_t ONE = F16 ? 0x3c00u : 0x3f80u;
-    const uint4 w = {(in > 0 ? ONE : 0u) | (in > 1 ? ONE << 16 : 0u), (in > 2 ? ONE : 0u) | (in > 3 ? ONE << 16 : 0u),
-                     (in > 16 ? ONE : 0u) | (in > 17 ? ONE << 16 : 0u), (in > 18 ? ONE : 0u) | (in > 19 ? ONE << 16 : 0u)};
+    constexpr uint32_t ONES = F16 ? 0x3c003c00u : 0x3f803f80u;
+    const uint4 w = {ONES, ONES, ONES, ONES};
 #pragma unroll
     for (int u0 = 0; u0 < 4; u0 += WK) {  // this wave's block of the WK, selected without a branch
       uint4 y = a[p & 1][u0];
@@ -1267,6 +1265,14 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
     }
     if (p == PH - 1) next_bias += kt;
   };
+  // 16-bit dY: zeros for the copies behind the last row (whose infinities would be products 0 x inf)
+  auto clear_tail = [&](int t) {
+    const int in = (int)(re - rb - (int64_t)t * MS);
+    if (NP != 1 || in >= MS) return;  // (the whole workgroup)
+    for (int e = threadIdx.x; e < (MS - in) * (YROW / 16); e += T)
+      *reinterpret_cast<uint4*>(lds + (t & 1) * STAGE + in * YROW + 16 * e) = uint4{0u, 0u, 0u, 0u};
+    __syncthreads();
+  };
   if (total > 0) {
     stage_y(0);
     load_x(0);
@@ -1276,6 +1282,7 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
       stage_y(1);
     }
     staged_barrier();
+    clear_tail(0);
     read(0, 0, 0, 0);
     for (int t = 0; t + 1 < total; ++t) {
 #pragma unroll
@@ -1285,6 +1292,7 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
           read(t, p + 1, (p + 1) & 1, (p + 1) / (NP * NG));
         } else {
           staged_barrier();
+          clear_tail(t + 1);
           if (t + 2 < total) {
             load_x(t + 2);
             stage_y(t + 2);

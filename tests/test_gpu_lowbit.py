@@ -503,3 +503,59 @@ def test_workspace_sizes_are_enough():
     assert bool((guard[n:] == 255).all())
     with torch.no_grad():
         assert torch.equal(y, lb().checkpointed_linear(x, w))
+
+
+# large outputs (256 x 256 tiles, the codes' values written out), one part and several, both formats; float sums
+# cut over large tiles; many cuts of a long batch
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("m,k,n,dtype", [(777, 2048, 1030, F16), (1000, 1100, 2100, BF16), (64, 4096, 1024, BF16), (300, 2100, 1100, F32),
+                                         (1030, 260, 4100, F32), (40000, 60, 130, BF16), (70001, 20, 30, F32)])
+def test_layer_cuts(m, k, n, dtype, relu):
+    layer_case(m, k, n, dtype, relu, m + n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 40, 50), (70, 40, 50), (1000, 300, 40), (130, 2048, 1100)])
+def test_layer_bias_gradient_alone(m, k, n, dtype):
+    """db without dW, and dW without db, are what both together give."""
+    x, w = acts(m, k, dtype, 1).cuda(), acts(n, k, dtype, 2).cuda()
+    b, dy = acts(1, n, dtype, 3)[0].cuda(), acts(m, n, dtype, 4).cuda()
+    wl, bl = w.clone().requires_grad_(), b.clone().requires_grad_()
+    dw, db = torch.autograd.grad(lb().checkpointed_linear(x, wl, bl), (wl, bl), dy)
+    alone, = torch.autograd.grad(lb().checkpointed_linear(x, w, bl), bl, dy)
+    # (other parts of the sum: its roundings, not its terms)
+    t = 2 * (m / 8 + 300) * U * dy.double().abs().sum(0).cpu()
+    check(alone, db.double().cpu(), t + 2 * out_tol(db.double().cpu().abs() + t, dtype))
+    assert torch.equal(torch.autograd.grad(lb().checkpointed_linear(x, wl, b), wl, dy)[0], dw)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m,k,n", [(1, 40, 50), (70, 256, 50), (193, 300, 300), (130, 2048, 1100)])
+def test_layer_infinite_gradient_in_the_last_row(m, k, n, dtype):
+    """Rows behind the last one take no part: dW and db are infinite or NaN where the formula's are."""
+    x, dy = acts(m, k, dtype, 5), acts(m, n, dtype, 6)
+    x[-1, ::3] = 0.0  # codes of 0: inf x 0 is NaN
+    dy[-1, 7] = float("inf")
+    _, dw, db = layer_run(x, acts(n, k, dtype, 7), torch.zeros(n, dtype=dtype), dy, False)[1:]
+    v = LO.group_codes(x, False)[2]
+    want = torch.where(v[-1] == 0, math.nan, torch.where(v[-1] > 0, math.inf, -math.inf))
+    assert torch.equal(torch.nan_to_num(dw[7].double().cpu(), nan=5.0), torch.nan_to_num(want.double(), nan=5.0))
+    assert db[7].item() == math.inf
+    # the others are infinite only where the formula's value is beyond the type's range (float16: these inputs reach
+    # sums of |dy v| of 10^5, its largest number is 65504)
+    rest = [j for j in range(n) if j != 7]
+    exact = dy[:, rest].double().t() @ v
+    inside = exact.abs() + sum_tol(dy[:, rest].double().abs().t() @ v.abs(), m, 1) < torch.finfo(dtype).max
+    assert inside.double().mean() > 0.9 and torch.isfinite(dw[rest].cpu()[inside]).all() and torch.isfinite(db[rest]).all()
+
+
+@pytest.mark.parametrize("m,k,n", [(2000, 200, 64), (3000, 100, 128), (300, 4096, 1024), (1000, 2100, 1000), (4096, 300, 1500)])
+def test_quantized_linear_tiles(m, k, n):
+    """Few channels, the middle tiles, cut sums."""
+    x, w = acts(m, k, BF16, m).cuda(), acts(n, k, F32, n).cuda()
+    q, w8 = lb().quantize_rows(x), lb().quantize_rows(w)
+    got = lb().quantized_linear(x, w8, out_dtype=F32).double().cpu()
+    acc = q.codes.double().cpu() @ w8.codes.double().cpu().t()
+    want = acc * q.scales.double().cpu()[:, None] * w8.scales.double().cpu()
+    check(got, want, 4 * U * want.abs())
+    assert torch.equal(lb().quantized_linear(q, w8), lb().quantized_linear(x, w8))

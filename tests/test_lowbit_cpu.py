@@ -169,3 +169,26 @@ def test_activation_names_are_checked():
         imap.eval_points(m, torch.zeros(4, 3), activations="fp8")
     with pytest.raises(L.NiceCoreError, match="HIP device"):
         m.quantize()
+
+
+def test_overlaps_and_sizes_are_refused(lib):
+    """Rows of an output that overlap, codes with other strides, more threads than a launch has."""
+    def layer(**kw):
+        a = L.NcLayerArgs(abi_version=L.NC_ABI_VERSION, rows=4, inputs=100, outputs=8, x=16, x_stride=100, w=16, w_stride=100,
+                          y=16, y_stride=8, codes=32, steps=16, code_stride=128, dy=16, dy_stride=8, dx=16, dx_stride=100, dw=16, db=16)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+
+    for kw, msg in ((dict(y_stride=7), b"overlap"), (dict(dx_stride=99), b"overlap"), (dict(rows=1 << 28), b"2^34")):
+        for back, call in ((0, lib.nc_layer_forward), (1, lib.nc_layer_backward)):
+            assert lib.nc_layer_workspace_bytes(ctypes.byref(layer(**kw)), back) == 0 and msg in lib.nc_last_error(), kw
+            assert call(ctypes.byref(layer(**kw)), 256, 1 << 60, None) == -1, kw
+    assert lib.nc_layer_workspace_bytes(ctypes.byref(layer(rows=1, y_stride=0, dx_stride=0)), 1) > 0  # one row overlaps with none
+    for call in (lib.nc_layer_forward, lib.nc_layer_backward):
+        assert call(ctypes.byref(layer(code_stride=256)), 256, 1 << 60, None) == -1 and b"code_stride" in lib.nc_last_error()
+    assert lib.nc_decode_rows(ctypes.byref(codes_args(stride=99)), None) == -1 and b"overlap" in lib.nc_last_error()
+    assert lib.nc_encode_rows(ctypes.byref(codes_args(code_stride=256)), None) == -1
+    a = L.NcQlinearArgs(abi_version=L.NC_ABI_VERSION, rows=4, inputs=100, outputs=8, x=16, x_stride=100, code_stride=128, w_codes=32,
+                        w_scales=16, out=16, out_stride=7)
+    assert lib.nc_quantized_linear_workspace_bytes(ctypes.byref(a)) == 0 and b"overlap" in lib.nc_last_error()
