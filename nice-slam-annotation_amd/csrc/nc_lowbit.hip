@@ -313,7 +313,7 @@ template <int DT, bool VEC, int FMT>
 static int encode_groups(const CodeCtx& c, hipStream_t s) {
   int64_t width = FMT >= 0 ? c.code_stride : 0;
   if (c.copy && c.copy_stride > width) width = c.copy_stride;
-  const int64_t rc = width / 8, total = rc * (c.rows + c.zero_rows);
+  const int64_t rc = width / 8, total = rc * c.rows;
   const dim3 g(blocks_of(total, 256));
   if (!c.copy) {
     if (FMT >= 0) hipLaunchKernelGGL((k_encode_groups<DT, VEC, FMT, 0>), g, dim3(256), 0, s, c, rc, total);
