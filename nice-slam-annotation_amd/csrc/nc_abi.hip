@@ -1909,7 +1909,9 @@ struct QlinearWs {
 void qlinear_layout(const nc_qlinear_args* a, QlinearWs& w) {
   size_t o = 0;
   w.fused = a->x && low_small_encodes(a->rows, a->outputs, a->inputs);
-  w.small = w.fused || a->rows <= 64;
+  // Few rows: every 16 channels read all of x's codes, so up to 2^30 products (us, k_low_small and tiles, coded x:
+  // 32 x 4096 x 4096 10.2, 12.8; 64 x 4096 x 4096 11.7, 12.8; 17 x 8192 x 8192 19.4, 15.6; 64 x 8192 x 8192 39, 18).
+  w.small = w.fused || (a->rows <= 64 && a->rows * a->inputs * a->outputs <= (int64_t(1) << 30));
   if (a->x && !w.fused) {
     w.codes = o;
     o = align256(o + (size_t)a->rows * (size_t)a->code_stride);

@@ -1367,23 +1367,22 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
 }
 
 // Tiles: 256 x 256 (float: 128 of dY, whose three planes take the room, x 256) are 4/3 as fast in full, 128 x
-// 128 leave fewer partial sums when an output of few tiles has to be cut along the rows: M x K x N in us,
-// small and large tiles, bfloat16: 1237 x 517 x 1031 26, 41; 4096 x 256 x 256 21, 30; 4096 x 1024 x 1024 36, 38;
-// 4096 x 512 x 4096 52, 49; 8192 x 2048 x 2048 132, 90; 65536 x 1024 x 1024 302, 235.
-// Large tiles of 16-bit elements take the codes' values written out (4 bytes moved for a code, 0.6-1 ps):
-// decoding them in each tile column costs 0.3-0.4 ps a code and column, so small N stays with small tiles.
-// A whole step of 8192 x 4096 x 4096: 820 us decoding in the columns, 766 written out; 8192 x 4096 x 1024 293, 297.
+// 128 leave fewer partial sums when an output of few tiles has to be cut along the rows.  Large tiles of
+// 16-bit elements take the codes' values written out (4 bytes moved for a code, 0.6-1 ps): decoding them in
+// each tile column costs 0.3-0.4 ps a code and column.  M x K x N, us with the values' decoding, bfloat16, small and
+// large tiles: 1237 x 517 x 1031 53, 72; 4096 x 1024 x 1024 52, 59; 4096 x 512 x 4096 61, 65; 8192 x 2048 x 2048 150, 127;
+// 1000 x 4096 x 4096 93, 77; 65536 x 1024 x 1024 313, 262; float 4096 x 1024 x 1024 48, 43; 220000 x 256 x 256 120, 107.
 static bool wgrad_wide(int dtype, int64_t M, int64_t N, int64_t K) {
   if (dtype == NC_F32) return K > 128;
   const int64_t tiles = tiles_of(N, K, 256, 256);
-  return N >= 1024 && (tiles >= 32 || (tiles >= 16 && M >= 65536));
+  return N >= 1024 && (tiles >= 64 || (tiles >= 16 && M >= 65536));
 }
 bool low_wgrad_decodes(int dtype, int64_t M, int64_t N, int64_t K) { return dtype != NC_F32 && wgrad_wide(dtype, M, N, K); }
 
-// Cuts of the rows.  Large tiles: one workgroup a compute unit.  Small ones: a row costs a workgroup about
-// 20 ns and a cut 4 ps an element of dW to store and add, which sqrt(5000 M / (N K)) cuts balance (within 5 %
-// of the best of 1 to 64 from 200 x 256 x 256 to 65536 x 256 x 256).  Up to 256 rows stay whole, which
-// spares the launch that adds the parts.
+// Cuts of the rows.  Large tiles: one workgroup a compute unit.  Small ones: what a row costs a workgroup and
+// a cut costs for an element of dW is balanced by sqrt(8000 M / (N K)) cuts (of 1 to 192, within 6 % of the best
+// from 500 x 256 x 256 to 220000 x 256 x 256).  Up to 128 rows stay whole: 64 x 256 x 256 takes as long as in two
+// parts, with a launch less.
 void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, bool want_dw, int32_t& splits, int32_t& pieces,
                       int64_t& rows_per) {
   const bool wide = wgrad_wide(dtype, M, N, K);
@@ -1391,11 +1390,11 @@ void low_wgrad_splits(int dtype, int64_t M, int64_t N, int64_t K, bool want_dw, 
   const int64_t tiles = tiles_of(N, K, (int)tn, (int)tk);
   int64_t want = (wide ? 256 : 512) / tiles, most = wide ? (M + 127) / 128 : (M + 63) / 64;
   if (!wide) {
-    const int64_t balanced = (int64_t)(sqrt(5000. * (double)M / ((double)N * (double)K)) + 0.5);
+    const int64_t balanced = (int64_t)(sqrt(8000. * (double)M / ((double)N * (double)K)) + 0.5);
     if (want > balanced) want = balanced;
   }
   if (want > most) want = most;
-  if (want < 1 || M <= 256) want = 1;
+  if (want < 1 || M <= 128) want = 1;
   rows_per = round_up((M + want - 1) / want, 64);
   if (rows_per < 64) rows_per = 64;
   splits = (int32_t)((M + rows_per - 1) / rows_per);
