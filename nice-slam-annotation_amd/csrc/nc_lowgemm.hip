@@ -6,9 +6,10 @@
 //               x0 y0 + x0 y1 + x1 y0 + x0 y2 + x1 y1 + x2 y0; what is left out is below 2^-22 of |x y|,
 //               2^-24.5 on average.
 //               A is split while it is staged, and its 8-bit checkpoint written besides.
+// k_low_small   the int8 product of few rows or short sums, x encoded within it.
 // k_low_wgrad   dW[n][k] = sum_m dY[m][n] V[m][k], V the values of an 8-bit checkpoint, decoded while a
-//               tile is staged (a code times a power of two is exact in 16 bits), both operands
-//               read transposed from LDS (ds_read_b64_tr_b16).
+//               tile is staged or written out before (a code times a power of two is exact in 16 bits), both
+//               operands read transposed from LDS (ds_read_b64_tr_b16); db[n] = sum_m dY[m][n] beside it.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -258,6 +259,10 @@ __global__ void __launch_bounds__(256) k_low_finish(const LowGemm g, int64_t qua
 // A slice is worked off in phases of 4 x FN blocks; while a phase multiplies, the next one's operands
 // are read from LDS.  Before the last phase a barrier says that the slice is read and the next one
 // has arrived; the slice after that goes into the freed half then, a whole slice ahead of its use.
+// Measured, M x K x N: int8 16384 x 4096 x 4096 232 us = 2.37 POP/s (a library's int8 product on this card: 2.47), bfloat16
+// 8192 x 4096 x 4096 205 us = 1.34 PFLOP/s (1.57).  The matrix cores are busy 55 - 62 % of the cycles at the 2.0 - 2.2
+// GHz that their power leaves.  4 waves of 128 x 128 read a third less from LDS, but a wave alone on its SIMD waits
+// for every read: int8 392 us.
 template <int MODE, int DT, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int64_t mt, int64_t nt) {
   constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
@@ -382,6 +387,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 // slices: the next tile's first slices are on their way while a tile ends, and its results leave from
 // registers and are not waited for.
 // RELU: of max(A, 0); MASK: the output is masked by codes and has no bias (each would take 16 registers).
+// Measured, M x K x N: 220000 x 256 x 256 180 us with its codes = 0.96 PFLOP/s of plane products (506 MB: 102 us at a copy's
+// rate), 4096 x 4096 x 4096 730 us = 1.13.  Bound by the matrix cores' power (57 % busy at 1.8 - 2.0 GHz): the split's
+// instructions between the products, the split of half the waves a phase later or fewer instructions in the
+// epilogue are within 2 % of this.
 template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
 __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, int32_t tiles, int32_t nt) {
   constexpr int W = WM * WN, T = 64 * W, FM = BM / WM / 16, FN = BN / WN / 16;
@@ -759,7 +768,7 @@ int launch_low_gemm(const LowGemm& g, hipStream_t s) {
 // rows of x codes.  WK = 4: the waves share 16 channels and a quarter of the sum each (few rows, long sums);
 // WK = 1: 16 channels each (short sums).
 // DX >= 0: x is encoded here, by every workgroup for itself, while the first weights are on their way: one
-// launch instead of two, worth it up to 8192 values a workgroup.
+// launch instead of two, worth it up to 8192 values a workgroup.  1 x 8192 x 8192 bfloat16: 17.3 us, 3.9 TB/s of weight.
 constexpr int SMALL_PAD = 16;  // bytes behind a row of codes in LDS: rows start 4 banks apart
 
 template <int DX, bool VEC, int MT, int WK>
@@ -978,6 +987,8 @@ int launch_low_small(const LowSmall& a, hipStream_t s) {
 // make the 8 sum indices of a lane's operand: m = 4 q + e and 16 + 4 q + e, the same for both operands.
 // Rows of BN (BK) elements are cut into 32-byte units; unit u of row m lies at u ^ (m & 7): the 8 rows
 // that 32 lanes read together then cover all 64 banks.
+// Measured, M x K x N: bfloat16 8192 x 4096 x 4096 227 us = 1.21 PFLOP/s (the values' decoding 11 us besides), 220000 x 256 x
+// 256 81 us; float 220000 x 256 x 256 101 us = 0.86 PFLOP/s of plane products, both with the sums of the parts.
 __device__ __forceinline__ uint2 tr_read(uint32_t at) {
   typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)at));
@@ -1203,7 +1214,7 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
     for (int v = 0; v < FK; ++v) acc[u][v] = zero4();
   const int wn = (wave / WK) * (BN / WN), wk = (wave % WK) * (BK / WK);
   // 16-bit dY: the bias gradient as products with ones, every kt-th stage by each tile column and every
-  // WK-th block of n by each wave
+  // WK-th block of n by each wave (65536 x 1024 x 1024: workgroups that read dY again for it took 115 us more)
   constexpr int FB = NP == 1 ? FN / WK : 1;
   floatx4 bias[FB];
 #pragma unroll

@@ -267,6 +267,41 @@ int main() {
     EXPECT(nc_imap_render_workspace_bytes(&ir) > 0, "iMAP* workspace");
     ir.n_strat = 0;
     EXPECT(nc_imap_render_workspace_bytes(&ir) == 0, "iMAP*: n_strat 0");
+    ir.n_strat = 32;
+    ir.flags = NC_SAVE_FOR_BACKWARD | NC_CODED_ACTIVATIONS;
+    EXPECT(nc_imap_render_workspace_bytes(&ir) > 0, "iMAP*: workspace with 8-bit checkpoints");
+    EXPECT(nc_imap_features(nullptr, 5, nullptr, nullptr, nullptr) < 0, "iMAP* features: NULL");
+    nc_codes_args c;
+    std::memset(&c, 0, sizeof(c));
+    EXPECT(nc_encode_rows(&c, nullptr) == -2, "codes: ABI version");
+    c.abi_version = NC_ABI_VERSION;
+    c.rows = 4; c.cols = 100; c.stride = 100; c.code_stride = 256;
+    EXPECT(nc_encode_rows(&c, nullptr) < 0 && nc_decode_rows(&c, nullptr) < 0, "codes: code_stride");
+    c.code_stride = 128;
+    EXPECT(nc_encode_rows(&c, nullptr) < 0 && nc_decode_rows(&c, nullptr) < 0, "codes: NULL");
+    nc_qlinear_args q;
+    std::memset(&q, 0, sizeof(q));
+    q.abi_version = NC_ABI_VERSION;
+    q.x = fake_f(1);
+    nc_layer_args l;
+    std::memset(&l, 0, sizeof(l));
+    l.abi_version = NC_ABI_VERSION;
+    const int64_t sizes[][3] = {{1, 1, 1}, {200, 93, 256}, {777, 2048, 1030}, {220000, 256, 256}, {3, 131072, 131072}, {1 << 26, 3, 128}};
+    for (const auto& d : sizes)
+      for (int dt = NC_F32; dt <= NC_BF16; ++dt) {
+        q.dtype = q.out_dtype = l.dtype = dt;
+        q.rows = l.rows = d[0]; q.inputs = l.inputs = d[1]; q.outputs = l.outputs = d[2];
+        q.code_stride = l.code_stride = (d[1] + 127) / 128 * 128;
+        EXPECT(nc_quantized_linear_workspace_bytes(&q) > 0, "quantized linear: workspace");
+        EXPECT(nc_layer_workspace_bytes(&l, 0) > 0 && nc_layer_workspace_bytes(&l, 1) > 0, "layer: workspace");
+      }
+    l.rows = q.rows = INT64_MAX;
+    EXPECT(nc_layer_workspace_bytes(&l, 1) == 0 && nc_quantized_linear_workspace_bytes(&q) == 0, "layer: rows");
+    l.rows = 4; l.inputs = 100; l.code_stride = 128; l.dy_stride = INT64_MAX;
+    EXPECT(nc_layer_backward(&l, nullptr, 0, nullptr) < 0, "layer: stride");
+    l.dy_stride = l.outputs;
+    EXPECT(nc_layer_forward(&l, nullptr, 0, nullptr) < 0, "layer: NULL");
+    EXPECT(nc_quantized_linear(nullptr, nullptr, 0, nullptr) < 0, "quantized linear: NULL");
   }
   std::fprintf(stderr, "abi_host_check: %s (%d failures)\n", g_fail ? "FAILED" : "ok", g_fail);
   return g_fail ? 1 : 0;
