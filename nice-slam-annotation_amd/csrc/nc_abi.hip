@@ -1774,12 +1774,13 @@ bool in_place(int dtype, const void* p, int64_t cols, int64_t stride) {
          (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
-// [rows][cols] as the matrix kernels read it: in place, or a padded copy (float B: three planes) in the
+// [rows][cols] as the matrix kernels read it: in place, or a padded copy (float B: two planes) in the
 // workspace; float A is read as it is
 struct Operand {
   bool copy;
   size_t at;               // workspace
   int64_t stride, plane;   // elements
+  size_t unit = 0;         // float B: its rows' units
 };
 Operand operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t stride, bool change, size_t& o) {
   Operand r;
@@ -1787,7 +1788,11 @@ Operand operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t st
   r.at = o;
   r.stride = r.copy ? round_up(cols, ROW_ALIGN) : stride;
   r.plane = r.copy ? rows * r.stride : 0;
-  o = align256(o + (r.copy ? (size_t)(dtype == NC_F32 ? 3 : 1) * (size_t)r.plane * 2 : 0));
+  o = align256(o + (r.copy ? (size_t)(dtype == NC_F32 ? 2 : 1) * (size_t)r.plane * 2 : 0));
+  if (dtype == NC_F32) {
+    r.unit = o;
+    o = align256(o + (size_t)rows * 4);
+  }
   return r;
 }
 Operand operand_a(int dtype, const void* p, int64_t rows, int64_t cols, int64_t stride, bool change, size_t& o) {
@@ -1797,7 +1802,7 @@ Operand operand_a(int dtype, const void* p, int64_t rows, int64_t cols, int64_t 
 
 struct LayerWs {
   Operand a, b;            // the forward's x and W, the backward's dY and W^T
-  size_t gemm_part = 0, part = 0, sums = 0, values = 0, total = 0;
+  size_t gemm_part = 0, part = 0, sums = 0, values = 0, tops = 0, total = 0;
   bool decodes = false;    // dW: the codes' values are written out first
   int32_t gemm_splits = 1, splits = 0, pieces = 0;
   int64_t rows_per = 0;
@@ -1814,6 +1819,8 @@ void layer_layout(const nc_layer_args* a, bool backward, LayerWs& w) {
   } else {
     w.a = operand_a(a->dtype, a->dy, a->rows, k, a->dy_stride, false, o);
     w.b = operand(a->dtype, nullptr, n, k, 0, true, o);
+    w.tops = o;
+    if (a->dtype == NC_F32) o = align256(o + (size_t)((k + TOP_ROWS - 1) / TOP_ROWS) * (size_t)n * 4);
     low_wgrad_splits(a->dtype, a->rows, a->outputs, a->inputs, a->dw != nullptr, w.splits, w.pieces, w.rows_per);
     w.part = o;
     o = align256(o + (size_t)w.splits * (size_t)a->outputs * (size_t)a->inputs * 4);
@@ -1839,7 +1846,8 @@ int layer_check(const nc_layer_args* a) {
     return fail(-1, "nicecore: negative row stride");
   if (int e = check_written(a->y, a->rows, a->outputs, a->y_stride)) return e;
   if (int e = check_written(a->dx, a->rows, a->inputs, a->dx_stride)) return e;
-  if (a->x_stride > NC_MAX_STRIDE || a->dy_stride > NC_MAX_STRIDE) return fail(-1, "nicecore: row strides must not exceed 2^22 elements");
+  if (std::max(std::max(a->x_stride, a->dy_stride), std::max(a->y_stride, a->dx_stride)) > NC_MAX_STRIDE)
+    return fail(-1, "nicecore: row strides must not exceed 2^22 elements");
   return 0;
 }
 
@@ -1861,7 +1869,6 @@ int copy_operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t s
   if (op.copy) {
     c.copy = at<uint16_t>(ws, op.at);
     c.copy_stride = op.stride;
-    c.plane = op.plane;
   }
   if (!codes && !op.copy) return 0;
   return run_encode(c, s);
@@ -1879,6 +1886,7 @@ LowGemm layer_gemm(int dtype, const void* A, const void* B, const LayerWs& w, vo
   g.N = N;
   g.K = K;
   g.mode = layer_mode(dtype);
+  if (dtype == NC_F32) g.col_scale = at<float>(ws, w.b.unit);
   g.slices = (int32_t)(dtype == NC_F32 ? (K + 31) / 32 : (K + ROW_ALIGN - 1) / ROW_ALIGN);
   g.out_dtype = dtype;
   g.bias_dtype = dtype;
@@ -2029,7 +2037,20 @@ int nc_layer_forward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* st
     if (int e = copy_operand(a->dtype, a->x, a->rows, a->inputs, a->x_stride, a->relu != 0, w.a, ws, s, a->codes, a->steps,
                              a->code_stride))
       return e;
-  if (int e = copy_operand(a->dtype, a->w, a->outputs, a->inputs, a->w_stride, false, w.b, ws, s)) return e;
+  if (f32) {
+    SplitCtx c;
+    c.rows = a->outputs;
+    c.cols = a->inputs;
+    c.x = static_cast<const float*>(a->w);
+    c.x_stride = a->w_stride;
+    c.dst = at<uint16_t>(ws, w.b.at);
+    c.dst_stride = w.b.stride;
+    c.plane = w.b.plane;
+    c.unit = at<float>(ws, w.b.unit);
+    if (int e = check_hip(timed(KID_CODES, s, [&] { return launch_split(c, s); }), "split")) return e;
+  } else if (int e = copy_operand(a->dtype, a->w, a->outputs, a->inputs, a->w_stride, false, w.b, ws, s)) {
+    return e;
+  }
   LowGemm g = layer_gemm(a->dtype, a->x, a->w, w, ws, a->rows, a->outputs, a->inputs);
   g.out = a->y;
   g.ldc = a->y_stride;
@@ -2076,6 +2097,8 @@ int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* s
     t.dst = at<uint16_t>(ws, w.b.at);
     t.dst_stride = w.b.stride;
     t.plane = w.b.plane;
+    t.unit = at<float>(ws, w.b.unit);
+    t.tops = at<uint32_t>(ws, w.tops);
     if (int e = check_hip(timed(KID_CODES, s, [&] { return launch_transpose(t, s); }), "transpose")) return e;
     LowGemm g = layer_gemm(a->dtype, a->dy, nullptr, w, ws, a->rows, a->inputs, a->outputs);
     g.out = a->dx;

@@ -46,14 +46,26 @@ struct CodeCtx {
   int64_t zero_rows;       // decode: rows of zeros behind them
   // encode of the layer's input: what the matrix kernel reads besides
   int32_t relu;            // max(x, 0) in the 16-bit copy / planes
-  uint16_t* copy;          // 16-bit x: [rows][copy_stride]; float x: three bfloat16 planes of that
+  uint16_t* copy;          // 16-bit x: [rows][copy_stride]
   int64_t copy_stride;     // elements, a multiple of 64
-  int64_t plane;           // elements between planes
 };
 int launch_encode(const CodeCtx& c, hipStream_t s);   // ROW, or groups (+ copy), or copy alone
 int launch_decode(const CodeCtx& c, hipStream_t s);
 
-// dst[c][r] = src[r][c], rows padded with zeros to dst_stride (a multiple of 64); float: three planes
+// a float matrix as two half planes [rows][dst_stride] (a multiple of 64), each row by a power of two of its own
+// (split2), which `unit` undoes
+struct SplitCtx {
+  int64_t rows, cols;
+  const float* x;
+  int64_t x_stride;
+  uint16_t* dst;
+  int64_t dst_stride, plane;  // elements
+  float* unit;             // [rows]
+};
+int launch_split(const SplitCtx& c, hipStream_t s);
+
+// dst[c][r] = src[r][c], rows padded with zeros to dst_stride (a multiple of 64); float: split planes of it
+constexpr int TOP_ROWS = 256;
 struct TransposeCtx {
   int32_t dtype;
   int64_t rows, cols;
@@ -61,6 +73,8 @@ struct TransposeCtx {
   int64_t src_stride;
   uint16_t* dst;
   int64_t dst_stride, plane;
+  float* unit;             // float: [cols]
+  uint32_t* tops;          // float: scratch [ceil(rows / TOP_ROWS)][cols]
 };
 int launch_transpose(const TransposeCtx& c, hipStream_t s);
 
@@ -69,7 +83,7 @@ struct LowGemm {
   const uint8_t* A;        // rows of lda bytes: int8 codes or 16-bit elements, 128-byte slices
   const uint8_t* B;
   int64_t lda, ldb;        // bytes
-  int64_t plane_b;         // bytes between planes (LOW_F32)
+  int64_t plane_b;         // bytes between B's two planes (LOW_F32)
   int64_t M, N;
   int32_t slices;          // 128-byte slices of a row (LOW_F32: of 32 columns)
   int32_t mode;            // LOW_I8 / LOW_BF16 / LOW_F16
@@ -77,11 +91,11 @@ struct LowGemm {
   void* out;               // [M][ldc] elements
   int64_t ldc;
   const void* bias;        // [N] or NULL
-  const float* row_scale;  // LOW_I8: [M], [N]
-  const float* col_scale;
+  const float* row_scale;  // LOW_I8: [M]
+  const float* col_scale;  // LOW_I8, LOW_F32: [N]
   const uint8_t* mask;     // output zeroed where the code [m][n] is 0, or NULL
   int64_t ldm;
-  // LOW_F32: A is float [M][lda / 4] with K columns, split into planes while it is staged (B: three planes,
+  // LOW_F32: A is float [M][lda / 4] with K columns, split into planes while it is staged (B: two planes,
   // slices of 32 columns); a_relu: of max(A, 0); codes: its 8-bit checkpoint is written besides
   int64_t K;
   int32_t a_relu;
@@ -174,6 +188,27 @@ __device__ __forceinline__ void split3(const float (&x)[8], uint4 (&plane)[3]) {
       for (int e = 0; e < 8; ++e) r[e] = r[e] - cut_bf16(r[e]);
   }
 }
+
+// x scale = x0 + x1 in half, |x scale| < 2^15: x0 the nearest, x1 what is left, rounded: within 2^-22 of |x| or, for
+// an x below 2^-18 of that bound, 2^-25 / scale.  Of 8 values: a plane is 4 words.  An infinity leaves a
+// NaN in the second plane.
+__device__ __forceinline__ void split2(const float (&x)[8], float scale, uint4 (&plane)[2]) {
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = x[2 * j] * scale, b = x[2 * j + 1] * scale;
+    const _Float16 ah = (_Float16)a, bh = (_Float16)b;
+    const _Float16 al = (_Float16)(a - (float)ah), bl = (_Float16)(b - (float)bh);
+    hi[j] = __builtin_bit_cast(uint16_t, ah) | (uint32_t)__builtin_bit_cast(uint16_t, bh) << 16;
+    lo[j] = __builtin_bit_cast(uint16_t, al) | (uint32_t)__builtin_bit_cast(uint16_t, bl) << 16;
+  }
+  plane[0] = uint4{hi[0], hi[1], hi[2], hi[3]};
+  plane[1] = uint4{lo[0], lo[1], lo[2], lo[3]};
+}
+// the scale of split2 for values whose largest has these magnitude bits: 2^(14 - its exponent); its biased exponent
+// is taken as `least` at least (subnormal groups), 254 at most (infinities)
+__device__ __forceinline__ int top_exponent(uint32_t top, int least) { return min(max((int)(top >> 23), least), 254); }
+__device__ __forceinline__ float split_scale(int e) { return __builtin_bit_cast(float, (uint32_t)(268 - e) << 23); }
 
 // biased exponent of a group's step from the bits of its amax (magnitude bits)
 __device__ __forceinline__ int step_byte(uint32_t amax, bool relu) {

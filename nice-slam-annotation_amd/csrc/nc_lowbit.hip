@@ -138,8 +138,8 @@ __global__ void __launch_bounds__(NT == 64 ? 256 : NT) k_encode_rows(const CodeC
 // ---- groups with one step, and the copies for the matrix kernels ----------------------------------------
 // A thread takes one chunk of 8 columns; 4 neighbouring lanes are a group of 32 (rows hold a multiple
 // of 4 chunks and workgroups of 256 threads start on one, so a group never crosses a row or a wave).
-// FMT: -1 no codes; OUT: 0 none, 1 a 16-bit copy (max(x, 0) when relu), 2 three bfloat16 planes (of a weight).
-template <int DT, bool VEC, int FMT, int OUT>
+// FMT: -1 no codes; COPY: a 16-bit copy (max(x, 0) when relu).
+template <int DT, bool VEC, int FMT, bool COPY>
 __global__ void __launch_bounds__(256) k_encode_groups(const CodeCtx a, int64_t row_chunks, int64_t total) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= total) return;  // a multiple of 4: whole groups
@@ -160,16 +160,7 @@ __global__ void __launch_bounds__(256) k_encode_groups(const CodeCtx a, int64_t 
       if ((c & 3) == 0) reinterpret_cast<uint8_t*>(a.scales)[r * (a.code_stride / CODE_GROUP) + (c >> 2)] = (uint8_t)sb;
     }
   }
-  if (OUT > 0 && 8 * c < a.copy_stride) {
-    if (OUT == 1) {
-      store8<DT == NC_F32 ? NC_BF16 : DT, true>(a.copy, r * a.copy_stride, c, a.copy_stride, v);  // exact: v is of that type
-    } else {
-      uint4 p[3];
-      split3(v, p);
-#pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(a.copy + k * a.plane + r * a.copy_stride + 8 * c) = p[k];
-    }
-  }
+  if (COPY && 8 * c < a.copy_stride) store8<DT, true>(a.copy, r * a.copy_stride, c, a.copy_stride, v);  // exact: v is of that type
 }
 
 template <int DT, bool VEC>
@@ -200,6 +191,56 @@ __global__ void __launch_bounds__(256) k_decode(const CodeCtx a, int64_t row_chu
   store8<DT, VEC>(a.values, r * a.x_stride, c, a.cols, v);
 }
 
+// ---- float matrices in two half planes --------------------------------------------------------------------
+// a wave a row, read twice (the second time from the cache)
+template <bool VEC>
+__global__ void __launch_bounds__(256) k_split(const SplitCtx a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= a.rows) return;
+  const int64_t off = r * a.x_stride;
+  uint32_t top = 0;
+  for (int64_t c = lane; 8 * c < a.cols; c += 64) {
+    float v[8];
+    load8<NC_F32, VEC>(a.x, off, c, a.cols, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, mag_bits(v[e]));  // (columns behind the last are copies)
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+  const int e = top_exponent(top, 15);
+  if (lane == 0) a.unit[r] = __builtin_bit_cast(float, (uint32_t)e << 23);
+  for (int64_t c = lane; 8 * c < a.dst_stride; c += 64) {
+    float v[8];
+    load8<NC_F32, VEC>(a.x, off, c, a.cols, v);
+    clear8<VEC>(c, a.cols, v);
+    uint4 p[2];
+    split2(v, split_scale(e), p);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(a.dst + k * a.plane + r * a.dst_stride + 8 * c) = p[k];
+  }
+}
+
+// the largest magnitude of each column in every TOP_ROWS rows: 64 columns a workgroup, a quarter of the rows a wave
+__global__ void __launch_bounds__(256) k_tops(const TransposeCtx a) {
+  __shared__ uint32_t red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane, cc = c < a.cols ? c : a.cols - 1;
+  const int64_t r0 = (int64_t)blockIdx.y * TOP_ROWS + wave * (TOP_ROWS / 4);
+  const float* x = reinterpret_cast<const float*>(a.src) + cc;
+  uint32_t top = 0;
+  for (int k = 0; k < TOP_ROWS / 4; k += 16) {
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = x[(r0 + k + j < a.rows ? r0 + k + j : a.rows - 1) * a.src_stride];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = max(top, mag_bits(v[j]));
+  }
+  red[wave][lane] = top;
+  __syncthreads();
+  if (wave == 0 && c < a.cols) a.tops[blockIdx.y * a.cols + c] = max(max(red[0][lane], red[1][lane]), max(red[2][lane], red[3][lane]));
+}
+
 // ---- transpose into padded 16-bit rows: 64 x 64 tiles through LDS -------------------------------------
 // A lane loads 16 bytes of its row (VEC; else element by element) and writes them down a column of the tile:
 // a wave's 64 lanes are a column's 64 elements, side by side in LDS.  Then 8 lanes write a row of the
@@ -228,6 +269,13 @@ __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
   for (int j = 0; j < CH; ++j)
 #pragma unroll
     for (int e = 0; e < EC; ++e) tile[EC * (wave + 4 * j) + e][lane] = in ? v[j][e] : E(0);
+  __shared__ uint32_t red[4][64];
+  if (DT == NC_F32) {  // the columns' exponents
+    const int64_t c = c0 + lane < a.cols ? c0 + lane : a.cols - 1, parts = (a.rows + TOP_ROWS - 1) / TOP_ROWS;
+    uint32_t top = 0;
+    for (int64_t k = wave; k < parts; k += 4) top = max(top, a.tops[k * a.cols + c]);
+    red[wave][lane] = top;
+  }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -238,10 +286,12 @@ __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = tile[cc][r8 + e];
-      uint4 p[3];
-      split3(x, p);
+      const int e = top_exponent(max(max(red[0][cc], red[1][cc]), max(red[2][cc], red[3][cc])), 15);
+      if (r0 + r8 == 0) a.unit[c0 + cc] = __builtin_bit_cast(float, (uint32_t)e << 23);
+      uint4 p[2];
+      split2(x, split_scale(e), p);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(d + k * a.plane) = p[k];
+      for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(d + k * a.plane) = p[k];
     } else {
       *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(&tile[cc][r8]);
     }
@@ -318,11 +368,11 @@ static int encode_groups(const CodeCtx& c, hipStream_t s) {
   const int64_t rc = width / 8, total = rc * c.rows;
   const dim3 g(blocks_of(total, 256));
   if (c.copy) {
-    if constexpr (DT == NC_F32 && FMT >= 0) return (int)hipErrorInvalidValue;  // float inputs are read as they are
-    else hipLaunchKernelGGL((k_encode_groups<DT, VEC, FMT, DT == NC_F32 ? 2 : 1>), g, dim3(256), 0, s, c, rc, total);
+    if constexpr (DT == NC_F32) return (int)hipErrorInvalidValue;  // float inputs are read as they are
+    else hipLaunchKernelGGL((k_encode_groups<DT, VEC, FMT, true>), g, dim3(256), 0, s, c, rc, total);
   } else {
     if constexpr (FMT < 0) return (int)hipErrorInvalidValue;
-    else hipLaunchKernelGGL((k_encode_groups<DT, VEC, FMT, 0>), g, dim3(256), 0, s, c, rc, total);
+    else hipLaunchKernelGGL((k_encode_groups<DT, VEC, FMT, false>), g, dim3(256), 0, s, c, rc, total);
   }
   return (int)hipGetLastError();
 }
@@ -371,8 +421,16 @@ int launch_decode(const CodeCtx& c, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
+int launch_split(const SplitCtx& c, hipStream_t s) {
+  if (c.rows <= 0 || c.cols <= 0) return 0;
+  if (load8_vec(c.x, c.x_stride, c.cols, NC_F32)) hipLaunchKernelGGL((k_split<true>), dim3(blocks_of(c.rows, 4)), dim3(256), 0, s, c);
+  else hipLaunchKernelGGL((k_split<false>), dim3(blocks_of(c.rows, 4)), dim3(256), 0, s, c);
+  return (int)hipGetLastError();
+}
+
 template <int DT>
 static int transpose(const TransposeCtx& c, hipStream_t s) {
+  if (DT == NC_F32) hipLaunchKernelGGL(k_tops, dim3(blocks_of(c.cols, 64), blocks_of(c.rows, TOP_ROWS)), dim3(256), 0, s, c);
   const dim3 g(blocks_of(c.dst_stride, 64), blocks_of(c.cols, 64));
   if (load8_vec(c.src, c.src_stride, c.cols, c.dtype)) hipLaunchKernelGGL((k_transpose<DT, true>), g, dim3(256), 0, s, c);
   else hipLaunchKernelGGL((k_transpose<DT, false>), g, dim3(256), 0, s, c);

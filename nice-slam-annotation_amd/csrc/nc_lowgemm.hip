@@ -2,10 +2,8 @@
 //
 // k_low_gemm    C[m][n] = sum_k A[m][k] B[n][k]: int8 codes (v_mfma_i32_16x16x64_i8, exact sums) or
 //               16-bit elements (v_mfma_f32_16x16x32_bf16 / _f16, float sums).
-// k_low_gemm_f  the same for float A: six products of bfloat16 planes (split3: x = x0 + x1 + x2),
-//               x0 y0 + x0 y1 + x1 y0 + x0 y2 + x1 y1 + x2 y0; what is left out is below 2^-22 of |x y|,
-//               2^-24.5 on average.
-//               A is split while it is staged, and its 8-bit checkpoint written besides.
+// k_low_gemm_f  the same for float A: three products of half planes with scales (split2).  A is split while it is
+//               staged, and its 8-bit checkpoint written besides.
 // k_low_small   the int8 product of few rows or short sums, x encoded within it.
 // k_low_wgrad   dW[n][k] = sum_m dY[m][n] V[m][k], V the values of an 8-bit checkpoint, decoded while a
 //               tile is staged or written out before (a code times a power of two is exact in 16 bits), both
@@ -376,29 +374,36 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 }
 
 // ---- float A ------------------------------------------------------------------------------------------
-// The same pipeline over slices of 32 columns.  Planes lie in LDS as rows of 64 bytes, 16-byte chunk c of
-// row r at c ^ F((r >> 2) & 3), F = (0, 2, 3, 1): conflict-free for ds_read_b128 (the third weight plane's
-// layout of nc_device.h).  A's floats go into a piece of LDS of their own, where each lane finds the 8
-// columns that it asked for; it splits them and writes the planes before a slice's last phases.  4
-// neighbouring lanes hold a group of 32 columns, so the workgroups of the first column tile write the
-// checkpoint's codes in passing.  The six products of a slice are its phases; their order keeps few
-// planes alive: a2 b0, a1 b0, a0 b0, a1 b1, a0 b1, a0 b2.
+// The same pipeline over slices of 32 columns, as three products of half planes: x = (x0 + x1) / scale
+// (split2), C = x0 y0 + x0 y1 + x1 y0.  A's scale is a power of two of a row's 32 columns, so a slice's sum is
+// multiplied by its inverse (`units`) as it is added to the float accumulator; B's is one of its row, undone in the
+// epilogue.  A value keeps 22 bits, or 2^-40 of the largest in its group of A (row of B); the product left
+// out is below 2^-22: 2^-20.4 of |x y| at most, about 2^-23 on average.  The sums over slices make up for it: 1.1e-7
+// off the exact result at 200 x 93 x 256 (a plain float product 2.9e-7), 3.0e-7 at 2048 x 1024 x 4096 (1.1e-6).  Six products of
+// exact bfloat16 planes, 2.5e-7 and 5.1e-7 there, are twice the work for matrix cores that are bound by their power:
+// 4096 x 4096 x 4096 740 us, here 430.
+// Planes lie in LDS as rows of 64 bytes, 16-byte chunk c of row r at c ^ F((r >> 2) & 3), F = (0, 2, 3, 1):
+// conflict-free for ds_read_b128 (the third weight plane's layout of nc_device.h).  A's floats go into a piece of LDS of their own, where each lane finds the 8
+// columns that it asked for; it splits them and writes the planes.  4 neighbouring lanes hold a group of 32 columns,
+// so the workgroups of the first column tile write the checkpoint's codes in passing.
+// A slice goes block by block of 16 rows: its 3 FN products while the block before is added and the next one's planes
+// are read; the last block's products take turns with the reads of the next slice's B.
 // A layer's sums are short (8 slices for 256 inputs), so a workgroup goes through its tiles as one stream of
 // slices: the next tile's first slices are on their way while a tile ends, and its results leave from
 // registers and are not waited for.
 // RELU: of max(A, 0); MASK: the output is masked by codes and has no bias (each would take 16 registers).
-// Measured, M x K x N: 220000 x 256 x 256 180 us with its codes = 0.96 PFLOP/s of plane products (506 MB: 102 us at a copy's
-// rate), 4096 x 4096 x 4096 730 us = 1.13.  Bound by the matrix cores' power (57 % busy at 1.8 - 2.0 GHz): the split's
-// instructions between the products, the split of half the waves a phase later or fewer instructions in the
-// epilogue are within 2 % of this.
+// Measured, M x K x N: 220000 x 256 x 256 159 us with its codes (506 MB: 102 us at a copy's rate; all workgroups store at
+// once, and loads behind stores wait for them), 4096 x 4096 x 4096 430 us = 0.96 PFLOP/s of plane products.
 template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
 __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, int32_t tiles, int32_t nt) {
   constexpr int W = WM * WN, T = 64 * W, FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int APL = BM * 64, BPL = BN * 64, STAGE = 3 * (APL + BPL);
+  constexpr int APL = BM * 64, BPL = BN * 64, STAGE = 2 * (APL + BPL);
   constexpr int XA = BM * 4 / T;                   // chunks of A a thread
   constexpr int LA = XA * (VEC ? 2 : 8);           // loads of A a wave
-  constexpr int LB = 3 * BPL / 1024 / W;           // 1-KB loads of B a wave
-  static_assert(BM * 4 % T == 0 && 3 * BPL % (1024 * W) == 0, "whole chunks a thread, whole loads a wave");
+  constexpr int LB = 2 * BPL / 1024 / W;           // 1-KB loads of B a wave
+  constexpr int RAW = 2 * STAGE, UNITS = RAW + W * XA * 2048;  // A's floats, then its units [2][BM]
+  static_assert(BM * 4 % T == 0 && 2 * BPL % (1024 * W) == 0, "whole chunks a thread, whole loads a wave");
+  static_assert(FM % 2 == 0 && FN % 2 == 0, "pairs");
   extern __shared__ __attribute__((aligned(256))) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
@@ -407,7 +412,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   const int mine = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
   const int steps = mine * total;
   const uint32_t lds0 = lds_address(lds);
-  unsigned char* raw = lds + 2 * STAGE + wave * (XA * 2048);  // this wave's floats
+  unsigned char* raw = lds + RAW + wave * (XA * 2048);  // this wave's floats
+  float* const units = reinterpret_cast<float*>(lds + UNITS);
   const int pads = (int)(g.code_stride / CODE_GROUP) - g.slices;  // code groups behind the last slice
   auto tile_at = [&](int k, int64_t& m0, int64_t& n0) {
     const uint32_t t = (uint32_t)chiplet_order(blockIdx.x + k * gridDim.x, tiles), tm = t / (uint32_t)nt;
@@ -455,7 +461,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
     xm0 = lm0;
     xt = first + lt;
     xcode = g.codes && ln0 == 0;
-    const uint32_t to = lds0 + 2 * STAGE + wave * (XA * 2048);
+    const uint32_t to = lds0 + RAW + wave * (XA * 2048);
 #pragma unroll
     for (int l = 0; l < XA; ++l) {
       const int c = 8 * (4 * xt + (int)(threadIdx.x & 3)), k = (int)g.K;
@@ -472,7 +478,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
 #pragma unroll
     for (int j = 0; j < LB; ++j) {
       const int pl = (wave * LB + j) * 16 / BN;
-      load_lds16(b_next + pl * g.plane_b, ob[j], lds0 + half * STAGE + 3 * APL + (wave * LB + j) * 1024);
+      load_lds16(b_next + pl * g.plane_b, ob[j], lds0 + half * STAGE + 2 * APL + (wave * LB + j) * 1024);
     }
     b_next += 64;
     if (++lt == total) {
@@ -508,10 +514,17 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
           if (c == 0) (g.steps + xm0 * sr)[(uint32_t)(r * sr + xt)] = (uint8_t)sb;
         }
       }
-      uint4 p[3];
-      split3(x, p);
+      uint32_t top = 0;
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(s + k * APL + r * 64 + hchunk3(r, c)) = p[k];
+      for (int e = 0; e < 8; ++e) top = max(top, mag_bits(x[e]));
+      top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true));  // lane ^ 1
+      top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4e, 0xf, 0xf, true));  // lane ^ 2
+      const int e = top_exponent(top, 29);  // sums are kept in units of B's row: 2^(e - 141) 2^-14
+      if (c == 0) units[half * BM + r] = __builtin_bit_cast(float, (uint32_t)(e - 28) << 23);
+      uint4 p[2];
+      split2(x, split_scale(e), p);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(s + k * APL + r * 64 + hchunk3(r, c)) = p[k];
     }
     xcode = false;  // a step behind the last one stores the same again, which nobody reads
   };
@@ -522,23 +535,37 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
     for (int v = 0; v < FN; ++v) acc[u][v] = zero4();
   const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
   const unsigned char* fa = lds + (wm + i) * 64 + hchunk3(i, q);  // wm, wn and 16 u leave the chunk order as it is
-  const unsigned char* fb = lds + 3 * APL + (wn + i) * 64 + hchunk3(i, q);
-  uint4 a[3][FM], b[3][FN];
-  auto read_a = [&](int half, int p) {
+  const unsigned char* fb = lds + 2 * APL + (wn + i) * 64 + hchunk3(i, q);
+  uint4 a[2][2], b[2][FN];  // a[block & 1][plane], b[plane][block]
+  floatx4 t[2][FN];         // a block's sums over a slice
+  float unit[FM];
+  auto read_a = [&](int half, int u) {
 #pragma unroll
-    for (int u = 0; u < FM; ++u) a[p][u] = *reinterpret_cast<const uint4*>(fa + half * STAGE + p * APL + 16 * u * 64);
+    for (int p = 0; p < 2; ++p) a[u & 1][p] = *reinterpret_cast<const uint4*>(fa + half * STAGE + p * APL + 16 * u * 64);
   };
-  auto read_b = [&](int half, int p) {
+  auto read_b = [&](int half, int v) {
 #pragma unroll
-    for (int v = 0; v < FN; ++v) b[p][v] = *reinterpret_cast<const uint4*>(fb + half * STAGE + p * BPL + 16 * v * 64);
+    for (int p = 0; p < 2; ++p) b[p][v] = *reinterpret_cast<const uint4*>(fb + half * STAGE + p * BPL + 16 * v * 64);
   };
-  auto multiply = [&](int pa, int pb) {
+  auto read_units = [&](int half) {
+#pragma unroll
+    for (int u = 0; u < FM; ++u) unit[u] = units[half * BM + wm + 16 * u + i];
+  };
+  auto multiply = [&](int u, int v0) {  // blocks (u, v0) and (u, v0 + 1); the smallest products first
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < FM; ++u)
+    for (int v = v0; v < v0 + 2; ++v) t[u & 1][v] = Mac<LOW_F16>::mac(b[0][v], a[u & 1][1], zero4());
 #pragma unroll
-      for (int v = 0; v < FN; ++v) acc[u][v] = Mac<LOW_BF16>::mac(b[pb][v], a[pa][u], acc[u][v]);
+    for (int v = v0; v < v0 + 2; ++v) t[u & 1][v] = Mac<LOW_F16>::mac(b[1][v], a[u & 1][0], t[u & 1][v]);
+#pragma unroll
+    for (int v = v0; v < v0 + 2; ++v) t[u & 1][v] = Mac<LOW_F16>::mac(b[0][v], a[u & 1][0], t[u & 1][v]);
     __builtin_amdgcn_sched_barrier(0);
+  };
+  auto add = [&](int u) {
+#pragma unroll
+    for (int v = 0; v < FN; ++v)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[u][v][j] = __builtin_fmaf(t[u & 1][v][j], unit[u], acc[u][v][j]);
   };
   enter();
   load(0);
@@ -547,60 +574,85 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   lds_barrier();  // (a wave's floats are read before the wave asks for the next ones)
   if (steps > 1) load(1);
   staged_barrier();
-  read_a(0, 2);
-  read_b(0, 0);
+  read_a(0, 0);
+#pragma unroll
+  for (int v = 0; v < FN; ++v) read_b(0, v);
+  read_units(0);
   const bool vec = store4_vec<NC_F32>(g) && (g.splits == 1 || g.N % 4 == 0);
+  float* const to = g.splits > 1 ? g.part + (int64_t)blockIdx.y * g.M * g.N : reinterpret_cast<float*>(g.out);
+  const int64_t ldo = g.splits > 1 ? g.N : g.ldc;
+  const bool biased = g.bias && g.splits == 1;
   constexpr int RESULTS = FM * FN;  // stores of a whole tile's results
   int s = 0;
   bool left = false;  // RESULTS stores were issued after the loads that the next slice waits for: they stay in flight
   auto slice = [&](auto arrived) {
     const int h = s & 1;
-    read_a(h, 1);
-    multiply(2, 0);
-    read_a(h, 0);
-    multiply(1, 0);
-    read_b(h, 1);
-    multiply(0, 0);
-    if (left) wait_loads<LB + RESULTS>();  // A's floats are here, asked for before B's slice
-    else wait_loads<LB>();
-    store_a(h ^ 1);
-    multiply(1, 1);
-    read_b(h, 2);
-    multiply(0, 1);
+#pragma unroll
+    for (int u = 0; u + 1 < FM; ++u) {
+      read_a(h, u + 1);
+#pragma unroll
+      for (int v = 0; v < FN; v += 2) multiply(u, v);
+      if (u > 0) add(u - 1);
+      if (u == (FM > 2 ? 1 : 0)) {
+        if (left) wait_loads<LB + RESULTS>();  // A's floats are here, asked for before B's slice
+        else wait_loads<LB>();
+        store_a(h ^ 1);
+      }
+    }
     if (left) wait_loads<RESULTS>();
     else wait_loads<0>();
     lds_barrier();
     left = false;
     arrived();
     if (s + 2 < steps) load(h);
-    read_a(h ^ 1, 2);
-    read_b(h ^ 1, 0);
-    multiply(0, 2);
+    read_a(h ^ 1, 0);
+#pragma unroll
+    for (int v = 0; v < FN; v += 2) {
+      multiply(FM - 1, v);
+      read_b(h ^ 1, v);
+      read_b(h ^ 1, v + 1);
+    }
+    if (FM > 1) add(FM - 2);
+    add(FM - 1);
+    read_units(h ^ 1);
     ++s;
   };
   for (int k = 0; k < mine; ++k) {
-    for (int t = 0; t + 1 < total; ++t) slice([] {});
+    for (int n = 1; n < total; ++n) slice([] {});
     int64_t m0, n0;
     tile_at(k, m0, n0);
-    float cb[FN][4];  // what the results need, a slice ahead
+    float cb[FN][4], cs[FN][4];  // what the results need, a slice ahead; without a branch (what a branch loads is waited for at its end)
     uint32_t mask[FM][FN];
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // computed here: kept, it would take registers that the products need
+    const int row = wm + (ln & 15), col = wn + 4 * (ln >> 4);
+    const float* bias = biased ? reinterpret_cast<const float*>(g.bias) : g.col_scale;
 #pragma unroll
-    for (int v = 0; v < FN; ++v) {
-      const int64_t n = n0 + wn + 16 * v + 4 * q;
-      if (!MASK)
+    for (int v = 0; v < FN; ++v)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          cb[v][j] = g.bias ? reinterpret_cast<const float*>(g.bias)[n + j < g.N ? n + j : g.N - 1] : 0.f;
-      if (MASK)
+      for (int j = 0; j < 4; ++j) {
+        const int c = (int)n0 + col + 16 * v + j, n = c < (int)g.N ? c : (int)g.N - 1;
+        cs[v][j] = g.col_scale[n];
+        if (!MASK) cb[v][j] = bias[n];
+      }
+    if (MASK) {
+      const uint8_t* base = g.mask + m0 * g.ldm;
 #pragma unroll
-        for (int u = 0; u < FM; ++u) {
-          const int64_t m = m0 + wm + 16 * u + i, mm = m < g.M ? m : g.M - 1;
-          mask[u][v] = *reinterpret_cast<const uint32_t*>(g.mask + mm * g.ldm + (n < g.ldm ? n : 0));
+      for (int u = 0; u < FM; ++u) {
+        const int last = (int)(g.M - 1 - m0 < BM ? g.M - 1 - m0 : BM);
+        const uint32_t r = (uint32_t)(row + 16 * u < last ? row + 16 * u : last) * (uint32_t)g.ldm;
+#pragma unroll
+        for (int v = 0; v < FN; ++v) {
+          const int c = (int)n0 + col + 16 * v;
+          mask[u][v] = *reinterpret_cast<const uint32_t*>(base + (r + (c < (int)g.ldm ? (uint32_t)c : 0u)));
         }
+      }
     }
     slice([&] {  // here by now: taken before the next loads, so that nothing is waited for between the stores
 #pragma unroll
       for (int v = 0; v < FN; ++v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(cs[v][j]));
         if (!MASK)
 #pragma unroll
           for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(cb[v][j]));
@@ -609,34 +661,54 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
           for (int u = 0; u < FM; ++u) asm volatile("" : "+v"(mask[u][v]));
       }
     });
-    matrix_drain();
-    float* part = g.splits > 1 ? g.part + (int64_t)blockIdx.y * g.M * g.N : nullptr;
+    if (!MASK && !biased)
 #pragma unroll
-    for (int u = 0; u < FM; ++u) {
-      const int64_t m = m0 + wm + 16 * u + i;
+      for (int v = 0; v < FN; ++v)
 #pragma unroll
-      for (int v = 0; v < FN; ++v) {
-        const int64_t n = n0 + wn + 16 * v + 4 * q;
-        floatx4 o = acc[u][v];
-        acc[u][v] = zero4();
-        if (!part) {
+        for (int j = 0; j < 4; ++j) cb[v][j] = 0.f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            o[j] = MASK ? (((mask[u][v] >> (8 * j)) & 255u) ? o[j] : 0.f) : g.bias ? o[j] + cb[v][j] : o[j];
+    for (int u = 0; u < FM; ++u)
+#pragma unroll
+      for (int v = 0; v < FN; ++v)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // (a cut sum: the mask of each part, no bias)
+          if (MASK) acc[u][v][j] = ((mask[u][v] >> (8 * j)) & 255u) ? acc[u][v][j] * cs[v][j] : 0.f;
+          else acc[u][v][j] = acc[u][v][j] * cs[v][j] + cb[v][j];
         }
-        if (m >= g.M || n >= g.N) continue;
-        float* p = part ? part + m * g.N + n : reinterpret_cast<float*>(g.out) + m * g.ldc + n;
-        if (vec) {
-          *reinterpret_cast<floatx4*>(p) = o;
-        } else {
+    left = vec && m0 + BM <= g.M && n0 + BN <= g.N;  // (a tile cut off by the matrix's end stores less)
+    int at = lane;
+    asm volatile("" : "+v"(at));
+    if (left) {  // offsets in a tile fit 32 bits: row strides are at most 2^22
+      float* const base = to + m0 * ldo + n0;
+      const uint32_t o = 4 * ((uint32_t)(wm + (at & 15)) * (uint32_t)ldo + (uint32_t)(wn + 4 * (at >> 4)));
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (n + j < g.N) p[j] = o[j];
+      for (int u = 0; u < FM; ++u)
+#pragma unroll
+        for (int v = 0; v < FN; ++v)
+          *reinterpret_cast<floatx4*>(reinterpret_cast<unsigned char*>(base) + (o + 64u * u * (uint32_t)ldo) + 64 * v) = acc[u][v];
+    } else {
+#pragma unroll
+      for (int u = 0; u < FM; ++u) {
+        const int64_t m = m0 + wm + 16 * u + (at & 15);
+#pragma unroll
+        for (int v = 0; v < FN; ++v) {
+          const int64_t n = n0 + wn + 16 * v + 4 * (at >> 4);
+          if (m >= g.M || n >= g.N) continue;
+          float* p = to + m * ldo + n;
+          if (vec) {
+            *reinterpret_cast<floatx4*>(p) = acc[u][v];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (n + j < g.N) p[j] = acc[u][v][j];
+          }
         }
       }
     }
-    // (a tile cut off by the matrix's end stores less)
-    left = vec && m0 + BM <= g.M && n0 + BN <= g.N;
+#pragma unroll
+    for (int u = 0; u < FM; ++u)
+#pragma unroll
+      for (int v = 0; v < FN; ++v) acc[u][v] = zero4();
   }
 }
 
@@ -676,7 +748,7 @@ static int run_low_gemm(const LowGemm& g, hipStream_t s) {
 template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
 static int run_low_gemm_f(const LowGemm& g, hipStream_t s) {
   const int64_t mt = (g.M + BM - 1) / BM, nt = (g.N + BN - 1) / BN, tiles = mt * nt;
-  constexpr int lds = 2 * 192 * (BM + BN) + 128 * BM, per_cu = 163840 / lds;  // resident workgroups
+  constexpr int lds = 2 * 128 * (BM + BN) + 128 * BM + 8 * BM, per_cu = 163840 / lds;  // resident workgroups
   auto kernel = k_low_gemm_f<BM, BN, WM, WN, VEC, RELU, MASK>;
   static std::atomic<uint64_t> done{0};
   if (const int e = allow_lds(kernel, lds, done)) return e;
@@ -688,9 +760,9 @@ static int run_low_gemm_f(const LowGemm& g, hipStream_t s) {
 
 // Tiles and cuts of the sum.  256 compute units; a large tile reads less LDS for each product, a small one (or
 // a cut sum) fills the units when the output is small.  M x K x N in us (S, M, L: tiles; x4: cuts):
-//   float     8192 x 1024 x 1024 S 135, M 100, L 91;  4096 x 1024 x 1024 S 67, M 54, L 103;  2048 x 1024 x 1024 S 37,
-//             M 50;  2048 x 4096 x 1024 S 129, M x2 106, L x4 101;  8192 x 8192 x 256 S 278, L x4 189;  65536 x 1024 x 64
-//             S 85, M 103
+//   float     8192 x 1024 x 1024 S 110, M 78, L 67;  4096 x 1024 x 1024 S 61, M 44, L x2 51;  1024 x 4096 x 4096 M 148,
+//             L x2 136;  2048 x 4096 x 1024 S 115, M x2 90, L x4 79;  8192 x 8192 x 256 S 234, L x4 145;  2000 x 2000 x 500
+//             S x2 41, M x4 33;  500 x 1024 x 1024 S x4 22, M x8 23;  65536 x 1024 x 64 S 82, M 95, L 115
 //   bfloat16  8192 x 1024 x 1024 S 32, M 28, L 37;  4096 x 1024 x 1024 S 19, M 22;  1024 x 4096 x 4096 S 61, M 58;
 //             1000 x 1000 x 1000 S 14, S x2 17;  200 x 4096 x 256 S x12 12, x4 13
 //   int8      8192 x 1024 x 1024 S 22, M 20, L 27;  4096 x 1024 x 1024 S 14, M 16;  65536 x 1024 x 64 S 17, M 20, L 27
@@ -707,11 +779,10 @@ static LowCut low_cut(int mode, int64_t M, int64_t N, int64_t K) {
   if (mode == LOW_F32) {
     const int64_t large = N > 128 ? tiles_of(M, N, 128, 256) : 0;
     if (large >= 192) return {TILE_LARGE, 1};
+    auto cut = [&](int64_t tiles, int64_t most) { return tiles > 0 ? std::min(256 / tiles, slices / most) : 0; };
+    if (large * cut(large, 32) >= 192) return {TILE_LARGE, (int)cut(large, 32)};
     if (middle >= 192) return {TILE_MIDDLE, 1};
-    if (large > 0) {
-      const int64_t cuts = std::min(256 / large, slices / 32);
-      if (large * cuts >= 192) return {TILE_LARGE, (int)cuts};
-    }
+    if (middle * cut(middle, 8) >= 192) return {TILE_MIDDLE, (int)cut(middle, 8)};
   } else {
     if (N > 128 && tiles_of(M, N, 256, 256) >= 192) return {TILE_LARGE, 1};
     if (middle >= (slices >= 32 ? 192 : 320)) return {TILE_MIDDLE, 1};
