@@ -5,6 +5,7 @@ Public surface (drop-in for the reference's renderer / decoder APIs):
   nicecore.decoder.NICE / MLP / MLP_no_xyz / get_model
                                    src/conv_onet/models/decoder.py, src/conv_onet/config.py
   nicecore.ops.render_rays / eval_points   functional forms
+  nicecore.lowbit                  8-bit operators of the scene MLP's layers
   nicecore.scene                   bounds, grid shapes/init, presets, synthetic rays
   nicecore.distributed             ray-sharded data parallelism over RCCL
 """
