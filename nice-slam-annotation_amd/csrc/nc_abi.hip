@@ -1780,7 +1780,7 @@ struct Operand {
   bool copy;
   size_t at;               // workspace
   int64_t stride, plane;   // elements
-  size_t unit = 0;         // float B: its rows' units
+  size_t exponent = 0;     // float B: its rows' exponents
 };
 Operand operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t stride, bool change, size_t& o) {
   Operand r;
@@ -1790,7 +1790,7 @@ Operand operand(int dtype, const void* p, int64_t rows, int64_t cols, int64_t st
   r.plane = r.copy ? rows * r.stride : 0;
   o = align256(o + (r.copy ? (size_t)(dtype == NC_F32 ? 2 : 1) * (size_t)r.plane * 2 : 0));
   if (dtype == NC_F32) {
-    r.unit = o;
+    r.exponent = o;
     o = align256(o + (size_t)rows * 4);
   }
   return r;
@@ -1886,7 +1886,7 @@ LowGemm layer_gemm(int dtype, const void* A, const void* B, const LayerWs& w, vo
   g.N = N;
   g.K = K;
   g.mode = layer_mode(dtype);
-  if (dtype == NC_F32) g.col_scale = at<float>(ws, w.b.unit);
+  if (dtype == NC_F32) g.exponent = at<int32_t>(ws, w.b.exponent);
   g.slices = (int32_t)(dtype == NC_F32 ? (K + 31) / 32 : (K + ROW_ALIGN - 1) / ROW_ALIGN);
   g.out_dtype = dtype;
   g.bias_dtype = dtype;
@@ -2046,7 +2046,7 @@ int nc_layer_forward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* st
     c.dst = at<uint16_t>(ws, w.b.at);
     c.dst_stride = w.b.stride;
     c.plane = w.b.plane;
-    c.unit = at<float>(ws, w.b.unit);
+    c.exponent = at<int32_t>(ws, w.b.exponent);
     if (int e = check_hip(timed(KID_CODES, s, [&] { return launch_split(c, s); }), "split")) return e;
   } else if (int e = copy_operand(a->dtype, a->w, a->outputs, a->inputs, a->w_stride, false, w.b, ws, s)) {
     return e;
@@ -2097,7 +2097,7 @@ int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* s
     t.dst = at<uint16_t>(ws, w.b.at);
     t.dst_stride = w.b.stride;
     t.plane = w.b.plane;
-    t.unit = at<float>(ws, w.b.unit);
+    t.exponent = at<int32_t>(ws, w.b.exponent);
     t.tops = at<uint32_t>(ws, w.tops);
     if (int e = check_hip(timed(KID_CODES, s, [&] { return launch_transpose(t, s); }), "transpose")) return e;
     LowGemm g = layer_gemm(a->dtype, a->dy, nullptr, w, ws, a->rows, a->inputs, a->outputs);

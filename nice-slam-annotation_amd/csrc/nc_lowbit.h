@@ -53,14 +53,14 @@ int launch_encode(const CodeCtx& c, hipStream_t s);   // ROW, or groups (+ copy)
 int launch_decode(const CodeCtx& c, hipStream_t s);
 
 // a float matrix as two half planes [rows][dst_stride] (a multiple of 64), each row by a power of two of its own
-// (split2), which `unit` undoes
+// (split2): 2^(141 - exponent)
 struct SplitCtx {
   int64_t rows, cols;
   const float* x;
   int64_t x_stride;
   uint16_t* dst;
   int64_t dst_stride, plane;  // elements
-  float* unit;             // [rows]
+  int32_t* exponent;       // [rows]
 };
 int launch_split(const SplitCtx& c, hipStream_t s);
 
@@ -73,7 +73,7 @@ struct TransposeCtx {
   int64_t src_stride;
   uint16_t* dst;
   int64_t dst_stride, plane;
-  float* unit;             // float: [cols]
+  int32_t* exponent;       // float: [cols]
   uint32_t* tops;          // float: scratch [ceil(rows / TOP_ROWS)][cols]
 };
 int launch_transpose(const TransposeCtx& c, hipStream_t s);
@@ -92,7 +92,8 @@ struct LowGemm {
   int64_t ldc;
   const void* bias;        // [N] or NULL
   const float* row_scale;  // LOW_I8: [M]
-  const float* col_scale;  // LOW_I8, LOW_F32: [N]
+  const float* col_scale;  // LOW_I8: [N]
+  const int32_t* exponent; // LOW_F32: [N], of B's rows
   const uint8_t* mask;     // output zeroed where the code [m][n] is 0, or NULL
   int64_t ldm;
   // LOW_F32: A is float [M][lda / 4] with K columns, split into planes while it is staged (B: two planes,
@@ -189,26 +190,27 @@ __device__ __forceinline__ void split3(const float (&x)[8], uint4 (&plane)[3]) {
   }
 }
 
-// x scale = x0 + x1 in half, |x scale| < 2^15: x0 the nearest, x1 what is left, rounded: within 2^-22 of |x| or, for
-// an x below 2^-18 of that bound, 2^-25 / scale.  Of 8 values: a plane is 4 words.  An infinity leaves a
-// NaN in the second plane.
+// x scale = x0 + x1 in half, |x scale| < 2^15: x0 the nearest, x1 what is left, rounded: within 2^-22 of |x|, or
+// 2^-25 / scale for small ones.  Of 8 values: a plane is 4 words.  An infinity leaves a NaN in the second plane.
+// (Written as fused multiply-adds that end in half: one instruction an element and plane.)
 __device__ __forceinline__ void split2(const float (&x)[8], float scale, uint4 (&plane)[2]) {
   uint32_t hi[4], lo[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float a = x[2 * j] * scale, b = x[2 * j + 1] * scale;
-    const _Float16 ah = (_Float16)a, bh = (_Float16)b;
-    const _Float16 al = (_Float16)(a - (float)ah), bl = (_Float16)(b - (float)bh);
+    const float a = x[2 * j], b = x[2 * j + 1];
+    const _Float16 ah = (_Float16)__builtin_fmaf(a, scale, 0.f), bh = (_Float16)__builtin_fmaf(b, scale, 0.f);
+    const _Float16 al = (_Float16)__builtin_fmaf(a, scale, -(float)ah), bl = (_Float16)__builtin_fmaf(b, scale, -(float)bh);
     hi[j] = __builtin_bit_cast(uint16_t, ah) | (uint32_t)__builtin_bit_cast(uint16_t, bh) << 16;
     lo[j] = __builtin_bit_cast(uint16_t, al) | (uint32_t)__builtin_bit_cast(uint16_t, bl) << 16;
   }
   plane[0] = uint4{hi[0], hi[1], hi[2], hi[3]};
   plane[1] = uint4{lo[0], lo[1], lo[2], lo[3]};
 }
-// the scale of split2 for values whose largest has these magnitude bits: 2^(14 - its exponent); its biased exponent
-// is taken as `least` at least (subnormal groups), 254 at most (infinities)
-__device__ __forceinline__ int top_exponent(uint32_t top, int least) { return min(max((int)(top >> 23), least), 254); }
-__device__ __forceinline__ float split_scale(int e) { return __builtin_bit_cast(float, (uint32_t)(268 - e) << 23); }
+// biased exponent of the largest magnitude, for scales that are normal floats too: zero and subnormals count as 15,
+// infinities as 254
+__device__ __forceinline__ int top_exponent(uint32_t top) { return min(max((int)(top >> 23), 15), 254); }
+// 2^(to - e): what has exponent e is below 2^(to - 126)
+__device__ __forceinline__ float scale_to(int to, int e) { return __builtin_bit_cast(float, (uint32_t)(127 + to - e) << 23); }
 
 // biased exponent of a group's step from the bits of its amax (magnitude bits)
 __device__ __forceinline__ int step_byte(uint32_t amax, bool relu) {

@@ -375,10 +375,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 
 // ---- float A ------------------------------------------------------------------------------------------
 // The same pipeline over slices of 32 columns, as three products of half planes: x = (x0 + x1) / scale
-// (split2), C = x0 y0 + x0 y1 + x1 y0.  A's scale is a power of two of a row's 32 columns, so a slice's sum is
-// multiplied by its inverse (`units`) as it is added to the float accumulator; B's is one of its row, undone in the
-// epilogue.  A value keeps 22 bits, or 2^-40 of the largest in its group of A (row of B); the product left
-// out is below 2^-22: 2^-20.4 of |x y| at most, about 2^-23 on average.  The sums over slices make up for it: 1.1e-7
+// (split2), C = x0 y0 + x0 y1 + x1 y0.  B's scale is a power of two of its row, A's one of its row so far: it puts the
+// first 32 columns' largest below 2^12 and stays until one reaches 2^15, when the row's sums are scaled down with
+// it (seldom after the first slices).  Both are undone in the epilogue.  A value keeps 22 bits, or 2^-36 of the
+// largest before it in its row of A (2^-40 of the largest in its row of B); the product left out is below 2^-22: 2^-20.4 of |x y| at most, about 2^-23 on average.  The sums over slices make up for it: 1.1e-7
 // off the exact result at 200 x 93 x 256 (a plain float product 2.9e-7), 3.0e-7 at 2048 x 1024 x 4096 (1.1e-6).  Six products of
 // exact bfloat16 planes, 2.5e-7 and 5.1e-7 there, are twice the work for matrix cores that are bound by their power:
 // 4096 x 4096 x 4096 740 us, here 430.
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   constexpr int XA = BM * 4 / T;                   // chunks of A a thread
   constexpr int LA = XA * (VEC ? 2 : 8);           // loads of A a wave
   constexpr int LB = 2 * BPL / 1024 / W;           // 1-KB loads of B a wave
-  constexpr int RAW = 2 * STAGE, UNITS = RAW + W * XA * 2048;  // A's floats, then its units [2][BM]
+  constexpr int RAW = 2 * STAGE, EXPS = RAW + W * XA * 2048;  // A's floats, then its exponents [2][BM]
   static_assert(BM * 4 % T == 0 && 2 * BPL % (1024 * W) == 0, "whole chunks a thread, whole loads a wave");
   static_assert(FM % 2 == 0 && FN % 2 == 0, "pairs");
   extern __shared__ __attribute__((aligned(256))) unsigned char lds[];
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   const int steps = mine * total;
   const uint32_t lds0 = lds_address(lds);
   unsigned char* raw = lds + RAW + wave * (XA * 2048);  // this wave's floats
-  float* const units = reinterpret_cast<float*>(lds + UNITS);
+  int32_t* const exps = reinterpret_cast<int32_t*>(lds + EXPS);
   const int pads = (int)(g.code_stride / CODE_GROUP) - g.slices;  // code groups behind the last slice
   auto tile_at = [&](int k, int64_t& m0, int64_t& n0) {
     const uint32_t t = (uint32_t)chiplet_order(blockIdx.x + k * gridDim.x, tiles), tm = t / (uint32_t)nt;
@@ -456,8 +456,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   // what the floats in LDS are: tile and slice, and whether their codes are written
   int64_t xm0 = 0;
   int xt = 0;
-  bool xcode = false;
+  bool xcode = false, xnew = false;  // xnew: a tile's first slice
+  int xe[XA];                        // the exponents that the rows' scales are made of
   auto load = [&](int half) {
+    xnew = lt == 0;
     xm0 = lm0;
     xt = first + lt;
     xcode = g.codes && ln0 == 0;
@@ -501,7 +503,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const float*>(raw + l * 2048 + e * 256 + 4 * lane);
       }
-      clear8<VEC>((int64_t)xt * 4 + c, g.K, x);
+      if ((xt + 1) * 32 > (int)g.K) clear8<VEC>((int64_t)xt * 4 + c, g.K, x);
       if (RELU)
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = relu_keep_nan(x[e]);
@@ -514,15 +516,17 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
           if (c == 0) (g.steps + xm0 * sr)[(uint32_t)(r * sr + xt)] = (uint8_t)sb;
         }
       }
-      uint32_t top = 0;
+      float top = 0.f;  // (NaN counts as nothing: it is one in the planes)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, mag_bits(x[e]));
-      top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true));  // lane ^ 1
-      top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4e, 0xf, 0xf, true));  // lane ^ 2
-      const int e = top_exponent(top, 29);  // sums are kept in units of B's row: 2^(e - 141) 2^-14
-      if (c == 0) units[half * BM + r] = __builtin_bit_cast(float, (uint32_t)(e - 28) << 23);
+      for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, __builtin_fabsf(x[e]));
+      uint32_t bits = __builtin_bit_cast(uint32_t, top);
+      bits = max(bits, (uint32_t)__builtin_amdgcn_mov_dpp((int)bits, 0xb1, 0xf, 0xf, true));  // lane ^ 1
+      bits = max(bits, (uint32_t)__builtin_amdgcn_mov_dpp((int)bits, 0x4e, 0xf, 0xf, true));  // lane ^ 2
+      const int e = top_exponent(bits);
+      xe[l] = xnew || e > xe[l] + 3 ? e : xe[l];
+      if (c == 0) exps[half * BM + r] = xe[l];
       uint4 p[2];
-      split2(x, split_scale(e), p);
+      split2(x, scale_to(138, xe[l]), p);
 #pragma unroll
       for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(s + k * APL + r * 64 + hchunk3(r, c)) = p[k];
     }
@@ -537,8 +541,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   const unsigned char* fa = lds + (wm + i) * 64 + hchunk3(i, q);  // wm, wn and 16 u leave the chunk order as it is
   const unsigned char* fb = lds + 2 * APL + (wn + i) * 64 + hchunk3(i, q);
   uint4 a[2][2], b[2][FN];  // a[block & 1][plane], b[plane][block]
-  floatx4 t[2][FN];         // a block's sums over a slice
-  float unit[FM];
+  int ea[FM], next_ea[FM];  // exponents of the sums, of the next slice's rows
+  bool fresh = true;        // the sums are zero
   auto read_a = [&](int half, int u) {
 #pragma unroll
     for (int p = 0; p < 2; ++p) a[u & 1][p] = *reinterpret_cast<const uint4*>(fa + half * STAGE + p * APL + 16 * u * 64);
@@ -547,25 +551,35 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
 #pragma unroll
     for (int p = 0; p < 2; ++p) b[p][v] = *reinterpret_cast<const uint4*>(fb + half * STAGE + p * BPL + 16 * v * 64);
   };
-  auto read_units = [&](int half) {
+  auto read_exps = [&](int half) {
 #pragma unroll
-    for (int u = 0; u < FM; ++u) unit[u] = units[half * BM + wm + 16 * u + i];
+    for (int u = 0; u < FM; ++u) next_ea[u] = exps[half * BM + wm + 16 * u + i];
+  };
+  auto rescale = [&]() {  // the sums in the units of the slice to come
+    bool differ = false;
+#pragma unroll
+    for (int u = 0; u < FM; ++u) differ = differ || ea[u] != next_ea[u];
+    if (!fresh && __any(differ)) {
+      matrix_drain();
+#pragma unroll
+      for (int u = 0; u < FM; ++u)
+#pragma unroll
+        for (int v = 0; v < FN; ++v)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[u][v][j] = __builtin_ldexpf(acc[u][v][j], ea[u] - next_ea[u]);
+      matrix_drain();
+    }
+#pragma unroll
+    for (int u = 0; u < FM; ++u) ea[u] = next_ea[u];
+    fresh = false;
   };
   auto multiply = [&](int u, int v0) {  // blocks (u, v0) and (u, v0 + 1); the smallest products first
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int v = v0; v < v0 + 2; ++v) t[u & 1][v] = Mac<LOW_F16>::mac(b[0][v], a[u & 1][1], zero4());
+    for (int p = 0; p < 3; ++p)
 #pragma unroll
-    for (int v = v0; v < v0 + 2; ++v) t[u & 1][v] = Mac<LOW_F16>::mac(b[1][v], a[u & 1][0], t[u & 1][v]);
-#pragma unroll
-    for (int v = v0; v < v0 + 2; ++v) t[u & 1][v] = Mac<LOW_F16>::mac(b[0][v], a[u & 1][0], t[u & 1][v]);
+      for (int v = v0; v < v0 + 2; ++v) acc[u][v] = Mac<LOW_F16>::mac(b[p == 1][v], a[u & 1][p == 0], acc[u][v]);
     __builtin_amdgcn_sched_barrier(0);
-  };
-  auto add = [&](int u) {
-#pragma unroll
-    for (int v = 0; v < FN; ++v)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[u][v][j] = __builtin_fmaf(t[u & 1][v][j], unit[u], acc[u][v][j]);
   };
   enter();
   load(0);
@@ -577,7 +591,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   read_a(0, 0);
 #pragma unroll
   for (int v = 0; v < FN; ++v) read_b(0, v);
-  read_units(0);
+  read_exps(0);
   const bool vec = store4_vec<NC_F32>(g) && (g.splits == 1 || g.N % 4 == 0);
   float* const to = g.splits > 1 ? g.part + (int64_t)blockIdx.y * g.M * g.N : reinterpret_cast<float*>(g.out);
   const int64_t ldo = g.splits > 1 ? g.N : g.ldc;
@@ -587,12 +601,12 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   bool left = false;  // RESULTS stores were issued after the loads that the next slice waits for: they stay in flight
   auto slice = [&](auto arrived) {
     const int h = s & 1;
+    rescale();
 #pragma unroll
     for (int u = 0; u + 1 < FM; ++u) {
       read_a(h, u + 1);
 #pragma unroll
       for (int v = 0; v < FN; v += 2) multiply(u, v);
-      if (u > 0) add(u - 1);
       if (u == (FM > 2 ? 1 : 0)) {
         if (left) wait_loads<LB + RESULTS>();  // A's floats are here, asked for before B's slice
         else wait_loads<LB>();
@@ -612,27 +626,26 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
       read_b(h ^ 1, v);
       read_b(h ^ 1, v + 1);
     }
-    if (FM > 1) add(FM - 2);
-    add(FM - 1);
-    read_units(h ^ 1);
+    read_exps(h ^ 1);
     ++s;
   };
   for (int k = 0; k < mine; ++k) {
     for (int n = 1; n < total; ++n) slice([] {});
     int64_t m0, n0;
     tile_at(k, m0, n0);
-    float cb[FN][4], cs[FN][4];  // what the results need, a slice ahead; without a branch (what a branch loads is waited for at its end)
+    float cb[FN][4];  // what the results need, a slice ahead; without a branch (what a branch loads is waited for at its end)
+    int ec[FN][4];
     uint32_t mask[FM][FN];
     int ln = lane;
     asm volatile("" : "+v"(ln));  // computed here: kept, it would take registers that the products need
     const int row = wm + (ln & 15), col = wn + 4 * (ln >> 4);
-    const float* bias = biased ? reinterpret_cast<const float*>(g.bias) : g.col_scale;
+    const float* bias = reinterpret_cast<const float*>(biased ? g.bias : g.exponent);
 #pragma unroll
     for (int v = 0; v < FN; ++v)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = (int)n0 + col + 16 * v + j, n = c < (int)g.N ? c : (int)g.N - 1;
-        cs[v][j] = g.col_scale[n];
+        ec[v][j] = g.exponent[n];
         if (!MASK) cb[v][j] = bias[n];
       }
     if (MASK) {
@@ -652,7 +665,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
 #pragma unroll
       for (int v = 0; v < FN; ++v) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(cs[v][j]));
+        for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(ec[v][j]));
         if (!MASK)
 #pragma unroll
           for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(cb[v][j]));
@@ -661,6 +674,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
           for (int u = 0; u < FM; ++u) asm volatile("" : "+v"(mask[u][v]));
       }
     });
+    matrix_drain();
     if (!MASK && !biased)
 #pragma unroll
       for (int v = 0; v < FN; ++v)
@@ -672,9 +686,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
       for (int v = 0; v < FN; ++v)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // (a cut sum: the mask of each part, no bias)
-          if (MASK) acc[u][v][j] = ((mask[u][v] >> (8 * j)) & 255u) ? acc[u][v][j] * cs[v][j] : 0.f;
-          else acc[u][v][j] = acc[u][v][j] * cs[v][j] + cb[v][j];
+          const float o = __builtin_ldexpf(acc[u][v][j], ea[u] + ec[v][j] - 279);  // 138 + 141
+          acc[u][v][j] = !MASK ? o + cb[v][j] : ((mask[u][v] >> (8 * j)) & 255u) ? o : 0.f;
         }
+    fresh = true;
     left = vec && m0 + BM <= g.M && n0 + BN <= g.N;  // (a tile cut off by the matrix's end stores less)
     int at = lane;
     asm volatile("" : "+v"(at));
