@@ -48,6 +48,7 @@ __device__ __forceinline__ void staged_barrier() {
   wait_loads<0>();
   __syncthreads();
 }
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 // a barrier for LDS alone: __syncthreads() would also wait for every store in flight
 __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -375,33 +376,37 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 
 // ---- float A ------------------------------------------------------------------------------------------
 // The same pipeline over slices of 32 columns, as three products of half planes: x = (x0 + x1) / scale
-// (split2), C = x0 y0 + x0 y1 + x1 y0.  B's scale is a power of two of its row, A's one of its row so far: it puts the
-// first 32 columns' largest below 2^12 and stays until one reaches 2^15, when the row's sums are scaled down with
-// it (seldom after the first slices).  Both are undone in the epilogue.  A value keeps 22 bits, or 2^-36 of the
-// largest before it in its row of A (2^-40 of the largest in its row of B); the product left out is below 2^-22: 2^-20.4 of |x y| at most, about 2^-23 on average.  The sums over slices make up for it: 1.1e-7
-// off the exact result at 200 x 93 x 256 (a plain float product 2.9e-7), 3.0e-7 at 2048 x 1024 x 4096 (1.1e-6).  Six products of
-// exact bfloat16 planes, 2.5e-7 and 5.1e-7 there, are twice the work for matrix cores that are bound by their power:
-// 4096 x 4096 x 4096 740 us, here 430.
+// (split2), C = x0 y0 + x0 y1 + x1 y0.  B's scale is a power of two of its row, A's one of its row so far: it puts
+// the first 32 columns' largest below 2^12 and stays until one reaches 2^15, when the row's sums are scaled
+// down with it (seldom after the first slices).  Both are undone in the epilogue.  A value keeps 22 bits, or 2^-36
+// of the largest before it in its row of A (2^-40 of the largest in its row of B); the product left out is
+// below 2^-22: 2^-20.4 of |x y| at most, about 2^-23 on average.  Off the exact result by 1.9e-7 at 200 x 93 x 256 (a plain
+// float product: 2.9e-7), 3.6e-7 at 2048 x 1024 x 4096 (1.1e-6).  Six products of exact bfloat16 planes, 2.5e-7 and
+// 5.1e-7 there for the longer chain of sums, are twice the work for matrix cores that are bound by their
+// power: 4096 x 4096 x 4096 740 us, here 385.
 // Planes lie in LDS as rows of 64 bytes, 16-byte chunk c of row r at c ^ F((r >> 2) & 3), F = (0, 2, 3, 1):
-// conflict-free for ds_read_b128 (the third weight plane's layout of nc_device.h).  A's floats go into a piece of LDS of their own, where each lane finds the 8
-// columns that it asked for; it splits them and writes the planes.  4 neighbouring lanes hold a group of 32 columns,
-// so the workgroups of the first column tile write the checkpoint's codes in passing.
-// A slice goes block by block of 16 rows: its 3 FN products while the block before is added and the next one's planes
-// are read; the last block's products take turns with the reads of the next slice's B.
+// conflict-free for ds_read_b128 (the third weight plane's layout of nc_device.h).  A's floats go into a piece of
+// LDS of their own, where each lane finds the 8 columns that it asked for; it splits them, writes the planes
+// and asks for those two slices on.  B's planes have room for three slices and are asked for three ahead (two,
+// and A's floats with them half a slice before their use: 409 us).  4 neighbouring lanes hold a group of 32
+// columns, so the workgroups of the first column tile write the checkpoint's codes in passing.
+// A slice goes block by block of 16 rows: its 3 FN products while the next one's planes are read; the last block's
+// products take turns with the reads of the next slice's B.
 // A layer's sums are short (8 slices for 256 inputs), so a workgroup goes through its tiles as one stream of
 // slices: the next tile's first slices are on their way while a tile ends, and its results leave from
 // registers and are not waited for.
 // RELU: of max(A, 0); MASK: the output is masked by codes and has no bias (each would take 16 registers).
-// Measured, M x K x N: 220000 x 256 x 256 159 us with its codes (506 MB: 102 us at a copy's rate; all workgroups store at
-// once, and loads behind stores wait for them), 4096 x 4096 x 4096 430 us = 0.96 PFLOP/s of plane products.
+// Measured, M x K x N: 220000 x 256 x 256 144 us (450 MB: 91 us at a copy's rate; all workgroups store at once, and
+// loads behind stores wait for them), 4096 x 4096 x 4096 385 us = 1.07 PFLOP/s of plane products.
 template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
 __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, int32_t tiles, int32_t nt) {
   constexpr int W = WM * WN, T = 64 * W, FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int APL = BM * 64, BPL = BN * 64, STAGE = 2 * (APL + BPL);
+  constexpr int APL = BM * 64, BPL = BN * 64;      // bytes of a plane's slice
+  constexpr int B0 = 4 * APL;                      // two slices of A's planes, then three of B's
   constexpr int XA = BM * 4 / T;                   // chunks of A a thread
   constexpr int LA = XA * (VEC ? 2 : 8);           // loads of A a wave
   constexpr int LB = 2 * BPL / 1024 / W;           // 1-KB loads of B a wave
-  constexpr int RAW = 2 * STAGE, EXPS = RAW + W * XA * 2048;  // A's floats, then its exponents [2][BM]
+  constexpr int RAW = B0 + 6 * BPL, EXPS = RAW + W * XA * 2048;  // A's floats, then its exponents [2][BM]
   static_assert(BM * 4 % T == 0 && 2 * BPL % (1024 * W) == 0, "whole chunks a thread, whole loads a wave");
   static_assert(FM % 2 == 0 && FN % 2 == 0, "pairs");
   extern __shared__ __attribute__((aligned(256))) unsigned char lds[];
@@ -421,31 +426,24 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
     n0 = (int64_t)(t - tm * (uint32_t)nt) * BN;
   };
 
-  // what is loaded next: tile lk, slice lt
-  int lk = 0, lt = 0;
-  int64_t lm0 = 0, ln0 = 0;
+  // what is loaded next, tile and slice: A's floats run two slices ahead, B's planes three
+  int ak = 0, as = 0, bk = 0, bs = 0;
+  int64_t am0 = 0, an0 = 0;
   uint32_t oa[XA], ob[LB];
   const uint8_t* a_next = nullptr;
   const uint8_t* b_next = nullptr;
-  auto enter = [&]() {
-    tile_at(lk, lm0, ln0);
+  auto enter_a = [&]() {
+    tile_at(ak, am0, an0);
 #pragma unroll
     for (int l = 0; l < XA; ++l) {
       const int r = (l * T + (int)threadIdx.x) >> 2;
-      const int64_t rr = lm0 + r < g.M ? r : g.M - 1 - lm0;  // rows behind the last: its copies, not stored
+      const int64_t rr = am0 + r < g.M ? r : g.M - 1 - am0;  // rows behind the last: its copies, not stored
       oa[l] = (uint32_t)(rr * g.lda);
     }
-#pragma unroll
-    for (int j = 0; j < LB; ++j) {
-      const int at = (wave * LB + j) * 16 + (lane >> 2), r = at % BN;  // a row of a plane
-      const int64_t rr = ln0 + r < g.N ? r : g.N - 1 - ln0;
-      ob[j] = (uint32_t)(rr * g.ldb) + hchunk3(r, lane & 3);
-    }
-    a_next = g.A + lm0 * g.lda;
-    b_next = g.B + ln0 * g.ldb + (int64_t)first * 64;
-    if (g.codes && ln0 == 0 && first == 0) {
+    a_next = g.A + am0 * g.lda;
+    if (g.codes && an0 == 0 && first == 0) {
       for (int e = threadIdx.x; e < BM * pads; e += T) {
-        const int64_t m = lm0 + e / pads, gr = g.slices + e % pads;
+        const int64_t m = am0 + e / pads, gr = g.slices + e % pads;
         if (m >= g.M) break;
         uint4* c = reinterpret_cast<uint4*>(g.codes + m * g.code_stride + gr * CODE_GROUP);
         c[0] = c[1] = uint4{0u, 0u, 0u, 0u};
@@ -453,16 +451,27 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
       }
     }
   };
+  auto enter_b = [&]() {
+    int64_t m0, n0;
+    tile_at(bk, m0, n0);
+#pragma unroll
+    for (int j = 0; j < LB; ++j) {
+      const int at = (wave * LB + j) * 16 + (lane >> 2), r = at % BN;  // a row of a plane
+      const int64_t rr = n0 + r < g.N ? r : g.N - 1 - n0;
+      ob[j] = (uint32_t)(rr * g.ldb) + hchunk3(r, lane & 3);
+    }
+    b_next = g.B + n0 * g.ldb + (int64_t)first * 64;
+  };
   // what the floats in LDS are: tile and slice, and whether their codes are written
   int64_t xm0 = 0;
   int xt = 0;
   bool xcode = false, xnew = false;  // xnew: a tile's first slice
   int xe[XA];                        // the exponents that the rows' scales are made of
-  auto load = [&](int half) {
-    xnew = lt == 0;
-    xm0 = lm0;
-    xt = first + lt;
-    xcode = g.codes && ln0 == 0;
+  auto load_a = [&]() {
+    xnew = as == 0;
+    xm0 = am0;
+    xt = first + as;
+    xcode = g.codes && an0 == 0;
     const uint32_t to = lds0 + RAW + wave * (XA * 2048);
 #pragma unroll
     for (int l = 0; l < XA; ++l) {
@@ -477,19 +486,25 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
           load_lds4(a_next, oa[l] + 4 * (uint32_t)(c + e < k ? c + e : k - 1), to + l * 2048 + e * 256);
       }
     }
+    if (++as == total) {
+      as = 0;
+      if (++ak < mine) enter_a();
+    }
+  };
+  auto load_b = [&](int third) {
 #pragma unroll
     for (int j = 0; j < LB; ++j) {
       const int pl = (wave * LB + j) * 16 / BN;
-      load_lds16(b_next + pl * g.plane_b, ob[j], lds0 + half * STAGE + 2 * APL + (wave * LB + j) * 1024);
+      load_lds16(b_next + pl * g.plane_b, ob[j], lds0 + B0 + third * (2 * BPL) + (wave * LB + j) * 1024);
     }
     b_next += 64;
-    if (++lt == total) {
-      lt = 0;
-      if (++lk < mine) enter();
+    if (++bs == total) {
+      bs = 0;
+      if (++bk < mine) enter_b();
     }
   };
   auto store_a = [&](int half) {
-    unsigned char* s = lds + half * STAGE;
+    unsigned char* s = lds + half * (2 * APL);
 #pragma unroll
     for (int l = 0; l < XA; ++l) {
       const int at = l * T + threadIdx.x, r = at >> 2, c = at & 3;
@@ -539,17 +554,17 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
     for (int v = 0; v < FN; ++v) acc[u][v] = zero4();
   const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
   const unsigned char* fa = lds + (wm + i) * 64 + hchunk3(i, q);  // wm, wn and 16 u leave the chunk order as it is
-  const unsigned char* fb = lds + 2 * APL + (wn + i) * 64 + hchunk3(i, q);
+  const unsigned char* fb = lds + B0 + (wn + i) * 64 + hchunk3(i, q);
   uint4 a[2][2], b[2][FN];  // a[block & 1][plane], b[plane][block]
   int ea[FM], next_ea[FM];  // exponents of the sums, of the next slice's rows
   bool fresh = true;        // the sums are zero
   auto read_a = [&](int half, int u) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) a[u & 1][p] = *reinterpret_cast<const uint4*>(fa + half * STAGE + p * APL + 16 * u * 64);
+    for (int p = 0; p < 2; ++p) a[u & 1][p] = *reinterpret_cast<const uint4*>(fa + half * (2 * APL) + p * APL + 16 * u * 64);
   };
-  auto read_b = [&](int half, int v) {
+  auto read_b = [&](int third, int v) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) b[p][v] = *reinterpret_cast<const uint4*>(fb + half * STAGE + p * BPL + 16 * v * 64);
+    for (int p = 0; p < 2; ++p) b[p][v] = *reinterpret_cast<const uint4*>(fb + third * (2 * BPL) + p * BPL + 16 * v * 64);
   };
   auto read_exps = [&](int half) {
 #pragma unroll
@@ -581,13 +596,21 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
       for (int v = v0; v < v0 + 2; ++v) acc[u][v] = Mac<LOW_F16>::mac(b[p == 1][v], a[u & 1][p == 0], acc[u][v]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  enter();
-  load(0);
-  wait_loads<0>();
+  enter_a();
+  enter_b();
+  load_a();
+  load_b(0);
+  if (steps > 1) {
+    load_b(1);
+    wait_loads<LB>();
+  } else {
+    wait_loads<0>();
+  }
   store_a(0);
-  lds_barrier();  // (a wave's floats are read before the wave asks for the next ones)
-  if (steps > 1) load(1);
-  staged_barrier();
+  wait_lds();
+  if (steps > 1) load_a();
+  if (steps > 2) load_b(2);
+  lds_barrier();
   read_a(0, 0);
 #pragma unroll
   for (int v = 0; v < FN; ++v) read_b(0, v);
@@ -599,8 +622,9 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   constexpr int RESULTS = FM * FN;  // stores of a whole tile's results
   int s = 0;
   bool left = false;  // RESULTS stores were issued after the loads that the next slice waits for: they stay in flight
+  int third = 0;  // of B, where this slice's was
   auto slice = [&](auto arrived) {
-    const int h = s & 1;
+    const int h = s & 1, next = third == 2 ? 0 : third + 1;
     rescale();
 #pragma unroll
     for (int u = 0; u + 1 < FM; ++u) {
@@ -608,25 +632,29 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
 #pragma unroll
       for (int v = 0; v < FN; v += 2) multiply(u, v);
       if (u == (FM > 2 ? 1 : 0)) {
-        if (left) wait_loads<LB + RESULTS>();  // A's floats are here, asked for before B's slice
+        // the next slice's floats, and with them its B, which was asked for before; behind them only the B after
+        // next and a tile's results are in flight
+        if (s + 2 >= steps) wait_loads<0>();
+        else if (left) wait_loads<LB + RESULTS>();
         else wait_loads<LB>();
+        left = false;
         store_a(h ^ 1);
+        arrived();
+        wait_lds();  // the floats are read: the next ones may come
+        if (s + 2 < steps) load_a();
       }
     }
-    if (left) wait_loads<RESULTS>();
-    else wait_loads<0>();
     lds_barrier();
-    left = false;
-    arrived();
-    if (s + 2 < steps) load(h);
+    if (s + 3 < steps) load_b(third);
     read_a(h ^ 1, 0);
 #pragma unroll
     for (int v = 0; v < FN; v += 2) {
       multiply(FM - 1, v);
-      read_b(h ^ 1, v);
-      read_b(h ^ 1, v + 1);
+      read_b(next, v);
+      read_b(next, v + 1);
     }
     read_exps(h ^ 1);
+    third = next;
     ++s;
   };
   for (int k = 0; k < mine; ++k) {
@@ -763,7 +791,7 @@ static int run_low_gemm(const LowGemm& g, hipStream_t s) {
 template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
 static int run_low_gemm_f(const LowGemm& g, hipStream_t s) {
   const int64_t mt = (g.M + BM - 1) / BM, nt = (g.N + BN - 1) / BN, tiles = mt * nt;
-  constexpr int lds = 2 * 128 * (BM + BN) + 128 * BM + 8 * BM, per_cu = 163840 / lds;  // resident workgroups
+  constexpr int lds = 256 * BM + 384 * BN + 128 * BM + 8 * BM, per_cu = 163840 / lds;  // resident workgroups
   auto kernel = k_low_gemm_f<BM, BN, WM, WN, VEC, RELU, MASK>;
   static std::atomic<uint64_t> done{0};
   if (const int e = allow_lds(kernel, lds, done)) return e;

@@ -8,10 +8,9 @@ scale product, their product, bias) and the output's.  The layer's products: a m
 instruction adds 32 products to a float32 sum; its error is taken as 2 roundings of the
 running sum (1.9 measured) for each of the n / 32 instructions, and one for each of its 32
 products; a float32 product is 6 (weight gradient 3) such sums of planes and leaves out 2^-25.
-The float32 products of y and dx (half planes, three products and one scaled addition for each 32
-columns) are inside that bound: 3 x 2 roundings of a slice's own sum, one of the running sum for each slice, a
-representation of 2^-22 on either side and a product of 2^-22 left out, (n / 32 + 6 + 12 + 2) u in all against
-(12 n / 32 + 40) u.
+The float32 products of y and dx (half planes: three products for each 32 columns, n / 32 x 3 x 2 roundings of
+the running sum; a representation of 2^-22 on either side and a product of 2^-22 left out; products of 11-bit
+numbers are exact) are inside that bound: (6 n / 32 + 12 + 4) u against (12 n / 32 + 40) u.
 """
 import ctypes
 import math
