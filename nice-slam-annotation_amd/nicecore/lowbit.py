@@ -308,8 +308,9 @@ def checkpointed_linear(x, weight, bias=None, relu=False):
     Instead of the input its backward keeps the 8-bit checkpoint of ``a`` (pack_activations: 1.03
     bytes a channel):  dx = (dy W) [x > 0 if relu]  and  db  are those of the full layer, dW = dy^T a8
     sees the checkpoint's values.  All tensors have one dtype; sums are held in float32.  A float32
-    product keeps 22 bits of each value (or 2^-36 of the largest in its row: far smaller ones lose bits) and is as near to the exact result as a plain float32 product; an infinity in x or dy makes
-    NaN of its row.  A chain of such layers trains an MLP.  Has no second derivative."""
+    product keeps 22 bits of a value down to 2^-14 of the largest in its row of x, dy or W (fewer below: its
+    floor is 2^-36 of that) and is then as near to the exact result as a plain float32 product; an infinity
+    in x or dy makes NaN of its row.  A chain of such layers trains an MLP.  Has no second derivative."""
     if not torch.is_grad_enabled():  # no backward, no checkpoint (a Function sees the inputs' own requires_grad)
         x, weight, bias = (t.detach() if isinstance(t, torch.Tensor) else t for t in (x, weight, bias))
     return _CheckpointedLinear.apply(x, weight, bias, bool(relu))

@@ -562,3 +562,38 @@ def test_quantized_linear_tiles(m, k, n):
     want = acc * q.scales.double().cpu()[:, None] * w8.scales.double().cpu()
     check(got, want, 4 * U * want.abs())
     assert torch.equal(lb().quantized_linear(q, w8), lb().quantized_linear(x, w8))
+
+
+@pytest.mark.parametrize("shape", ["grows", "shrinks", "zeros first", "one spike", "rows apart"])
+@pytest.mark.parametrize("m,k,n", [(70, 700, 130), (300, 1024, 257), (2000, 96, 300), (40, 4096, 256)])
+def test_layer_float32_scales_within_rows(m, k, n, shape):
+    """The power of two that a row's values are split by follows the row: a value is off by at most 2^-22 of itself or
+    2^-36 of the largest in its row (of W 2^-40), beside the bound of the sums."""
+    g = gen(k + n)
+    x, w = torch.randn(m, k, generator=g), torch.randn(n, k, generator=g)
+    dy = torch.randn(m, n, generator=g)
+    if shape == "grows":
+        x = x * torch.exp2(torch.linspace(-30, 30, k))
+        dy = dy * torch.exp2(torch.linspace(-30, 30, n))
+    elif shape == "shrinks":
+        x = x * torch.exp2(torch.linspace(30, -30, k))
+        dy = dy * torch.exp2(torch.linspace(30, -30, n))
+    elif shape == "zeros first":
+        x[:, :k // 2] = 0.0
+        dy[:, :n // 2] = 0.0
+    elif shape == "one spike":
+        x[torch.arange(m), torch.randint(k, (m,), generator=g)] = 3e4
+        dy[torch.arange(m), torch.randint(n, (m,), generator=g)] = -2e5
+        w[torch.arange(n), torch.randint(k, (n,), generator=g)] = 1e3
+    else:
+        x, dy = x * torch.exp2(torch.linspace(-60, 40, m))[:, None], dy * torch.exp2(torch.linspace(40, -60, m))[:, None]
+        w = w * torch.exp2(torch.linspace(-12, 12, n))[:, None]
+    y, dx, _ = layer_run(x, w, None, dy, False)
+
+    def bound(a, b):  # of a b^T
+        a, b = a.double().abs(), b.double().abs()
+        small = 2.0 ** -36 * a.amax(1, keepdim=True) * b.sum(1) + 2.0 ** -40 * a.sum(1, keepdim=True) * b.amax(1)
+        return sum_tol(a @ b.t(), a.shape[1], 6) + small
+
+    check(y, x.double() @ w.double().t(), bound(x, w))
+    check(dx, dy.double() @ w.double(), bound(dy, w.t()))
