@@ -1706,8 +1706,8 @@ int nc_imap_points_backward(const nc_imap_points_args* a, void* ws, size_t ws_by
 
 // ---------------------------------------------------------------------------
 // 8-bit layer operators (ABI v12, nc_lowbit.h): [encode] -> k_low_gemm; the layer's forward
-// is encode (codes + the 16-bit copy or planes of the input) -> k_low_gemm, its backward
-// encode (dY's copy or planes) -> transpose (W) -> k_low_gemm (dX) -> k_low_wgrad -> sums.
+// is encode (codes + the 16-bit copy of the input; float: W's planes) -> k_low_gemm, its backward
+// encode (dY's 16-bit copy) -> transpose (W) -> k_low_gemm (dX) -> [decode] k_low_wgrad -> sums.
 // ---------------------------------------------------------------------------
 namespace {
 

@@ -33,7 +33,7 @@ constexpr int ROW_ALIGN = 64;    // padded 16-bit rows: elements (128 bytes)
 
 __host__ __device__ inline int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// ---- elementwise: codes, padded 16-bit copies, three-plane splits, transposes, sums --------------
+// ---- elementwise: codes, padded 16-bit copies, float planes, transposes, sums ----------------------
 struct CodeCtx {
   int32_t dtype, format;   // nc_dtype of x / values, nc_code_format (-1: no codes)
   int64_t rows, cols;
@@ -45,7 +45,7 @@ struct CodeCtx {
   void* values;            // decode: [rows][x_stride]
   int64_t zero_rows;       // decode: rows of zeros behind them
   // encode of the layer's input: what the matrix kernel reads besides
-  int32_t relu;            // max(x, 0) in the 16-bit copy / planes
+  int32_t relu;            // max(x, 0) in the 16-bit copy
   uint16_t* copy;          // 16-bit x: [rows][copy_stride]
   int64_t copy_stride;     // elements, a multiple of 64
 };
@@ -78,7 +78,7 @@ struct TransposeCtx {
 };
 int launch_transpose(const TransposeCtx& c, hipStream_t s);
 
-// ---- C[m][n] = sum over plane pairs of A_p[m][:] . B_p[n][:] (both row-major along the sum) --------
+// ---- C[m][n] = sum_k A[m][k] B[n][k] (both row-major along the sum) --------------------------------
 struct LowGemm {
   const uint8_t* A;        // rows of lda bytes: int8 codes or 16-bit elements, 128-byte slices
   const uint8_t* B;
