@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(256) k_low_finish(const LowGemm g, int64_t qua
 // Measured, M x K x N: int8 16384 x 4096 x 4096 232 us = 2.37 POP/s (a library's int8 product on this card: 2.47), bfloat16
 // 8192 x 4096 x 4096 205 us = 1.34 PFLOP/s (1.57).  The matrix cores are busy 55 - 62 % of the cycles at the 2.0 - 2.2
 // GHz that their power leaves.  4 waves of 128 x 128 read a third less from LDS, but a wave alone on its SIMD waits
-// for every read: int8 392 us.
+// for every read: int8 392 us.  Half slices (64 bytes of a row) five deep: 255 us; memory prefers whole lines.
 template <int MODE, int DT, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int64_t mt, int64_t nt) {
   constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
