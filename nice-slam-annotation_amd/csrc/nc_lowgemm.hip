@@ -386,18 +386,18 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 // power: 4096 x 4096 x 4096 740 us, here 385.
 // Planes lie in LDS as rows of 64 bytes, 16-byte chunk c of row r at c ^ F((r >> 2) & 3), F = (0, 2, 3, 1):
 // conflict-free for ds_read_b128 (the third weight plane's layout of nc_device.h).  A's floats go into a piece of
-// LDS of their own, where each lane finds the 8 columns that it asked for; it splits them, writes the planes
-// and asks for those two slices on.  B's planes have room for three slices and are asked for three ahead (two,
-// and A's floats with them half a slice before their use: 409 us).  4 neighbouring lanes hold a group of 32
-// columns, so the workgroups of the first column tile write the checkpoint's codes in passing.
+// LDS of their own, where each lane finds the 8 columns that it asked for; it reads them, asks for those two
+// slices on, splits them and writes the planes.  B's planes have room for three slices and are asked for three
+// ahead (two, and A's floats with them half a slice before their use: 409 us).  4 neighbouring lanes hold a
+// group of 32 columns, so the workgroups of the first column tile write the checkpoint's codes in passing.
 // A slice goes block by block of 16 rows: its 3 FN products while the next one's planes are read; the last block's
 // products take turns with the reads of the next slice's B.
 // A layer's sums are short (8 slices for 256 inputs), so a workgroup goes through its tiles as one stream of
 // slices: the next tile's first slices are on their way while a tile ends, and its results leave from
 // registers and are not waited for.
 // RELU: of max(A, 0); MASK: the output is masked by codes and has no bias (each would take 16 registers).
-// Measured, M x K x N: 220000 x 256 x 256 144 us (450 MB: 91 us at a copy's rate; all workgroups store at once, and
-// loads behind stores wait for them), 4096 x 4096 x 4096 385 us = 1.07 PFLOP/s of plane products.
+// Measured, M x K x N: 220000 x 256 x 256 141 us (450 MB: 91 us at a copy's rate; all workgroups store at once, and
+// loads behind stores wait for them), 4096 x 4096 x 4096 385 - 400 us = 1.05 PFLOP/s of plane products.
 template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
 __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, int32_t tiles, int32_t nt) {
   constexpr int W = WM * WN, T = 64 * W, FM = BM / WM / 16, FN = BN / WN / 16;
@@ -503,12 +503,11 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
       if (++bk < mine) enter_b();
     }
   };
-  auto store_a = [&](int half) {
-    unsigned char* s = lds + half * (2 * APL);
+  float xs[XA][8];
+  auto fetch_a = [&]() {
 #pragma unroll
     for (int l = 0; l < XA; ++l) {
-      const int at = l * T + threadIdx.x, r = at >> 2, c = at & 3;
-      float x[8];
+      float(&x)[8] = xs[l];
       if (VEC) {
         const float4 lo = *reinterpret_cast<const float4*>(raw + l * 2048 + 16 * lane);
         const float4 hi = *reinterpret_cast<const float4*>(raw + l * 2048 + 1024 + 16 * lane);
@@ -518,17 +517,32 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const float*>(raw + l * 2048 + e * 256 + 4 * lane);
       }
-      if ((xt + 1) * 32 > (int)g.K) clear8<VEC>((int64_t)xt * 4 + c, g.K, x);
+    }
+  };
+  // more: the floats after next are asked for as soon as these are read
+  auto store_a = [&](int half, bool more) {
+    unsigned char* s = lds + half * (2 * APL);
+    wait_lds();
+    const int64_t m0 = xm0;
+    const int t = xt;
+    const bool code = xcode, fresh_row = xnew;
+    xcode = false;  // a step behind the last one stores the same planes again, which nobody reads
+    if (more) load_a();
+#pragma unroll
+    for (int l = 0; l < XA; ++l) {
+      const int at = l * T + threadIdx.x, r = at >> 2, c = at & 3;
+      float(&x)[8] = xs[l];
+      if ((t + 1) * 32 > (int)g.K) clear8<VEC>((int64_t)t * 4 + c, g.K, x);
       if (RELU)
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = relu_keep_nan(x[e]);
-      if (xcode) {
+      if (code) {
         int sb;
         const uint2 w = group_codes<RELU>(x, sb);
-        if (xm0 + r < g.M) {
-          *reinterpret_cast<uint2*>(g.codes + xm0 * g.code_stride + (uint32_t)(r * (int)g.code_stride + 32 * xt + 8 * c)) = w;
+        if (m0 + r < g.M) {
+          *reinterpret_cast<uint2*>(g.codes + m0 * g.code_stride + (uint32_t)(r * (int)g.code_stride + 32 * t + 8 * c)) = w;
           const int sr = (int)(g.code_stride / CODE_GROUP);
-          if (c == 0) (g.steps + xm0 * sr)[(uint32_t)(r * sr + xt)] = (uint8_t)sb;
+          if (c == 0) (g.steps + m0 * sr)[(uint32_t)(r * sr + t)] = (uint8_t)sb;
         }
       }
       float top = 0.f;  // (NaN counts as nothing: it is one in the planes)
@@ -538,14 +552,13 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
       bits = max(bits, (uint32_t)__builtin_amdgcn_mov_dpp((int)bits, 0xb1, 0xf, 0xf, true));  // lane ^ 1
       bits = max(bits, (uint32_t)__builtin_amdgcn_mov_dpp((int)bits, 0x4e, 0xf, 0xf, true));  // lane ^ 2
       const int e = top_exponent(bits);
-      xe[l] = xnew || e > xe[l] + 3 ? e : xe[l];
+      xe[l] = fresh_row || e > xe[l] + 3 ? e : xe[l];
       if (c == 0) exps[half * BM + r] = xe[l];
       uint4 p[2];
       split2(x, scale_to(138, xe[l]), p);
 #pragma unroll
       for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(s + k * APL + r * 64 + hchunk3(r, c)) = p[k];
     }
-    xcode = false;  // a step behind the last one stores the same again, which nobody reads
   };
   floatx4 acc[FM][FN];
 #pragma unroll
@@ -606,9 +619,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   } else {
     wait_loads<0>();
   }
-  store_a(0);
-  wait_lds();
-  if (steps > 1) load_a();
+  fetch_a();
+  store_a(0, steps > 1);
   if (steps > 2) load_b(2);
   lds_barrier();
   read_a(0, 0);
@@ -629,19 +641,21 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
 #pragma unroll
     for (int u = 0; u + 1 < FM; ++u) {
       read_a(h, u + 1);
-#pragma unroll
-      for (int v = 0; v < FN; v += 2) multiply(u, v);
-      if (u == (FM > 2 ? 1 : 0)) {
+      const bool split = u == (FM > 2 ? 1 : 0);
+      if (split) {
         // the next slice's floats, and with them its B, which was asked for before; behind them only the B after
         // next and a tile's results are in flight
         if (s + 2 >= steps) wait_loads<0>();
         else if (left) wait_loads<LB + RESULTS>();
         else wait_loads<LB>();
         left = false;
-        store_a(h ^ 1);
+        fetch_a();
+      }
+#pragma unroll
+      for (int v = 0; v < FN; v += 2) multiply(u, v);
+      if (split) {
         arrived();
-        wait_lds();  // the floats are read: the next ones may come
-        if (s + 2 < steps) load_a();
+        store_a(h ^ 1, s + 2 < steps);
       }
     }
     lds_barrier();
