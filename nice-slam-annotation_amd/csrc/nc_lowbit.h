@@ -218,27 +218,56 @@ __device__ __forceinline__ int step_byte(uint32_t amax, bool relu) {
   return amax >= 0x7f800000u ? 255 : max(e, 1);
 }
 
-// 8 columns [8 c, 8 c + 8) of a row as float; those behind the last are copies of others (clear8 zeroes them).
-// No branch: what a branch loads is waited for where its sides meet.  VEC: 16-byte aligned rows of a
-// multiple of 8 columns.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const void* x, int64_t off, int64_t c, int64_t cols, float (&v)[8]) {
-  if (VEC) {
-    const int64_t last = cols / 8 - 1, at = off + 8 * (c < last ? c : last);
-    if (DT == NC_F32) {
-      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + at);
-      const float4 a = p[0], b = p[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + at);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// 16 (8) bytes at any element's address: one instruction, whose address need not be a multiple of its size
+template <typename T>
+__device__ __forceinline__ T load_any(const void* p) {
+  T v;
+  __builtin_memcpy(&v, p, sizeof(T));
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store_any(void* p, T v) {
+  __builtin_memcpy(p, &v, sizeof(T));
+}
+// v[j] = v[j + s], 0 <= s < 8, for the values that are there
+template <int BIT>
+__device__ __forceinline__ void shift_by(float (&v)[8], bool on) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = elem_f32<DT>((uint16_t)w[j]);
-        v[2 * j + 1] = elem_f32<DT>((uint16_t)(w[j] >> 16));
-      }
+  for (int j = 0; j < 8 - BIT; ++j) {
+    const float there = v[j + BIT], here = v[j];  // (values: a choice of places would put the array into memory)
+    v[j] = on ? there : here;
+  }
+}
+__device__ __forceinline__ void shift8(float (&v)[8], int s) {
+  shift_by<4>(v, (s & 4) != 0);
+  shift_by<2>(v, (s & 2) != 0);
+  shift_by<1>(v, (s & 1) != 0);
+}
+
+// 8 columns [8 c, 8 c + 8) of a row as float, from any address; clear8 puts zeros for those behind the last.  WIDE:
+// rows of at least 8 columns, whose last chunk is loaded as the row's last 8 and moved to its place by clear8, away
+// from the loads (what waits for a load keeps the next one from being asked for).
+template <int DT>
+__device__ __forceinline__ void load8_at(const void* x, int64_t at, float (&v)[8]) {
+  if (DT == NC_F32) {
+    const float* p = reinterpret_cast<const float*>(x) + at;
+    const float4 a = load_any<float4>(p), b = load_any<float4>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 a = load_any<uint4>(reinterpret_cast<const uint16_t*>(x) + at);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = elem_f32<DT>((uint16_t)w[j]);
+      v[2 * j + 1] = elem_f32<DT>((uint16_t)(w[j] >> 16));
     }
+  }
+}
+template <int DT, bool WIDE>
+__device__ __forceinline__ void load8(const void* x, int64_t off, int64_t c, int64_t cols, float (&v)[8]) {
+  if (WIDE) {
+    load8_at<DT>(x, off + (8 * c < cols - 8 ? 8 * c : cols - 8), v);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -247,14 +276,18 @@ __device__ __forceinline__ void load8(const void* x, int64_t off, int64_t c, int
     }
   }
 }
-template <bool VEC>
+template <bool WIDE>
 __device__ __forceinline__ void clear8(int64_t c, int64_t cols, float (&v)[8]) {
+  if (WIDE && cols % 8 == 0) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (VEC ? 8 * c : 8 * c + j) < cols ? v[j] : 0.f;
+    for (int j = 0; j < 8; ++j) v[j] = 8 * c < cols ? v[j] : 0.f;
+  } else {
+    if (WIDE) shift8(v, 8 * c > cols - 8 ? (int)(8 * c - cols) & 7 : 0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 8 * c + j < cols ? v[j] : 0.f;
+  }
 }
-inline bool load8_vec(const void* p, int64_t stride, int64_t cols, int dtype) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * (dtype == NC_F32 ? 4 : 2)) % 16 == 0 && cols % 8 == 0;
-}
+inline bool wide8(int64_t cols) { return cols >= 8; }
 
 // the low bytes of 8 words
 __device__ __forceinline__ uint2 pack8(const uint32_t (&q)[8]) {

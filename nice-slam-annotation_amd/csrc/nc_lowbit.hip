@@ -12,13 +12,13 @@ namespace nc {
 
 static inline unsigned blocks_of(int64_t n, int b) { return (unsigned)((n + b - 1) / b); }
 
-template <int DT, bool VEC>
+template <int DT>
 __device__ __forceinline__ void store8(void* x, int64_t off, int64_t c, int64_t cols, const float (&v)[8]) {
   if (DT == NC_F32) {
     float* p = reinterpret_cast<float*>(x) + off + 8 * c;
-    if (VEC && 8 * c + 8 <= cols) {
-      reinterpret_cast<float4*>(p)[0] = float4{v[0], v[1], v[2], v[3]};
-      reinterpret_cast<float4*>(p)[1] = float4{v[4], v[5], v[6], v[7]};
+    if (8 * c + 8 <= cols) {
+      store_any(p, float4{v[0], v[1], v[2], v[3]});
+      store_any(p + 4, float4{v[4], v[5], v[6], v[7]});
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -29,13 +29,9 @@ __device__ __forceinline__ void store8(void* x, int64_t off, int64_t c, int64_t 
     uint16_t e[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) e[j] = f32_elem<DT>(v[j]);
-    if (VEC && 8 * c + 8 <= cols) {
-      uint4 a;
-      a.x = e[0] | (uint32_t)e[1] << 16;
-      a.y = e[2] | (uint32_t)e[3] << 16;
-      a.z = e[4] | (uint32_t)e[5] << 16;
-      a.w = e[6] | (uint32_t)e[7] << 16;
-      *reinterpret_cast<uint4*>(p) = a;
+    if (8 * c + 8 <= cols) {
+      store_any(p, uint4{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                         e[6] | (uint32_t)e[7] << 16});
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -160,17 +156,17 @@ __global__ void __launch_bounds__(256) k_encode_groups(const CodeCtx a, int64_t 
       if ((c & 3) == 0) reinterpret_cast<uint8_t*>(a.scales)[r * (a.code_stride / CODE_GROUP) + (c >> 2)] = (uint8_t)sb;
     }
   }
-  if (COPY && 8 * c < a.copy_stride) store8<DT, true>(a.copy, r * a.copy_stride, c, a.copy_stride, v);  // exact: v is of that type
+  if (COPY && 8 * c < a.copy_stride) store8<DT>(a.copy, r * a.copy_stride, c, a.copy_stride, v);  // exact: v is of that type
 }
 
-template <int DT, bool VEC>
+template <int DT>
 __global__ void __launch_bounds__(256) k_decode(const CodeCtx a, int64_t row_chunks, int64_t total) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= total) return;
   const int64_t r = id / row_chunks, c = id - r * row_chunks;
   if (r >= a.rows) {
     const float zero[8] = {};
-    store8<DT, VEC>(a.values, r * a.x_stride, c, a.cols, zero);
+    store8<DT>(a.values, r * a.x_stride, c, a.cols, zero);
     return;
   }
   const uint2 w = *reinterpret_cast<const uint2*>(a.codes + r * a.code_stride + 8 * c);
@@ -188,7 +184,7 @@ __global__ void __launch_bounds__(256) k_decode(const CodeCtx a, int64_t row_chu
     const int q = a.format == NC_CODES_RELU ? (b > 0 ? (int)b - 1 : 0) : (int)(int8_t)b;
     v[e] = (float)q * s;
   }
-  store8<DT, VEC>(a.values, r * a.x_stride, c, a.cols, v);
+  store8<DT>(a.values, r * a.x_stride, c, a.cols, v);
 }
 
 // ---- float matrices in two half planes --------------------------------------------------------------------
@@ -242,10 +238,10 @@ __global__ void __launch_bounds__(256) k_tops(const TransposeCtx a) {
 }
 
 // ---- transpose into padded 16-bit rows: 64 x 64 tiles through LDS -------------------------------------
-// A lane loads 16 bytes of its row (VEC; else element by element) and writes them down a column of the tile:
+// A lane loads 16 bytes of its row and writes them down a column of the tile:
 // a wave's 64 lanes are a column's 64 elements, side by side in LDS.  Then 8 lanes write a row of the
 // result, 16 bytes each (float: to each plane).  4096 x 4096 bfloat16 12 us (5.6 TB/s); 31 with 2 bytes a lane.
-template <int DT, bool VEC>
+template <int DT>
 __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
   using E = typename std::conditional<DT == NC_F32, float, uint16_t>::type;
   constexpr int EC = 16 / sizeof(E), CH = 64 / EC / 4;  // elements a chunk, chunks a thread
@@ -258,8 +254,9 @@ __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
     const int64_t c = c0 + EC * (wave + 4 * j);
-    if (VEC) {  // columns behind the last: others, not stored
-      *reinterpret_cast<uint4*>(v[j]) = *reinterpret_cast<const uint4*>(src + (c < a.cols ? c : a.cols - EC));
+    if (c + EC <= a.cols) {  // (a wave's lanes all)
+      const uint4 w = load_any<uint4>(src + c);
+      __builtin_memcpy(v[j], &w, 16);
     } else {
 #pragma unroll
       for (int e = 0; e < EC; ++e) v[j][e] = src[c + e < a.cols ? c + e : a.cols - 1];
@@ -299,41 +296,44 @@ __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
 }
 
 // ---- sums in a fixed order ---------------------------------------------------------------------------
-// V neighbouring elements a thread.  The 128 parts of 220000 x 256 x 256 take 9 us; one load at a time, 25 more.
-template <int DT, int V>
+// 4 neighbouring elements a thread.  The 128 parts of 220000 x 256 x 256 take 9 us; one load at a time, 25 more.
+template <int DT>
 __global__ void __launch_bounds__(256) k_sum_parts(const SumParts a, unsigned first_blocks) {
   const int w = blockIdx.x >= first_blocks ? 1 : 0;
-  const int64_t n = a.n[w], e = ((int64_t)(blockIdx.x - (w ? first_blocks : 0)) * 256 + threadIdx.x) * V;
+  const int64_t n = a.n[w], last = n > 4 ? n - 4 : 0;
+  int64_t e = ((int64_t)(blockIdx.x - (w ? first_blocks : 0)) * 256 + threadIdx.x) * 4;
   if (e >= n) return;
-  typedef float floatv __attribute__((ext_vector_type(V)));
-  floatv t = 0.f;
-  const float* p = a.part[w] + e;
+  const float* p = a.part[w];
+  if (n < 4) {  // the last 4 are written twice where n is no multiple; fewer go one by one
+    for (; e < n; ++e) {
+      float t = 0.f;
+      for (int k = 0; k < a.parts[w]; ++k) t += p[k * n + e];
+      if (DT == NC_F32) reinterpret_cast<float*>(a.out[w])[e] = t;
+      else reinterpret_cast<uint16_t*>(a.out[w])[e] = f32_elem<DT>(t);
+    }
+    return;
+  }
+  e = e < last ? e : last;
+  p += e;
+  floatx4 t = zero4();
   int k = a.parts[w];
   for (; k >= 8; k -= 8, p += 8 * n) {  // 8 loads in flight, added in order
-    floatv v[8];
+    floatx4 v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const floatv*>(p + j * n);
+    for (int j = 0; j < 8; ++j) v[j] = load_any<floatx4>(p + j * n);
 #pragma unroll
     for (int j = 0; j < 8; ++j) t += v[j];
   }
-  for (; k > 0; --k, p += n) t += *reinterpret_cast<const floatv*>(p);
+  for (; k > 0; --k, p += n) t += load_any<floatx4>(p);
   if (DT == NC_F32) {
-    *reinterpret_cast<floatv*>(reinterpret_cast<float*>(a.out[w]) + e) = t;
+    store_any(reinterpret_cast<float*>(a.out[w]) + e, t);
   } else {
-    typedef uint16_t shortv __attribute__((ext_vector_type(V)));
-    shortv o;
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = f32_elem<DT>(t[j]);
-    *reinterpret_cast<shortv*>(reinterpret_cast<uint16_t*>(a.out[w]) + e) = o;
+    const uint16_t o[4] = {f32_elem<DT>(t[0]), f32_elem<DT>(t[1]), f32_elem<DT>(t[2]), f32_elem<DT>(t[3])};
+    store_any(reinterpret_cast<uint16_t*>(a.out[w]) + e, uint2{o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16});
   }
 }
 
 // ---- launchers ---------------------------------------------------------------------------------------
-static bool vec_rows(const void* p, int64_t stride, int dtype) {
-  const int64_t b = dtype == NC_F32 ? 4 : 2;
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * b) % 16 == 0;
-}
-
 template <int DT, bool VEC>
 static int encode_rows(const CodeCtx& c, hipStream_t s) {
   // A wave a row needs no barrier (16384 x 4096 bfloat16: 49 us; 79 us with 1024 threads a row); few rows get
@@ -389,7 +389,7 @@ static int encode(const CodeCtx& c, hipStream_t s) {
 
 int launch_encode(const CodeCtx& c, hipStream_t s) {
   if (c.rows <= 0) return 0;
-  const bool v = load8_vec(c.x, c.x_stride, c.cols, c.dtype);
+  const bool v = wide8(c.cols);
   switch (c.dtype) {
     case NC_F32: return v ? encode<NC_F32, true>(c, s) : encode<NC_F32, false>(c, s);
     case NC_F16: return v ? encode<NC_F16, true>(c, s) : encode<NC_F16, false>(c, s);
@@ -400,22 +400,12 @@ int launch_encode(const CodeCtx& c, hipStream_t s) {
 
 int launch_decode(const CodeCtx& c, hipStream_t s) {
   if (c.rows <= 0) return 0;
-  const bool v = vec_rows(c.values, c.x_stride, c.dtype);
   const int64_t rc = (c.cols + 7) / 8, total = rc * (c.rows + c.zero_rows);
   const dim3 g(blocks_of(total, 256)), b(256);
   switch (c.dtype) {
-    case NC_F32:
-      if (v) hipLaunchKernelGGL((k_decode<NC_F32, true>), g, b, 0, s, c, rc, total);
-      else hipLaunchKernelGGL((k_decode<NC_F32, false>), g, b, 0, s, c, rc, total);
-      break;
-    case NC_F16:
-      if (v) hipLaunchKernelGGL((k_decode<NC_F16, true>), g, b, 0, s, c, rc, total);
-      else hipLaunchKernelGGL((k_decode<NC_F16, false>), g, b, 0, s, c, rc, total);
-      break;
-    case NC_BF16:
-      if (v) hipLaunchKernelGGL((k_decode<NC_BF16, true>), g, b, 0, s, c, rc, total);
-      else hipLaunchKernelGGL((k_decode<NC_BF16, false>), g, b, 0, s, c, rc, total);
-      break;
+    case NC_F32: hipLaunchKernelGGL(k_decode<NC_F32>, g, b, 0, s, c, rc, total); break;
+    case NC_F16: hipLaunchKernelGGL(k_decode<NC_F16>, g, b, 0, s, c, rc, total); break;
+    case NC_BF16: hipLaunchKernelGGL(k_decode<NC_BF16>, g, b, 0, s, c, rc, total); break;
     default: return (int)hipErrorInvalidValue;
   }
   return (int)hipGetLastError();
@@ -423,7 +413,7 @@ int launch_decode(const CodeCtx& c, hipStream_t s) {
 
 int launch_split(const SplitCtx& c, hipStream_t s) {
   if (c.rows <= 0 || c.cols <= 0) return 0;
-  if (load8_vec(c.x, c.x_stride, c.cols, NC_F32)) hipLaunchKernelGGL((k_split<true>), dim3(blocks_of(c.rows, 4)), dim3(256), 0, s, c);
+  if (wide8(c.cols)) hipLaunchKernelGGL((k_split<true>), dim3(blocks_of(c.rows, 4)), dim3(256), 0, s, c);
   else hipLaunchKernelGGL((k_split<false>), dim3(blocks_of(c.rows, 4)), dim3(256), 0, s, c);
   return (int)hipGetLastError();
 }
@@ -432,8 +422,7 @@ template <int DT>
 static int transpose(const TransposeCtx& c, hipStream_t s) {
   if (DT == NC_F32) hipLaunchKernelGGL(k_tops, dim3(blocks_of(c.cols, 64), blocks_of(c.rows, TOP_ROWS)), dim3(256), 0, s, c);
   const dim3 g(blocks_of(c.dst_stride, 64), blocks_of(c.cols, 64));
-  if (load8_vec(c.src, c.src_stride, c.cols, c.dtype)) hipLaunchKernelGGL((k_transpose<DT, true>), g, dim3(256), 0, s, c);
-  else hipLaunchKernelGGL((k_transpose<DT, false>), g, dim3(256), 0, s, c);
+  hipLaunchKernelGGL(k_transpose<DT>, g, dim3(256), 0, s, c);
   return (int)hipGetLastError();
 }
 
@@ -449,17 +438,9 @@ int launch_transpose(const TransposeCtx& c, hipStream_t s) {
 
 template <int DT>
 static int sum_parts(const SumParts& a, hipStream_t s) {
-  int64_t n[2];
-  bool vec = true;
-  for (int w = 0; w < 2; ++w) {
-    n[w] = a.out[w] ? a.n[w] : 0;
-    vec = vec && n[w] % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.out[w]) | reinterpret_cast<uintptr_t>(a.part[w])) & 15) == 0;
-  }
-  const int per = vec ? 1024 : 256;
-  const unsigned first = blocks_of(n[0], per), all = first + blocks_of(n[1], per);
+  const unsigned first = blocks_of(a.out[0] ? a.n[0] : 0, 1024), all = first + blocks_of(a.out[1] ? a.n[1] : 0, 1024);
   if (all == 0) return 0;
-  if (vec) hipLaunchKernelGGL((k_sum_parts<DT, 4>), dim3(all), dim3(256), 0, s, a, first);
-  else hipLaunchKernelGGL((k_sum_parts<DT, 1>), dim3(all), dim3(256), 0, s, a, first);
+  hipLaunchKernelGGL(k_sum_parts<DT>, dim3(all), dim3(256), 0, s, a, first);
   return (int)hipGetLastError();
 }
 

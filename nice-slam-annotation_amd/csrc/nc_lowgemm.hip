@@ -102,13 +102,13 @@ __device__ __forceinline__ float load_bias(const void* b, int dtype, int64_t n) 
   return dtype == NC_BF16 ? elem_f32<NC_BF16>(e) : elem_f32<NC_F16>(e);
 }
 
-// 4 neighbouring outputs [m][n .. n + 3]; vec: rows and columns allow one store
+// 4 neighbouring outputs [m][n .. n + 3], one store where all are there
 template <int DT>
-__device__ __forceinline__ void store4(const LowGemm& g, bool vec, int64_t m, int64_t n, const float (&v)[4]) {
+__device__ __forceinline__ void store4(const LowGemm& g, int64_t m, int64_t n, const float (&v)[4]) {
   if (DT == NC_F32) {
     float* p = reinterpret_cast<float*>(g.out) + m * g.ldc + n;
-    if (vec) {
-      *reinterpret_cast<float4*>(p) = float4{v[0], v[1], v[2], v[3]};
+    if (n + 4 <= g.N) {
+      store_any(p, float4{v[0], v[1], v[2], v[3]});
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -119,8 +119,8 @@ __device__ __forceinline__ void store4(const LowGemm& g, bool vec, int64_t m, in
     uint16_t e[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) e[j] = f32_elem<DT>(v[j]);
-    if (vec) {
-      *reinterpret_cast<uint2*>(p) = uint2{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16};
+    if (n + 4 <= g.N) {
+      store_any(p, uint2{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16});
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -128,12 +128,6 @@ __device__ __forceinline__ void store4(const LowGemm& g, bool vec, int64_t m, in
     }
   }
 }
-template <int DT>
-__device__ __forceinline__ bool store4_vec(const LowGemm& g) {
-  const int b = DT == NC_F32 ? 16 : 8;
-  return g.N % 4 == 0 && g.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(g.out) & (b - 1)) == 0;
-}
-
 // one column's result of a sum
 template <int MODE>
 __device__ __forceinline__ float finish(const LowGemm& g, float x, float scale, float bias, uint32_t code) {
@@ -156,7 +150,6 @@ __device__ __forceinline__ void store_tile(const LowGemm& g, unsigned char* cw, 
   const int i = lane & 15, q = lane >> 4;
   const int64_t n = n0 + 4 * (lane % LPR);
   float* part = g.splits > 1 ? g.part + (int64_t)blockIdx.y * g.M * g.N : nullptr;
-  const bool vec = store4_vec<DT>(g);
   float cs[4], cb[4];
   float rs[MODE == LOW_I8 ? FM : 1][16 / RPI];
   uint32_t mask[FM][16 / RPI];
@@ -191,8 +184,8 @@ __device__ __forceinline__ void store_tile(const LowGemm& g, unsigned char* cw, 
       if (m >= g.M || n >= g.N) continue;
       if (part) {
         float* p = part + m * g.N + n;
-        if (g.N % 4 == 0) {
-          *reinterpret_cast<Acc*>(p) = c;
+        if (n + 4 <= g.N) {
+          store_any(p, c);
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -203,7 +196,7 @@ __device__ __forceinline__ void store_tile(const LowGemm& g, unsigned char* cw, 
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           o[j] = finish<MODE>(g, (float)c[j], MODE == LOW_I8 ? rs[u][k] * cs[j] : 1.f, cb[j], (mask[u][k] >> (8 * j)) & 255u);
-        store4<DT>(g, vec, m, n, o);
+        store4<DT>(g, m, n, o);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -229,10 +222,10 @@ __global__ void __launch_bounds__(256) k_low_finish(const LowGemm g, int64_t qua
   typedef typename M::Acc Acc;
   Acc t = M::zero();
   const float* p = g.part + m * g.N + n;
-  const bool whole = g.N % 4 == 0;
+  const bool whole = n + 4 <= g.N;
   auto part = [&](int k) {
     const typename M::Elem* e = reinterpret_cast<const typename M::Elem*>(p + k * (g.M * g.N));
-    if (whole) return *reinterpret_cast<const Acc*>(e);
+    if (whole) return load_any<Acc>(e);
     Acc v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = e[n + j < g.N ? j : 0];  // columns behind the last: not stored
@@ -249,7 +242,7 @@ __global__ void __launch_bounds__(256) k_low_finish(const LowGemm g, int64_t qua
   for (; k < g.splits; ++k) t += part(k);
 #pragma unroll
   for (int j = 0; j < 4; ++j) o[j] = finish<MODE>(g, (float)t[j], cs[j], cb[j], (mask >> (8 * j)) & 255u);
-  store4<DT>(g, store4_vec<DT>(g), m, n, o);
+  store4<DT>(g, m, n, o);
 }
 
 // BM x BN tile, WM x WN waves, each (BM / WM) x (BN / WN) in blocks of 16 x 16.  The instruction
@@ -477,7 +470,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
     for (int l = 0; l < XA; ++l) {
       const int c = 8 * (4 * xt + (int)(threadIdx.x & 3)), k = (int)g.K;
       if (VEC) {
-        const uint32_t at = oa[l] + 4 * (uint32_t)(c < k ? c : k - 8);  // columns behind the last: others, cleared
+        const uint32_t at = oa[l] + 4 * (uint32_t)(c < k - 8 ? c : k - 8);  // the last chunk: the row's last 8, moved and cleared later
         load_lds16(a_next, at, to + l * 2048);
         load_lds16(a_next, at + 16, to + l * 2048 + 1024);
       } else {
@@ -627,7 +620,6 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
 #pragma unroll
   for (int v = 0; v < FN; ++v) read_b(0, v);
   read_exps(0);
-  const bool vec = store4_vec<NC_F32>(g) && (g.splits == 1 || g.N % 4 == 0);
   float* const to = g.splits > 1 ? g.part + (int64_t)blockIdx.y * g.M * g.N : reinterpret_cast<float*>(g.out);
   const int64_t ldo = g.splits > 1 ? g.N : g.ldc;
   const bool biased = g.bias && g.splits == 1;
@@ -732,7 +724,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
           acc[u][v][j] = !MASK ? o + cb[v][j] : ((mask[u][v] >> (8 * j)) & 255u) ? o : 0.f;
         }
     fresh = true;
-    left = vec && m0 + BM <= g.M && n0 + BN <= g.N;  // (a tile cut off by the matrix's end stores less)
+    left = m0 + BM <= g.M && n0 + BN <= g.N;  // (a tile cut off by the matrix's end stores less)
     int at = lane;
     asm volatile("" : "+v"(at));
     if (left) {  // offsets in a tile fit 32 bits: row strides are at most 2^22
@@ -742,7 +734,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
       for (int u = 0; u < FM; ++u)
 #pragma unroll
         for (int v = 0; v < FN; ++v)
-          *reinterpret_cast<floatx4*>(reinterpret_cast<unsigned char*>(base) + (o + 64u * u * (uint32_t)ldo) + 64 * v) = acc[u][v];
+          store_any(reinterpret_cast<unsigned char*>(base) + (o + 64u * u * (uint32_t)ldo) + 64 * v, acc[u][v]);
     } else {
 #pragma unroll
       for (int u = 0; u < FM; ++u) {
@@ -752,8 +744,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
           const int64_t n = n0 + wn + 16 * v + 4 * (at >> 4);
           if (m >= g.M || n >= g.N) continue;
           float* p = to + m * ldo + n;
-          if (vec) {
-            *reinterpret_cast<floatx4*>(p) = acc[u][v];
+          if (n + 4 <= g.N) {
+            store_any(p, acc[u][v]);
           } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -878,7 +870,7 @@ int launch_low_gemm(const LowGemm& g, hipStream_t s) {
     case LOW_BF16: return pick_low_gemm<LOW_BF16, NC_BF16>(g, s);
     case LOW_F16: return pick_low_gemm<LOW_F16, NC_F16>(g, s);
     case LOW_F32: {
-      const bool vec = load8_vec(g.A, g.lda / 4, g.K, NC_F32);
+      const bool vec = wide8(g.K);
       if (g.mask && (g.a_relu || g.bias || g.relu)) return (int)hipErrorInvalidValue;  // no call has both
       if (vec) return g.mask ? pick_low_gemm_f<true, false, true>(g, s)
                     : g.a_relu ? pick_low_gemm_f<true, true, false>(g, s) : pick_low_gemm_f<true, false, false>(g, s);
@@ -1065,9 +1057,9 @@ __global__ void __launch_bounds__(256) k_low_small(const LowSmall p) {
     float o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = finish<LOW_I8>(g, (float)acc[u][j], scale[r] * cs[j], cb[j], 1u);
-    if (g.out_dtype == NC_F32) store4<NC_F32>(g, store4_vec<NC_F32>(g), m0 + r, n, o);
-    else if (g.out_dtype == NC_F16) store4<NC_F16>(g, store4_vec<NC_F16>(g), m0 + r, n, o);
-    else store4<NC_BF16>(g, store4_vec<NC_BF16>(g), m0 + r, n, o);
+    if (g.out_dtype == NC_F32) store4<NC_F32>(g, m0 + r, n, o);
+    else if (g.out_dtype == NC_F16) store4<NC_F16>(g, m0 + r, n, o);
+    else store4<NC_BF16>(g, m0 + r, n, o);
   }
 }
 
@@ -1097,7 +1089,7 @@ static int encode_low_small(const LowSmall& a, hipStream_t s) {
 
 int launch_low_small(const LowSmall& a, hipStream_t s) {
   if (a.g.M <= 0 || a.g.N <= 0) return 0;
-  const bool vec = a.x_dtype >= 0 && load8_vec(a.x, a.x_stride, a.g.K, a.x_dtype);
+  const bool vec = a.x_dtype >= 0 && wide8(a.g.K);
   switch (a.x_dtype) {
     case NC_F32: return vec ? encode_low_small<NC_F32, true>(a, s) : encode_low_small<NC_F32, false>(a, s);
     case NC_F16: return vec ? encode_low_small<NC_F16, true>(a, s) : encode_low_small<NC_F16, false>(a, s);
@@ -1175,19 +1167,22 @@ template <int DT, int BN, int T, bool VEC>
 __device__ __forceinline__ void col_sums(const LowWgrad& g, int64_t n0, int64_t rb, int64_t re, int64_t piece, float* red) {
   constexpr int C8 = BN / 8, R = T / C8;
   const int64_t c = n0 / 8 + threadIdx.x % C8;
-  const int64_t cols = VEC ? (g.N + 7) / 8 * 8 : g.N;  // 16-bit rows are padded to 64 columns
+  const int64_t cols = DT == NC_F32 ? g.N : (g.N + 7) / 8 * 8;  // 16-bit rows are padded to 64 columns
   float t[8] = {};
   int64_t r = rb + threadIdx.x / C8;
   for (; r + 3 * R < re; r += 4 * R) {
     float v[4][8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load8<DT, VEC>(g.dy, (r + u * R) * g.ldy, c, cols, v[u]);  // (columns behind the last: not stored)
+    for (int u = 0; u < 4; ++u) load8<DT, VEC>(g.dy, (r + u * R) * g.ldy, c, cols, v[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) clear8<VEC>(c, cols, v[u]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] += (v[0][e] + v[1][e]) + (v[2][e] + v[3][e]);
   }
   for (; r < re; r += R) {
     float v[8];
     load8<DT, VEC>(g.dy, r * g.ldy, c, cols, v);
+    clear8<VEC>(c, cols, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] += v[e];
   }
@@ -1239,6 +1234,7 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
 
   float yf[YF > 0 ? YF : 1][8], ysum[8] = {};  // float dY: its columns' sums in passing (T is a multiple of BN / 8)
   const bool summing = YF > 0 && g.want_db && blockIdx.y == 0;
+  const bool ragged = g.N % 8 != 0 && n0 + BN > g.N;  // the last columns: moved to their places
   uint32_t yo[YL > 0 ? YL : 1];  // 16-bit dY: byte offsets from the stage's first row
   int yrow[YL > 0 ? YL : 1];
 #pragma unroll
@@ -1320,6 +1316,7 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
 #pragma unroll
     for (int l = 0; l < YF; ++l) {
       const int at = l * T + threadIdx.x, row = at / (BN / 8), c = at % (BN / 8);
+      if (ragged) clear8<VEC>(n0 / 8 + c, g.N, yf[l]);  // (columns behind the last are not stored)
       const bool in = rb + (int64_t)t * MS + row < re;
       if (!in)
 #pragma unroll
@@ -1459,7 +1456,6 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
   matrix_drain();
   const int i = j16;
   float* part = g.part + (int64_t)blockIdx.z * g.N * g.K;
-  const bool vec = g.K % 4 == 0 && (reinterpret_cast<uintptr_t>(g.dw) & (DT == NC_F32 ? 15 : 7)) == 0;
 #pragma unroll
   for (int u = 0; u < FN; ++u) {
     const int64_t n = n0 + wn + 16 * u + i;
@@ -1470,8 +1466,8 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
       const floatx4 c = acc[u][v];
       if (!g.dw || DT == NC_F32) {
         float* p = (g.dw ? reinterpret_cast<float*>(g.dw) : part) + at;
-        if (vec) {
-          *reinterpret_cast<floatx4*>(p) = c;
+        if (k + 4 <= g.K) {
+          store_any(p, c);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -1482,8 +1478,8 @@ __global__ void __launch_bounds__(64 * WN * WK) __attribute__((amdgpu_waves_per_
         uint16_t o[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = f32_elem<DT>(c[e]);
-        if (vec) {
-          *reinterpret_cast<uint2*>(p) = uint2{o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16};
+        if (k + 4 <= g.K) {
+          store_any(p, uint2{o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16});
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -1574,7 +1570,7 @@ int launch_low_wgrad(const LowWgrad& g, hipStream_t s) {
     case NC_F16: return pick_low_wgrad<NC_F16>(g, s);
     case NC_BF16: return pick_low_wgrad<NC_BF16>(g, s);
     case NC_F32: {
-      const bool vec = load8_vec(g.dy, g.ldy, g.N, NC_F32);
+      const bool vec = wide8(g.N);
       if (vec) return g.relu ? pick_low_wgrad_f<true, true>(g, s) : pick_low_wgrad_f<false, true>(g, s);
       return g.relu ? pick_low_wgrad_f<true, false>(g, s) : pick_low_wgrad_f<false, false>(g, s);
     }
