@@ -614,7 +614,8 @@ typedef struct nc_codes_args {
   void* scales;        /* NC_CODES_ROW: float [rows]; else uint8 [rows][code_stride / 32] */
   void* values;        /* decode */
 } nc_codes_args;
-/* A row (group) that holds an infinity or NaN decodes to NaN throughout. */
+/* A row (group) that holds an infinity or NaN decodes to NaN throughout.  Decoded as NC_F16 (and in a layer of
+ * that type) a group's code for 65536, the nearest one to a magnitude over 65024, is 65504, half's largest. */
 int nc_encode_rows(const nc_codes_args* args, void* stream);
 int nc_decode_rows(const nc_codes_args* args, void* stream);
 

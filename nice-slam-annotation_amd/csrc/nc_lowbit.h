@@ -10,8 +10,10 @@
 //                   steps >= amax.
 // A group or row that holds an infinity or a NaN gets byte 255 (scale NaN) and codes that stand
 // for 0 steps: all its values are NaN, so the fault stays visible.  A step is a power of two
-// so that every value (at most 8 significant bits) is exact in float, bfloat16 and half: the
-// weight gradient multiplies the checkpoint's values without a rounding of their own.
+// so that every value (at most 8 significant bits) is exact in float and bfloat16, and in half for a
+// checkpoint of half values, but one: the code nearest to a magnitude over 65024 (RELU: 65280) stands for
+// 65536, which as half is the largest number, 65504, itself within half a step of that magnitude.  The
+// weight gradient multiplies the checkpoint's values without another rounding of their own.
 // Codes are stored in rows of code_stride bytes, a multiple of 128, with codes of 0 behind the
 // last column, so the matrix kernels read whole 128-byte slices of every row.
 #pragma once

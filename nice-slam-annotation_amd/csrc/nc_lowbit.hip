@@ -183,6 +183,8 @@ __global__ void __launch_bounds__(256) k_decode(const CodeCtx a, int64_t row_chu
     const uint32_t b = ((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 255u;
     const int q = a.format == NC_CODES_RELU ? (b > 0 ? (int)b - 1 : 0) : (int)(int8_t)b;
     v[e] = (float)q * s;
+    // as half, the one group code beyond its largest number ends there (nc_lowbit.h)
+    if (DT == NC_F16 && a.format != NC_CODES_ROW && __builtin_fabsf(v[e]) == 65536.f) v[e] = __builtin_copysignf(65504.f, v[e]);
   }
   store8<DT>(a.values, r * a.x_stride, c, a.cols, v);
 }

@@ -1114,7 +1114,7 @@ __device__ __forceinline__ uint2 tr_read(uint32_t at) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)at));
 }
 
-// 16 codes of one row and group -> 16 elements of 16 bits; step is a power of two: exact
+// 16 codes of one row and group -> 16 elements of 16 bits: the values that k_decode gives too
 template <bool F16, bool RELU>
 __device__ __forceinline__ void decode16(uint4 c, float step, uint4& lo, uint4& hi) {
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
@@ -1131,8 +1131,8 @@ __device__ __forceinline__ void decode16(uint4 c, float step, uint4& lo, uint4& 
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      if (F16) {
-        o[2 * j + e] = f32_elem<NC_F16>(v[2 * e]) | (uint32_t)f32_elem<NC_F16>(v[2 * e + 1]) << 16;
+      if (F16) {  // exact in half, but 65536: a conversion toward 0 makes it 65504
+        o[2 * j + e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v[2 * e], v[2 * e + 1]));
       } else {  // exact in bfloat16: the upper halves
         o[2 * j + e] = upper_halves(v[2 * e], v[2 * e + 1]);
       }

@@ -154,7 +154,8 @@ def quantize_rows(x):
 def pack_activations(x, relu=False):
     """The 8-bit checkpoint of ``x`` (``relu``: of max(x, 0), in codes whose 0 says x <= 0): 32
     neighbouring channels share a step, the least power of two of which 127 (254) hold the
-    group's largest magnitude.  1.03 bytes a channel; half a step of error.  Carries no gradient."""
+    group's largest magnitude.  1.03 bytes a channel; half a step of error.  As float16 a value of 65536 (the
+    nearest one to a magnitude over 65024) is float16's largest number, 65504.  Carries no gradient."""
     return _encode(x, L.NC_CODES_RELU if relu else L.NC_CODES_GROUP, "x")
 
 

@@ -27,8 +27,10 @@ def row_codes(x):
 
 
 def group_codes(x, relu):
-    """(codes float64 [M, K] as stored, bytes int64 [M, ceil(K / 32)], values float64 [M, K])."""
+    """(codes float64 [M, K] as stored, bytes int64 [M, ceil(K / 32)], values float64 [M, K]).  float16's largest
+    number ends the values of a float16 x: the one code value beyond it, 65536, is 65504 there."""
     m, k = x.shape
+    half = x.dtype == torch.float16
     x = x.double()
     a = torch.where(x > 0, x, torch.zeros_like(x)) if relu else x
     a = torch.where(torch.isnan(x), x, a)
@@ -47,6 +49,8 @@ def group_codes(x, relu):
     clean = torch.where(bad[..., None], torch.zeros_like(g), g)
     q = torch.round(clean / step[..., None]).clamp(-most, most)
     v = torch.where(bad[..., None], torch.full_like(q, float("nan")), q * step[..., None])
+    if half:
+        v = v.clamp(-65504, 65504)
     q, v = (t.reshape(m, -1)[:, :k] for t in (q, v))
     if relu:
         q = torch.where((x > 0) | torch.isnan(x), q + 1, torch.zeros_like(q))

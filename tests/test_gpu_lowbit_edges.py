@@ -1,0 +1,67 @@
+"""The 8-bit layer operators (nicecore.lowbit) at the ends of their types, at the sizes of a mapper
+iteration, and what their autograd graph and workspaces hold.
+
+Tolerances are those of tests/test_gpu_lowbit.py: u = 2^-24 is half a float32 step, sums of
+products as in sum_tol, the output's rounding as in out_tol.
+"""
+import ctypes
+import math
+
+import pytest
+import torch
+import torch.utils.checkpoint
+
+from oracle import lowbit_oracle as LO
+from test_gpu_lowbit import BF16, F16, F32, TYPES, U, acts, check, gen, layer_run, lb, out_tol, sum_tol
+
+pytestmark = pytest.mark.gpu
+
+
+def check_dw(dw, x, dy, relu):
+    """dW against the float64 sum over the checkpoint's values."""
+    v = LO.group_codes(x, relu)[2]
+    want = dy.double().t() @ v
+    t = sum_tol(dy.double().abs().t() @ v.abs(), x.shape[0], 3 if x.dtype == F32 else 1)
+    assert torch.isfinite(want).all() and torch.isfinite(dw).all()
+    check(dw, want, t + out_tol(want.abs() + t, x.dtype))
+
+
+# small tiles decode while they stage, the large ones of 2048 x 2048 take the values written out
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("m,k,n", [(5, 96, 40), (200, 300, 130), (70, 2048, 2048)])
+def test_half_checkpoints_of_the_largest_numbers(m, k, n, relu):
+    """float16's largest numbers: the nearest code of a magnitude over 65024 (65280 with relu) stands for 65536,
+    which as float16 is its largest number, 65504."""
+    x = acts(m, k, F16, 3)
+    top = torch.tensor([65024., 65056., 65280., 65312., 65472., 65504.], dtype=F16)
+    for i, t in enumerate(top):  # alone in its group, and beside values of every size
+        x[i % m, (33 * i) % k] = t
+        x[(i + 2) % m, (33 * i + 7) % k] = -t
+    x[:, 60] = 6e-8  # the least subnormal
+    x[1, 64:96] = (1e-6 * x[1, 64:96].float()).to(F16)  # a group of them
+    p = lb().pack_activations(x.cuda(), relu=relu)
+    v = LO.group_codes(x, relu)[2]
+    assert v.abs().max() == 65504 and torch.equal(p.dequantize().cpu().double(), v)
+    a = torch.relu(x.double()) if relu else x.double()
+    step = torch.ldexp(torch.ones_like(p.scales.cpu(), dtype=torch.float64), p.scales.cpu().int() - 127)
+    assert ((v - a).abs() <= step.repeat_interleave(32, 1)[:, :k] / 2).all()
+    wide = v.clone()
+    wide[v.abs() == 65504] = 65536 * v[v.abs() == 65504].sign()  # the code's own value
+    assert torch.equal(p.dequantize(F32).cpu().double(), wide)
+    g = gen(4)
+    w = (1e-4 * torch.randn(n, k, generator=g)).to(F16)
+    dy = (1e-3 * torch.randn(m, n, generator=g)).to(F16)
+    y, _, dw = layer_run(x, w, None, dy, relu)
+    assert torch.isfinite(y).all()
+    check_dw(dw, x, dy, relu)
+
+
+def test_half_values_of_float32_codes():
+    """Codes of float32 rows as float16: 65536 ends at 65504 too, larger values are infinite, subnormals rounded."""
+    x = torch.tensor([65536., -65536., 65535.5, 131072., 3., -3., 0., 1.])[:, None].expand(8, 32).contiguous()
+    x = torch.cat([x, x * 2.0 ** -40])
+    d = lb().pack_activations(x.cuda()).dequantize(F16).cpu()
+    want = LO.group_codes(x, False)[2]
+    want = torch.where(want.abs() == 65536, 65504 * want.sign(), want).to(F16)
+    assert torch.equal(d, want)
+    assert d[3].isinf().all() and d[0, 0] == 65504 and d[1, 0] == -65504
