@@ -596,7 +596,7 @@ int nc_imap_features(const double* pts, int64_t n_points, const float* fourier_B
 #define NC_F16 1
 #define NC_BF16 2
 #define NC_CODES_ROW 0   /* int8, float scale per row: s = max(fl(amax fl(1 / 127)), 2^-126), q = nearest to x / s */
-#define NC_CODES_GROUP 1 /* int8, one byte b per 32 columns: the step is 2^(b - 127), the least with 127 steps >= amax */
+#define NC_CODES_GROUP 1 /* int8 (-127 to 127), one byte b per 32 columns: the step is 2^(b - 127), the least with 127 steps >= amax */
 #define NC_CODES_RELU 2  /* uint8 of max(x, 0): 0 where x <= 0, else 1 + the number of steps (254 steps >= amax) */
 #define NC_MAX_STRIDE 4194304 /* elements between rows of x, dy, y and dx of a layer: offsets inside a tile fit 32 bits */
 #define NC_MAX_INPUTS 131072 /* 127^2 * 131072 < 2^31: an int32 sum of code products cannot overflow */

@@ -1121,12 +1121,14 @@ __device__ __forceinline__ void decode16(uint4 c, float step, uint4& lo, uint4& 
   uint32_t o[8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t b = RELU ? w[j] : w[j] ^ 0x80808080u;  // signed codes as code + 128
+    // signed codes, -127 to 127, as code + 127 (no byte borrows from the next): 127 of the largest steps are a
+    // finite float, 128 are not
+    const uint32_t b = RELU ? w[j] : (w[j] ^ 0x80808080u) - 0x01010101u;
     float v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float f = (float)((b >> (8 * e)) & 255u);
-      v[e] = __builtin_fmaf(f, step, RELU ? -step : -128.f * step);
+      v[e] = __builtin_fmaf(f, step, RELU ? -step : -127.f * step);
       if (RELU) v[e] = relu_keep_nan(v[e]);
     }
 #pragma unroll

@@ -65,3 +65,24 @@ def test_half_values_of_float32_codes():
     want = torch.where(want.abs() == 65536, 65504 * want.sign(), want).to(F16)
     assert torch.equal(d, want)
     assert d[3].isinf().all() and d[0, 0] == 65504 and d[1, 0] == -65504
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", [(5, 96, 40), (200, 300, 130), (70, 2048, 2048)])
+def test_checkpoints_of_the_largest_numbers(m, k, n, dtype, relu):
+    """Magnitudes up to the largest float: their groups' step is 2^121, which 128 times would not be finite."""
+    x = acts(m, k, dtype, 5)
+    end = torch.finfo(dtype).max
+    for i, t in enumerate((1.6e38, 1.69e38, 1.8e38, 3e38, 3.37e38, end)):
+        x[i % m, (33 * i) % k] = min(t, end)
+        x[(i + 2) % m, (33 * i + 7) % k] = -min(t, end)
+    p = lb().pack_activations(x.cuda(), relu=relu)
+    v = LO.group_codes(x, relu)[2]
+    assert torch.equal(p.dequantize(F32).cpu().double(), v)
+    g = gen(6)
+    w = (1e-30 * torch.randn(n, k, generator=g)).to(dtype)
+    dy = (1e-30 * torch.randn(m, n, generator=g)).to(dtype)
+    y, _, dw = layer_run(x, w, None, dy, relu)
+    assert torch.isfinite(y).all()
+    check_dw(dw, x, dy, relu)
