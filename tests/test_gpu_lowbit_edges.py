@@ -86,3 +86,29 @@ def test_checkpoints_of_the_largest_numbers(m, k, n, dtype, relu):
     y, _, dw = layer_run(x, w, None, dy, relu)
     assert torch.isfinite(y).all()
     check_dw(dw, x, dy, relu)
+
+
+# one and few rows, short sums, tiles, sums cut in parts; the third size of rows is coded before the call
+@pytest.mark.parametrize("m,k,n", [(1, 256, 64), (16, 300, 33), (200, 93, 256), (50, 700, 40), (700, 256, 384), (2100, 512, 640), (90, 8200, 33),
+                                   (300, 4096, 256)])
+@pytest.mark.parametrize("coded", [False, True])
+def test_quantized_linear_of_far_scales(m, k, n, coded):
+    """Scales whose product is no normal number, where y is one."""
+    x, w = acts(m, k, F32, m), acts(n, k, F32, n)
+    for sx, sw in ((1e-20, 1e-21), (1e-36, 1e-3), (1e-3, 1e-36), (1e34, 1e-36), (1e34, 1e6), (1e6, 1e34), (1e-30, 1e-30)):
+        xs, ws = x * sx, w * sw
+        xs[0, :] = 0
+        xs[0, :2] = 100 * sx  # a sum of exactly 0 with the first channel, whatever the scales
+        ws[0, :] = 0
+        ws[0, 0], ws[0, 1] = 100 * sw, -100 * sw
+        q, w8 = lb().quantize_rows(xs.cuda()), lb().quantize_rows(ws.cuda())
+        y = lb().quantized_linear(q if coded else xs.cuda(), w8).double().cpu()
+        xq, xsc = LO.row_codes(xs)
+        wq, wsc = LO.row_codes(ws)
+        want = LO.quantized_linear(xq, xsc, wq, wsc)
+        assert y[0, 0] == 0
+        big = torch.finfo(F32).max
+        fits = want.abs() * (1 + 4 * U) < big
+        check(y[fits], want[fits], 4 * U * want[fits].abs() + 2.0 ** -148)
+        over = want.abs() * (1 - 4 * U) > big
+        assert torch.equal(y[over], math.inf * want[over].sign())
