@@ -162,8 +162,8 @@ def pack_activations(x, relu=False):
 def quantized_linear(x, weight, bias=None, relu=False, out_dtype=None):
     """y = x8 W8^T + bias [, ReLU]: ``x`` [..., inputs] is encoded by quantize_rows within the call
     (or given as its CodedRows), ``weight`` = quantize_rows(W), W [outputs, inputs].  The sum of the
-    code products is exact (int32); y has ``out_dtype`` (default: x's).  For inference: x must
-    not require grad."""
+    code products is exact (int32); y has ``out_dtype`` (default: x's).  For inference: x and
+    bias must not require grad."""
     coded = isinstance(x, CodedRows)
     dev = x.device if coded else _device(x, "x")
     if not isinstance(weight, CodedRows) or weight._fmt != L.NC_CODES_ROW or len(weight._lead) != 1:
@@ -172,9 +172,11 @@ def quantized_linear(x, weight, bias=None, relu=False, out_dtype=None):
         raise L.NiceCoreError("x must be a tensor or quantize_rows(x)")
     if x.shape[-1:] != weight.shape[-1:]:
         raise L.NiceCoreError(f"x has shape {tuple(x.shape)}, the weight {tuple(weight.shape)}: channels differ")
-    if not coded and x.requires_grad and torch.is_grad_enabled():
-        raise L.NiceCoreError("quantized_linear has no gradient: call it under torch.no_grad() or with x.detach() "
-                              "(checkpointed_linear is the layer for training)")
+    if torch.is_grad_enabled():
+        for t, what in ((None if coded else x, "x"), (bias, "bias")):
+            if t is not None and t.requires_grad:
+                raise L.NiceCoreError(f"quantized_linear has no gradient: call it under torch.no_grad() or with "
+                                      f"{what}.detach() (checkpointed_linear is the layer for training)")
     out_dtype = out_dtype or x.dtype
     if out_dtype not in _DTYPES:
         raise L.NiceCoreError(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
