@@ -221,6 +221,13 @@ def _weight_rows(w, inputs):
     return w, w.stride(0)
 
 
+def _came_back(t, what, dev, dtype, size):
+    """A saved tensor is what a hook made of it: nothing else is read."""
+    if t.device != dev or t.dtype != dtype or t.numel() != size:
+        raise L.NiceCoreError(f"the saved {what} came back as {t.numel()} x {t.dtype} on {t.device}, "
+                              f"kept were {size} x {dtype} on {dev}")
+
+
 class _CheckpointedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, relu):
@@ -265,8 +272,9 @@ class _CheckpointedLinear(torch.autograd.Function):
             ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
             with _on(dev):
                 L.check(lib.nc_layer_forward(ref, ws.data_ptr(), nbytes, L.raw_stream(dev)), "nc_layer_forward")
-        ctx.save_for_backward(weight if need[0] else None)  # (checked for changes in place)
-        ctx.kept, ctx.args, ctx.shape, ctx.dtype = kept, a, x.shape, x.dtype
+        # (the weight is checked for changes in place; the backward frees the checkpoint)
+        ctx.save_for_backward(weight if need[0] else None, kept)
+        ctx.args, ctx.shape, ctx.dtype = a, x.shape, x.dtype
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], outputs)
 
     @staticmethod
@@ -275,11 +283,15 @@ class _CheckpointedLinear(torch.autograd.Function):
             return None, None, None, None
         if torch.is_grad_enabled():
             raise L.NiceCoreError("checkpointed_linear has no second derivative (backward with create_graph=True)")
-        weight, = ctx.saved_tensors
-        kept, a, dtype = ctx.kept, ctx.args, ctx.dtype
+        weight, kept = ctx.saved_tensors
+        a, dtype = ctx.args, ctx.dtype
         rows, inputs, outputs, stride = a.rows, a.inputs, a.outputs, a.code_stride
         need = ctx.needs_input_grad
         dev = dy.device
+        if weight is not None:
+            _came_back(weight, "weight", dev, dtype, outputs * inputs)
+        if kept is not None:
+            _came_back(kept, "checkpoint", dev, torch.uint8, rows * (stride + stride // GROUP))
         dy2, _, _, dy_stride = _rows(dy, "the gradient")
         dx = torch.empty(ctx.shape, device=dev, dtype=dtype) if need[0] else None
         dw = torch.empty((outputs, inputs), device=dev, dtype=dtype) if need[1] else None
@@ -289,6 +301,7 @@ class _CheckpointedLinear(torch.autograd.Function):
             w2, w_stride = _weight_rows(weight, inputs)
             w_ptr = w2.data_ptr()
         if kept is not None:
+            kept = kept.contiguous()
             codes = kept.data_ptr()
         b = L.NcLayerArgs(L.NC_ABI_VERSION, a.dtype, a.relu, 0, rows, inputs, outputs, None, 0, w_ptr, w_stride, None, None, 0,
                           codes, codes + rows * stride if codes else None, stride, dy2.data_ptr(), dy_stride,
@@ -313,7 +326,8 @@ def checkpointed_linear(x, weight, bias=None, relu=False):
     sees the checkpoint's values.  All tensors have one dtype; sums are held in float32.  A float32
     product keeps 22 bits of a value down to 2^-14 of the largest in its row of x, dy or W (fewer below: its
     floor is 2^-36 of that) and is then as near to the exact result as a plain float32 product; an infinity
-    in x or dy makes NaN of its row.  A chain of such layers trains an MLP.  Has no second derivative."""
+    in x or dy makes NaN of its row.  A chain of such layers trains an MLP.  Has no second derivative.
+    The checkpoint is a saved tensor: a backward frees it, and saved-tensor hooks may move it."""
     if not torch.is_grad_enabled():  # no backward, no checkpoint (a Function sees the inputs' own requires_grad)
         x, weight, bias = (t.detach() if isinstance(t, torch.Tensor) else t for t in (x, weight, bias))
     return _CheckpointedLinear.apply(x, weight, bias, bool(relu))

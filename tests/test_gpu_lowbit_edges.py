@@ -112,3 +112,65 @@ def test_quantized_linear_of_far_scales(m, k, n, coded):
         check(y[fits], want[fits], 4 * U * want[fits].abs() + 2.0 ** -148)
         over = want.abs() * (1 - 4 * U) > big
         assert torch.equal(y[over], math.inf * want[over].sign())
+
+
+def step_leaves(dtype=F32, m=300, k=256, n=96):
+    x, w, dy = acts(m, k, dtype, 1).cuda(), acts(n, k, dtype, 2).cuda(), acts(m, n, dtype, 3).cuda()
+    b = torch.ones(n, device="cuda", dtype=dtype)
+    return [t.requires_grad_(True) for t in (x, w, b)], dy
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_checkpoint_is_a_saved_tensor(dtype, relu):
+    """Hooks on saved tensors see the codes, may move them, and the gradients are the same."""
+    leaves, dy = step_leaves(dtype)
+    want = torch.autograd.grad(lb().checkpointed_linear(*leaves, relu=relu), leaves, dy)
+    seen = []
+
+    def pack(t):
+        seen.append((t.dtype, t.numel()))
+        return t.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.cuda()):
+        y = lb().checkpointed_linear(*leaves, relu=relu)
+    assert (torch.uint8, 300 * (256 + 8)) in seen
+    for a, b in zip(torch.autograd.grad(y, leaves, dy), want):
+        assert torch.equal(a, b)
+    with torch.autograd.graph.save_on_cpu():
+        y = lb().checkpointed_linear(*leaves, relu=relu)
+    for a, b in zip(torch.autograd.grad(y, leaves, dy), want):
+        assert torch.equal(a, b)
+
+    def layer(*t):
+        return lb().checkpointed_linear(*t, relu=relu)
+
+    y = torch.utils.checkpoint.checkpoint(layer, *leaves, use_reentrant=False)
+    for a, b in zip(torch.autograd.grad(y, leaves, dy), want):
+        assert torch.equal(a, b)
+
+
+def test_the_checkpoint_is_freed_by_the_backward():
+    """An output that is kept after the backward holds no codes; a graph that is kept does, and serves again."""
+    leaves, dy = step_leaves(m=40000)
+    codes = 40000 * (256 + 8)
+    y = lb().checkpointed_linear(*leaves)
+    first = [t.cpu() for t in torch.autograd.grad(y, leaves, dy, retain_graph=True)]
+    held = torch.cuda.memory_allocated()
+    second = [t.cpu() for t in torch.autograd.grad(y, leaves, dy)]
+    assert held - torch.cuda.memory_allocated() >= codes
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, leaves, dy)
+
+
+@pytest.mark.parametrize("unpack", [lambda t: t, lambda t: t.cuda().short(), lambda t: t.cuda()[:1]])
+def test_a_checkpoint_that_comes_back_otherwise_is_refused(unpack):
+    """Saved tensors that hooks give back on another device, as another type or cut short are not read."""
+    from nicecore import _lib as L
+    leaves, dy = step_leaves()
+    leaves[0].requires_grad_(False)  # (the weight is not saved then)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), unpack):
+        y = lb().checkpointed_linear(*leaves)
+    with pytest.raises(L.NiceCoreError, match="checkpoint came back"):
+        torch.autograd.grad(y, leaves[1:], dy)
