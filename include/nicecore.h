@@ -646,7 +646,9 @@ int nc_quantized_linear(const nc_qlinear_args* args, void* workspace, size_t wor
  * NC_CODES_GROUP), all that the backward reads of x:
  *   dx = (dy W) [code != 0 if relu],  dw = dy^T value(codes),  db = sum_m dy.
  * codes may be NULL in a forward without a backward.  Every output of the backward may be NULL.
- * The workspace of either call is free again when the call's work on the stream has ended. */
+ * The workspace of either call is free again when the call's work on the stream has ended.  Its size is asked for with
+ * the call's arguments: it goes by the addresses' alignment (16-bit types) and by the backward's outputs (dx, dw, db;
+ * what is enough for some of them is enough for fewer). */
 typedef struct nc_layer_args {
   int32_t abi_version;
   int32_t dtype;       /* of every tensor; products and sums in 32 bits */

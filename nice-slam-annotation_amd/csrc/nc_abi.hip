@@ -1271,7 +1271,8 @@ void imap_layout(int64_t N, int64_t P, bool rays, bool bwd, bool coded, ImapWs& 
   take(w.pf, (size_t)P * 16);
   if (coded) {
     for (int l = 0; l < 5; ++l) {
-      const nc_layer_args a = imap_layer(l, P);
+      nc_layer_args a = imap_layer(l, P);
+      a.dx = a.dw = a.db = &a;  // the size with all outputs, which are not touched
       take(w.code[l], (size_t)P * a.code_stride);
       take(w.step[l], (size_t)P * (a.code_stride / CODE_GROUP));
       const size_t f = nc_layer_workspace_bytes(&a, 0), b = nc_layer_workspace_bytes(&a, 1);
@@ -1801,7 +1802,7 @@ Operand operand_a(int dtype, const void* p, int64_t rows, int64_t cols, int64_t 
 }
 
 struct LayerWs {
-  Operand a, b;            // the forward's x and W, the backward's dY and W^T
+  Operand a, b = {};       // the forward's x and W, the backward's dY and W^T
   size_t gemm_part = 0, part = 0, sums = 0, values = 0, tops = 0, total = 0;
   bool decodes = false;    // dW: the codes' values are written out first
   int32_t gemm_splits = 1, splits = 0, pieces = 0;
@@ -1816,20 +1817,30 @@ void layer_layout(const nc_layer_args* a, bool backward, LayerWs& w) {
   if (!backward) {
     w.a = operand_a(a->dtype, a->x, a->rows, k, a->x_stride, a->relu != 0, o);
     w.b = operand(a->dtype, a->w, n, k, a->w_stride, false, o);
-  } else {
+  } else {  // room for the outputs that are asked for, so that more of them never need less
     w.a = operand_a(a->dtype, a->dy, a->rows, k, a->dy_stride, false, o);
-    w.b = operand(a->dtype, nullptr, n, k, 0, true, o);
-    w.tops = o;
-    if (a->dtype == NC_F32) o = align256(o + (size_t)((k + TOP_ROWS - 1) / TOP_ROWS) * (size_t)n * 4);
     low_wgrad_splits(a->dtype, a->rows, a->outputs, a->inputs, a->dw != nullptr, w.splits, w.pieces, w.rows_per);
-    w.part = o;
-    o = align256(o + (size_t)w.splits * (size_t)a->outputs * (size_t)a->inputs * 4);
-    w.sums = o;
-    const int64_t pieces = std::max((w.rows_per + 511) / 512, (a->inputs + 127) / 128);  // with dW or without
-    o = align256(o + (size_t)w.splits * (size_t)pieces * (size_t)a->outputs * 4);
-    w.decodes = low_wgrad_decodes(a->dtype, a->rows, a->outputs, a->inputs);
-    w.values = o;
-    if (w.decodes) o = align256(o + (size_t)round_up(a->rows, 64) * (size_t)round_up(a->inputs, CODE_ALIGN) * 2);
+    if (a->dx) {
+      w.b = operand(a->dtype, nullptr, n, k, 0, true, o);
+      w.tops = o;
+      if (a->dtype == NC_F32) o = align256(o + (size_t)((k + TOP_ROWS - 1) / TOP_ROWS) * (size_t)n * 4);
+    }
+    if (a->dw) {
+      w.part = o;
+      if (w.splits > 1) o = align256(o + (size_t)w.splits * (size_t)a->outputs * (size_t)a->inputs * 4);
+      w.decodes = low_wgrad_decodes(a->dtype, a->rows, a->outputs, a->inputs);
+      w.values = o;
+      if (w.decodes) o = align256(o + (size_t)round_up(a->rows, 64) * (size_t)round_up(a->inputs, CODE_ALIGN) * 2);
+    }
+    if (a->db) {
+      w.sums = o;
+      const int64_t pieces = std::max((w.rows_per + 511) / 512, (a->inputs + 127) / 128);  // with dW or without
+      o = align256(o + (size_t)w.splits * (size_t)pieces * (size_t)a->outputs * 4);
+    }
+    if (!a->dx) {
+      w.total = o;
+      return;
+    }
   }
   w.gemm_splits = low_gemm_splits(layer_mode(a->dtype), a->rows, n, k);
   w.gemm_part = o;
@@ -2128,7 +2139,7 @@ int nc_layer_backward(const nc_layer_args* a, void* ws, size_t ws_bytes, void* s
     g.want_db = a->db != nullptr;
     g.pieces = w.pieces;
     const int32_t db_parts = w.splits * g.pieces;
-    if (w.decodes && a->dw) {
+    if (w.decodes) {
       CodeCtx c;
       std::memset(&c, 0, sizeof(c));
       c.dtype = a->dtype;

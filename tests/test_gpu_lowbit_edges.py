@@ -174,3 +174,76 @@ def test_a_checkpoint_that_comes_back_otherwise_is_refused(unpack):
         y = lb().checkpointed_linear(*leaves)
     with pytest.raises(L.NiceCoreError, match="checkpoint came back"):
         torch.autograd.grad(y, leaves[1:], dy)
+
+
+def in_guard(nbytes):
+    """A workspace of NaNs with as much behind it."""
+    return torch.full((nbytes + (1 << 20),), 255, device="cuda", dtype=torch.uint8)
+
+
+def intact(guard, nbytes):
+    torch.cuda.synchronize()
+    return bool((guard[nbytes:] == 255).all())
+
+
+# odd and whole sizes; cut sums of every product; few rows; the decoded values of the large tiles
+SIZES = [(77, 100, 50), (700, 200, 130), (2048, 64, 1), (200, 4096, 256), (500, 1024, 1024), (3000, 33, 70), (70, 2048, 2048)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", SIZES)
+def test_layers_stay_in_the_workspace_that_they_ask_for(m, k, n, dtype):
+    """Forward and backward, each choice of outputs, from exactly as many bytes as the query says."""
+    from nicecore import _lib as L
+    lib, s = L.load(), L.raw_stream(torch.device("cuda", 0))
+    x, w, b, dy = acts(m, k, dtype, 1).cuda(), acts(n, k, dtype, 2).cuda(), acts(1, n, dtype, 3)[0].cuda(), acts(m, n, dtype, 4).cuda()
+    want = layer_run(x, w, b, dy, True)
+    leaves = b.clone().requires_grad_()
+    alone = torch.autograd.grad(lb().checkpointed_linear(x, w, leaves, relu=True), leaves, dy)[0]
+    kp = (k + 127) // 128 * 128
+    codes, steps = torch.empty(m, kp, device="cuda", dtype=torch.uint8), torch.empty(m, kp // 32, device="cuda", dtype=torch.uint8)
+    y = torch.empty_like(dy)
+    kind = {F32: L.NC_F32, F16: L.NC_F16, BF16: L.NC_BF16}[dtype]
+
+    def run(call, back, **out):
+        a = L.NcLayerArgs(abi_version=L.NC_ABI_VERSION, dtype=kind, relu=1, rows=m, inputs=k, outputs=n, x=x.data_ptr(), x_stride=k,
+                          w=w.data_ptr(), w_stride=k, bias=b.data_ptr(), y=y.data_ptr(), y_stride=n, codes=codes.data_ptr(),
+                          steps=steps.data_ptr(), code_stride=kp, dy=dy.data_ptr(), dy_stride=n, dx_stride=k,
+                          **{o: t.data_ptr() for o, t in out.items()})
+        size = lib.nc_layer_workspace_bytes(ctypes.byref(a), back)
+        guard = in_guard(size)
+        assert call(ctypes.byref(a), guard.data_ptr(), size, s) == 0
+        assert intact(guard, size)
+        if size > 256:
+            assert call(ctypes.byref(a), guard.data_ptr(), size - 1, s) < 0
+
+    run(lib.nc_layer_forward, 0)
+    assert torch.equal(y, want[0])
+    for names in (("dx", "dw", "db"), ("dw", "db"), ("dx",), ("dw",), ("db",), ("dx", "db")):
+        out = {"dx": torch.full_like(x, math.nan), "dw": torch.full_like(w, math.nan), "db": torch.full_like(b, math.nan)}
+        run(lib.nc_layer_backward, 1, **{o: out[o] for o in names})
+        for o, t in zip(("dx", "dw", "db"), want[1:]):
+            # (db without dW adds its rows in other parts)
+            assert torch.equal(out[o], alone if o == "db" and "dw" not in names else t) if o in names else out[o].isnan().all(), (names, o)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", [(1, 256, 64), (64, 4096, 40), (200, 93, 256), (90, 8200, 33), (300, 4096, 256), (2100, 512, 640)])
+@pytest.mark.parametrize("coded", [False, True])
+def test_products_stay_in_the_workspace_that_they_ask_for(m, k, n, dtype, coded):
+    from nicecore import _lib as L
+    lib, s = L.load(), L.raw_stream(torch.device("cuda", 0))
+    x = acts(m, k, dtype, 1).cuda()
+    q, w8 = lb().quantize_rows(x), lb().quantize_rows(acts(n, k, F32, 2).cuda())
+    want = lb().quantized_linear(q if coded else x, w8)
+    out = torch.full((m, n), math.nan, device="cuda", dtype=dtype)
+    kind = L.NC_F32 if dtype == F32 else L.NC_BF16
+    a = L.NcQlinearArgs(abi_version=L.NC_ABI_VERSION, dtype=kind, out_dtype=kind, rows=m, inputs=k, outputs=n,
+                        x=None if coded else x.data_ptr(), x_stride=k, x_codes=q._storage.data_ptr(), x_scales=q._scales.data_ptr(),
+                        code_stride=w8._storage.shape[1], w_codes=w8._storage.data_ptr(), w_scales=w8._scales.data_ptr(),
+                        out=out.data_ptr(), out_stride=n)
+    size = lib.nc_quantized_linear_workspace_bytes(ctypes.byref(a))
+    guard = in_guard(size)
+    assert lib.nc_quantized_linear(ctypes.byref(a), guard.data_ptr(), size, s) == 0
+    assert intact(guard, size)
+    assert torch.equal(out, want)
