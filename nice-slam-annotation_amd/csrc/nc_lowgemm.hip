@@ -923,6 +923,7 @@ constexpr int SMALL_PAD = 16;  // bytes behind a row of codes in LDS: rows start
 template <int DX, bool VEC, int MT, int WK>
 __global__ void __launch_bounds__(256) k_low_small(const LowSmall p) {
   const LowGemm& g = p.g;
+  static_assert(WK == 4 || DX >= 0, "given codes: the sums' barriers are between the scales and their use");
   constexpr int RB = 16 * MT;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // x codes; then the waves' sums
   __shared__ float scale[RB];
@@ -1067,8 +1068,6 @@ __global__ void __launch_bounds__(256) k_low_small(const LowSmall p) {
 #pragma unroll
     for (int k = 1; k < 4; ++k) t += part[(k * MT + wave) * 64 + lane];
     acc[0] = t;
-  } else if (DX < 0) {
-    __syncthreads();  // scale[]
   }
   const int64_t n = n0 + 4 * q;
   if (n >= g.N) return;
