@@ -192,25 +192,32 @@ __device__ __forceinline__ void split3(const float (&x)[8], uint4 (&plane)[3]) {
   }
 }
 
-// x scale = x0 + x1 in half, |x scale| < 2^15: x0 the nearest, x1 what is left, rounded: within 2^-22 of |x|, or
-// 2^-25 / scale for small ones.  Of 8 values: a plane is 4 words.  An infinity leaves a NaN in the second plane.
-// (Written as fused multiply-adds that end in half: one instruction an element and plane.)
+// x scale = x0 + x1 in half, |x scale| < 2^15: x0 the nearest, x1 what is left, rounded.  x1 is given times 2^UP: within
+// 2^-22 of |x|, or 2^-(25 + UP) / scale for small ones.  Of 8 values: a plane is 4 words.  An infinity leaves a NaN in
+// the second plane.  (Written as fused multiply-adds that end in half: one instruction an element and plane.)
+template <int UP>
 __device__ __forceinline__ void split2(const float (&x)[8], float scale, uint4 (&plane)[2]) {
-  uint32_t hi[4], lo[4];
+  uint32_t w[2][4];
+  constexpr float up = (float)(1 << UP);
+  const float scaled = scale * up;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float a = x[2 * j], b = x[2 * j + 1];
-    const _Float16 ah = (_Float16)__builtin_fmaf(a, scale, 0.f), bh = (_Float16)__builtin_fmaf(b, scale, 0.f);
-    const _Float16 al = (_Float16)__builtin_fmaf(a, scale, -(float)ah), bl = (_Float16)__builtin_fmaf(b, scale, -(float)bh);
-    hi[j] = __builtin_bit_cast(uint16_t, ah) | (uint32_t)__builtin_bit_cast(uint16_t, bh) << 16;
-    lo[j] = __builtin_bit_cast(uint16_t, al) | (uint32_t)__builtin_bit_cast(uint16_t, bl) << 16;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float v = x[2 * j + k];
+      const _Float16 h = (_Float16)__builtin_fmaf(v, scale, 0.f);
+      const _Float16 l = (_Float16)(UP ? __builtin_fmaf(-(float)h, up, v * scaled) : __builtin_fmaf(v, scale, -(float)h));
+      w[0][j] = k ? w[0][j] | (uint32_t)__builtin_bit_cast(uint16_t, h) << 16 : __builtin_bit_cast(uint16_t, h);
+      w[1][j] = k ? w[1][j] | (uint32_t)__builtin_bit_cast(uint16_t, l) << 16 : __builtin_bit_cast(uint16_t, l);
+    }
   }
-  plane[0] = uint4{hi[0], hi[1], hi[2], hi[3]};
-  plane[1] = uint4{lo[0], lo[1], lo[2], lo[3]};
+#pragma unroll
+  for (int p = 0; p < 2; ++p) plane[p] = uint4{w[p][0], w[p][1], w[p][2], w[p][3]};
 }
-// biased exponent of the largest magnitude, for scales that are normal floats too: zero and subnormals count as 15,
-// infinities as 254
-__device__ __forceinline__ int top_exponent(uint32_t top) { return min(max((int)(top >> 23), 15), 254); }
+// biased exponent of the largest magnitude, for scales (times 2^UP) that are normal floats too: zero and what is below
+// 2^(UP - 112) count as 15 + UP, infinities as 254
+template <int UP>
+__device__ __forceinline__ int top_exponent(uint32_t top) { return min(max((int)(top >> 23), 15 + UP), 254); }
 // 2^(to - e): what has exponent e is below 2^(to - 126)
 __device__ __forceinline__ float scale_to(int to, int e) { return __builtin_bit_cast(float, (uint32_t)(127 + to - e) << 23); }
 

@@ -206,14 +206,14 @@ __global__ void __launch_bounds__(256) k_split(const SplitCtx a) {
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-  const int e = top_exponent(top);
+  const int e = top_exponent<0>(top);
   if (lane == 0) a.exponent[r] = e;
   for (int64_t c = lane; 8 * c < a.dst_stride; c += 64) {
     float v[8];
     load8<NC_F32, VEC>(a.x, off, c, a.cols, v);
     clear8<VEC>(c, a.cols, v);
     uint4 p[2];
-    split2(v, scale_to(141, e), p);
+    split2<0>(v, scale_to(141, e), p);
 #pragma unroll
     for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(a.dst + k * a.plane + r * a.dst_stride + 8 * c) = p[k];
   }
@@ -285,10 +285,10 @@ __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = tile[cc][r8 + e];
-      const int e = top_exponent(max(max(red[0][cc], red[1][cc]), max(red[2][cc], red[3][cc])));
+      const int e = top_exponent<0>(max(max(red[0][cc], red[1][cc]), max(red[2][cc], red[3][cc])));
       if (r0 + r8 == 0) a.exponent[c0 + cc] = e;
       uint4 p[2];
-      split2(x, scale_to(141, e), p);
+      split2<0>(x, scale_to(141, e), p);
 #pragma unroll
       for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(d + k * a.plane) = p[k];
     } else {

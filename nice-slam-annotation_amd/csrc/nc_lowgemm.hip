@@ -400,12 +400,15 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 // The same pipeline over slices of 32 columns, as three products of half planes: x = (x0 + x1) / scale
 // (split2), C = x0 y0 + x0 y1 + x1 y0.  B's scale is a power of two of its row, A's one of its row so far: it puts
 // the first 32 columns' largest below 2^12 and stays until one reaches 2^15, when the row's sums are scaled
-// down with it (seldom after the first slices).  Both are undone in the epilogue.  A value keeps 22 bits, or 2^-36
-// of the largest before it in its row of A (2^-40 of the largest in its row of B); the product left out is
-// below 2^-22: 2^-20.4 of |x y| at most, about 2^-23 on average.  Off the exact result by 1.9e-7 at 200 x 93 x 256 (a plain
-// float product: 2.9e-7), 3.6e-7 at 2048 x 1024 x 4096 (1.1e-6).  Six products of exact bfloat16 planes, 2.5e-7 and
+// down with it (seldom after the first slices).  Both are undone in the epilogue.  A's x1 is held times 2^11 and
+// multiplied by y0 2^-11, made of y0 as it arrives: a half has no digits below 2^-24, and x1 would lose its own there.
+// A value of A keeps 22 bits down to 2^-25 of the largest before it in its row (its floor is 2^-47 of that), one of B
+// down to 2^-17 of the largest in its row (2^-38); the product left out is below 2^-22: 2^-20.4 of |x y| at most, about
+// 2^-23 on average.  Off the exact result by 1.9e-7 at 200 x 93 x 256 (a plain float product: 2.9e-7), 3.6e-7 at
+// 2048 x 1024 x 4096 (1.1e-6); 2000 x 256 x 256 with one input of 10^6 beside those of 1: 1.9e-7 (x1 without its 2^11
+// 6e-6, a plain product 2.9e-7; the 2^11 cost 2 - 3 % of a product).  Six products of exact bfloat16 planes, 2.5e-7 and
 // 5.1e-7 there for the longer chain of sums, are twice the work for matrix cores that are bound by their
-// power: 4096 x 4096 x 4096 740 us, here 385.
+// power: 4096 x 4096 x 4096 740 us, here 385 - 465 by the clock.
 // Planes lie in LDS as rows of 64 bytes, 16-byte chunk c of row r at c ^ F((r >> 2) & 3), F = (0, 2, 3, 1):
 // conflict-free for ds_read_b128 (the third weight plane's layout of nc_device.h).  A's floats go into a piece of
 // LDS of their own, where each lane finds the 8 columns that it asked for; it reads them, asks for those two
@@ -420,6 +423,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 // RELU: of max(A, 0); MASK: the output is masked by codes and has no bias (each would take 16 registers).
 // Measured, M x K x N: 220000 x 256 x 256 141 us (450 MB: 91 us at a copy's rate; all workgroups store at once, and
 // loads behind stores wait for them), 4096 x 4096 x 4096 385 - 400 us = 1.05 PFLOP/s of plane products.
+constexpr int A_UP = 11;  // bits of a half: x1 2^11 is as large as x0
 template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
 __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, int32_t tiles, int32_t nt) {
   constexpr int W = WM * WN, T = 64 * W, FM = BM / WM / 16, FN = BN / WN / 16;
@@ -573,11 +577,11 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
       uint32_t bits = __builtin_bit_cast(uint32_t, top);
       bits = max(bits, (uint32_t)__builtin_amdgcn_mov_dpp((int)bits, 0xb1, 0xf, 0xf, true));  // lane ^ 1
       bits = max(bits, (uint32_t)__builtin_amdgcn_mov_dpp((int)bits, 0x4e, 0xf, 0xf, true));  // lane ^ 2
-      const int e = top_exponent(bits);
+      const int e = top_exponent<A_UP>(bits);
       xe[l] = fresh_row || e > xe[l] + 3 ? e : xe[l];
       if (c == 0) exps[half * BM + r] = xe[l];
       uint4 p[2];
-      split2(x, scale_to(138, xe[l]), p);
+      split2<A_UP>(x, scale_to(138, xe[l]), p);
 #pragma unroll
       for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(s + k * APL + r * 64 + hchunk3(r, c)) = p[k];
     }
@@ -591,6 +595,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   const unsigned char* fa = lds + (wm + i) * 64 + hchunk3(i, q);  // wm, wn and 16 u leave the chunk order as it is
   const unsigned char* fb = lds + B0 + (wn + i) * 64 + hchunk3(i, q);
   uint4 a[2][2], b[2][FN];  // a[block & 1][plane], b[plane][block]
+  uint4 down[FN];           // b[0] 2^-A_UP
   int ea[FM], next_ea[FM];  // exponents of the sums, of the next slice's rows
   bool fresh = true;        // the sums are zero
   auto read_a = [&](int half, int u) {
@@ -625,10 +630,17 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
   };
   auto multiply = [&](int u, int v0) {  // blocks (u, v0) and (u, v0 + 1); the smallest products first
     __builtin_amdgcn_sched_barrier(0);
+    if (u == 0)
 #pragma unroll
-    for (int p = 0; p < 3; ++p)
+      for (int v = v0; v < v0 + 2; ++v)
+        down[v] = __builtin_bit_cast(uint4, __builtin_bit_cast(half8, b[0][v]) * (_Float16)(1.f / (1 << A_UP)));
 #pragma unroll
-      for (int v = v0; v < v0 + 2; ++v) acc[u][v] = Mac<LOW_F16>::mac(b[p == 1][v], a[u & 1][p == 0], acc[u][v]);
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int v = v0; v < v0 + 2; ++v) {
+        const int p = u == 0 ? (k + 1) % 3 : k;
+        acc[u][v] = Mac<LOW_F16>::mac(p == 0 ? down[v] : b[p == 1][v], a[u & 1][p == 0], acc[u][v]);
+      }
     __builtin_amdgcn_sched_barrier(0);
   };
   enter_a();

@@ -247,3 +247,31 @@ def test_products_stay_in_the_workspace_that_they_ask_for(m, k, n, dtype, coded)
     assert lib.nc_quantized_linear(ctypes.byref(a), guard.data_ptr(), size, s) == 0
     assert intact(guard, size)
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("far,kind", [(1e4, "unused"), (1e6, "unused"), (1e7, "unused"), (1e4, "scaled"), (1e6, "scaled"), (1e8, "scaled")])
+@pytest.mark.parametrize("m,k,n", [(70, 256, 130), (300, 93, 256), (2000, 1024, 300), (4100, 256, 1500)])
+def test_float32_products_of_rows_with_a_far_value(m, k, n, far, kind, back):
+    """One input (one output's gradient) is far larger than the others, and its weights are 0 or as much smaller.
+    x = (x0 + x1) / scale with the largest so far at 2^11 or above: x0 is off by 2^-11 of x or 2^-25, x1 is that
+    remainder times 2^11, off by as much again: 2^-22 of x, or 2^-36 = 2^-47 of the largest.  W's planes, the largest at
+    2^14 or above, are off by 2^-22 of w or 2^-25 = 2^-39 of the largest, and as much for W's first plane times 2^-11,
+    which multiplies x1 2^11, no larger than x.  The rest as in test_gpu_lowbit.py."""
+    g = gen(k + n)
+    kk, nn = (n, k) if back else (k, n)  # the sum's length, the results
+    a, w = torch.randn(m, kk, generator=g), torch.randn(nn, kk, generator=g) / math.sqrt(kk)
+    a[:, 17] *= far
+    w[:, 17] *= 0.0 if kind == "unused" else 1 / far
+    if back:
+        got = layer_run(torch.randn(m, k, generator=g), w.t().contiguous(), None, a, False)[1]
+    else:
+        got = layer_run(a, w, None, torch.zeros(m, n), False)[0]
+    a, w = a.double(), w.double()
+    want = a @ w.t()
+    floors = 2.0 ** -47 * a.abs().amax(1, keepdim=True) * w.abs().sum(1) + 2.0 ** -38 * a.abs().sum(1, keepdim=True) * w.abs().amax(1)
+    t = sum_tol(a.abs() @ w.abs().t(), kk, 6) + floors
+    check(got, want, t + out_tol(want.abs() + t, F32))
+    if far <= 1e6 or kind == "unused":  # the floors are below the other roundings: as near as ordinary rows
+        rel = ((got.detach().double().cpu() - want).norm() / want.norm()).item()
+        assert rel <= 4 * U * math.sqrt(6 * kk / 32 + 16), rel
