@@ -229,10 +229,11 @@ def eval_points(module, p, activations=None):
 
 
 class QuantizedMLP:
-    """The iMAP* MLP held in 8 bits, for queries without gradients (meshing, rendering points): every
+    """The iMAP* MLP held in 8 bits, for point queries without gradients (meshing): every
     layer's weight as quantize_rows codes (nicecore.lowbit), made once from ``module``'s current
     parameters, and every layer a quantized_linear with the ReLU in its epilogue.  Takes the
-    module's place in eval_points and Renderer.eval_points.  Hidden activations are bfloat16."""
+    module's place in eval_points, Renderer.eval_points and calls as ``decoders(p, c_grid=None)``
+    (Renderer.py:74); rays are rendered with the module itself.  Hidden activations are bfloat16."""
 
     def __init__(self, module):
         from .lowbit import quantize_rows
@@ -260,7 +261,7 @@ class QuantizedMLP:
                                               L.raw_stream(self.device)), "nc_imap_features")
         return out
 
-    def __call__(self, p):
+    def __call__(self, p, c_grid=None):
         from .lowbit import quantized_linear
         h = self.features(p)
         with torch.no_grad():
@@ -281,6 +282,8 @@ def render_rays(module, rays_o, rays_d, bound, gt_depth=None, n_strat=32, n_impo
     9.5 KB; the weight gradients then see the checkpoints' values."""
     from .ops import sample_pdf
     from .render_fn import _bound_rows
+    if isinstance(module, QuantizedMLP):
+        raise L.NiceCoreError("a QuantizedMLP answers point queries (eval_points); rays are rendered with the MLP itself")
     if n_strat + n_importance > L.NC_MAX_SAMPLES:
         raise L.NiceCoreError("nicecore supports N_samples + N_importance <= 64")
     params = imap_params(module)

@@ -275,3 +275,12 @@ def test_float32_products_of_rows_with_a_far_value(m, k, n, far, kind, back):
     if far <= 1e6 or kind == "unused":  # the floors are below the other roundings: as near as ordinary rows
         rel = ((got.detach().double().cpu() - want).norm() / want.norm()).item()
         assert rel <= 4 * U * math.sqrt(6 * kk / 32 + 16), rel
+
+
+def test_a_quantised_mlp_is_called_as_the_module():
+    """decoders(p, c_grid=None), as the reference's renderer and mesher call the scene MLP."""
+    from nicecore import decoder as D
+    m = D.build_imap(seed=1).cuda()
+    q = m.quantize()
+    p = torch.rand(50, 3, generator=gen(1), dtype=torch.float64).cuda()
+    assert torch.equal(q(p, c_grid=None), q(p)) and q(p, c_grid=None).shape == m(p, c_grid=None).shape

@@ -41,3 +41,10 @@ def test_backward_workspace_goes_by_its_outputs():
     assert need(L.NC_BF16, 8192, 4096, 4096, dx=256) == 4096 * 4096 * 2
     assert need(L.NC_BF16, 8192, 4096, 4096, dw=256) == 8192 * 4096 * 2
     assert need(L.NC_BF16, 8192, 4096, 4096, db=256) < 1 << 20
+
+
+def test_a_quantised_mlp_renders_no_rays():
+    from nicecore import imap
+    q = object.__new__(imap.QuantizedMLP)
+    with pytest.raises(L.NiceCoreError, match="point queries"):
+        imap.render_rays(q, torch.zeros(1, 3), torch.ones(1, 3), torch.zeros(3, 2))
