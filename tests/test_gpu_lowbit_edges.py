@@ -284,3 +284,35 @@ def test_a_quantised_mlp_is_called_as_the_module():
     q = m.quantize()
     p = torch.rand(50, 3, generator=gen(1), dtype=torch.float64).cuda()
     assert torch.equal(q(p, c_grid=None), q(p)) and q(p, c_grid=None).shape == m(p, c_grid=None).shape
+
+
+@pytest.mark.parametrize("k,n,relu", [(93, 256, False), (256, 256, True), (256, 4, True)])
+def test_layers_of_a_mapper_iteration(k, n, relu):
+    """The scene MLP's layers on 5,000 rays of 44 samples, against the float64 layer on the device."""
+    m = 220000
+    g = torch.Generator(device="cuda").manual_seed(k + n)
+    x = torch.randn(m, k, generator=g, device="cuda")
+    w = torch.randn(n, k, generator=g, device="cuda") / math.sqrt(k)
+    b, dy = torch.randn(n, generator=g, device="cuda"), torch.randn(m, n, generator=g, device="cuda")
+    got = layer_run(x, w, b, dy, relu)
+    v = lb().pack_activations(x, relu=relu).dequantize().double()
+    rows = torch.randint(m, (4096,), generator=gen(1))  # of the codes against their definition
+    assert torch.equal(v[rows.cuda()].cpu(), LO.group_codes(x[rows.cuda()].cpu(), relu)[2])
+    a = (torch.relu(x) if relu else x).double()
+    w, dy = w.double(), dy.double()
+
+    def near(out, want, terms, count, planes):
+        tol = sum_tol(terms, count, planes)
+        assert ((out.detach().double() - want).abs() <= tol + U * (want.abs() + tol)).all()
+        rel = ((out.detach().double() - want).norm() / want.norm()).item()
+        assert rel <= 4 * U * math.sqrt(planes * count / 32 + 16), rel
+
+    wt, ones = w.t().contiguous(), torch.ones(1, m, device="cuda", dtype=torch.float64)
+    near(got[0], a @ wt + b.double(), a.abs() @ wt.abs() + b.double().abs(), k, 6)
+    mask = (x > 0).double() if relu else torch.ones_like(a)
+    near(got[1], (dy @ w) * mask, dy.abs() @ w.abs(), n, 6)
+    dyt = dy.t().contiguous()
+    near(got[2], dyt @ v, dyt.abs() @ v.abs(), m, 3)
+    sums, terms = (ones @ dy)[0], (ones @ dy.abs())[0]
+    tol = (m / 8 + 300) * U * terms
+    assert ((got[3].detach().double() - sums).abs() <= tol + U * sums.abs()).all()
