@@ -320,7 +320,9 @@ __device__ __forceinline__ int row_code(float x, float s, float rcp) {
   return (int)__builtin_fminf(__builtin_fmaxf(t, -127.f), 127.f);
 }
 
-// a row's scale from its amax (magnitude bits)
+// a row's scale from its amax (magnitude bits): the product with the rounded 1 / 127, as a float tensor divided by a
+// number comes out on this hardware (torch does so), so that codes made there and here are the same.  5 % of rows get
+// a neighbour of the rounded quotient, which moves a code only where x / s is next to a half.
 __device__ __forceinline__ float row_scale(uint32_t top) {
   return __builtin_fmaxf(__builtin_bit_cast(float, top) * (1.f / 127.f), 0x1p-126f);
 }

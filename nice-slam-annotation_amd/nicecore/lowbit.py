@@ -145,7 +145,8 @@ def _encode(x, fmt, what):
 
 def quantize_rows(x):
     """int8 codes of ``x`` [..., channels] with one float32 scale per row:
-    s = max(amax |x| fl(1 / 127), 2^-126) in float32, q = the integer nearest to x / s (ties to even), value q s.
+    s = max(amax |x| fl(1 / 127), 2^-126) in float32 (what ``amax / 127`` of a float32 tensor gives on the device; within
+    one unit of the rounded quotient), q = the integer nearest to x / s (ties to even), value q s.
     A row that holds an infinity or NaN decodes to NaN.  A layer's weight [outputs, inputs] is
     encoded the same way (a scale per output channel).  Carries no gradient."""
     return _encode(x, L.NC_CODES_ROW, "x")
@@ -160,7 +161,8 @@ def pack_activations(x, relu=False):
 
 
 def quantized_linear(x, weight, bias=None, relu=False, out_dtype=None):
-    """y = x8 W8^T + bias [, ReLU]: ``x`` [..., inputs] is encoded by quantize_rows within the call
+    """y = x8 W8^T + bias, ``relu``: max(y, 0), the activation after the layer (checkpointed_linear's is the one before
+    it): ``x`` [..., inputs] is encoded by quantize_rows within the call
     (or given as its CodedRows), ``weight`` = quantize_rows(W), W [outputs, inputs].  The sum of the
     code products is exact (int32); y has ``out_dtype`` (default: x's).  For inference: x and
     bias must not require grad."""
@@ -322,7 +324,7 @@ def checkpointed_linear(x, weight, bias=None, relu=False):
     one layer of a scene MLP (decoder.py:190-219), differentiable in x, weight and bias.
 
     Instead of the input its backward keeps the 8-bit checkpoint of ``a`` (pack_activations: 1.03
-    bytes a channel):  dx = (dy W) [x > 0 if relu]  and  db  are those of the full layer, dW = dy^T a8
+    bytes a channel):  dx = (dy W) [x > 0 or NaN if relu]  and  db  are those of the full layer, dW = dy^T a8
     sees the checkpoint's values.  All tensors have one dtype; sums are held in float32.  y and dx of a
     float32 layer keep 22 bits of a value of x or dy down to 2^-25 of the largest in its row (a floor of 2^-47 of
     that) and of W down to 2^-17 of the largest in its row (of W^T for dx; 2^-38), and are as near to the exact result as a

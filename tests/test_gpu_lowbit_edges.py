@@ -316,3 +316,14 @@ def test_layers_of_a_mapper_iteration(k, n, relu):
     sums, terms = (ones @ dy)[0], (ones @ dy.abs())[0]
     tol = (m / 8 + 300) * U * terms
     assert ((got[3].detach().double() - sums).abs() <= tol + U * sums.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_row_scales_are_those_of_the_devices_own_division(dtype):
+    """A float32 tensor's amax / 127 on the device is the product with the rounded 1 / 127: the scales' definition."""
+    x = acts(4000, 200, dtype, 8).cuda()
+    assert torch.equal(lb().quantize_rows(x).scales, x.float().abs().amax(1) / 127)
+    ends = torch.tensor([torch.finfo(dtype).max, torch.finfo(dtype).tiny, 1.0], device="cuda", dtype=dtype)[:, None]
+    q = lb().quantize_rows(ends)
+    assert torch.equal(q.scales, (ends.float().abs().amax(1) / 127).clamp_min(2.0 ** -126))
+    assert torch.isfinite(q.dequantize()).all()
