@@ -1,9 +1,9 @@
 // nc_lowbit.hip — codes of the 8-bit layer operators and the copies that their matrix kernels read.
 //
 // Everything here is one pass over its input and bound by memory: a thread takes 8 neighbouring
-// columns (16 or 32 bytes in, 8 bytes of codes out).  Measured: rows of 16384 x 4096 bfloat16 to codes 48 us (4.2
-// TB/s), codes to values 32 us (6.3, the codes in the cache); groups of 100000 x 256 float 19 us (6.8, most of it in
-// the cache); the copy with codes of 8192 x 4096 bfloat16 23 us.
+// columns (16 or 32 bytes in, 8 bytes of codes out).  Measured: rows of 16384 x 4096 bfloat16 to codes 42 us (4.8
+// TB/s), codes to values 31 us (6.5, the codes in the cache); groups of 100000 x 256 float 19 us (6.8, most of it in
+// the cache); the copy with codes of 8192 x 4096 bfloat16 28 us.
 #include "nc_lowbit.h"
 
 #include <type_traits>

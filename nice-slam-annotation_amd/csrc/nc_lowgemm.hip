@@ -280,8 +280,8 @@ __global__ void __launch_bounds__(256) k_low_finish(const LowGemm g, int64_t qua
 // A slice is worked off in phases of 4 x FN blocks; while a phase multiplies, the next one's operands
 // are read from LDS.  Before the last phase a barrier says that the slice is read and the next one
 // has arrived; the slice after that goes into the freed half then, a whole slice ahead of its use.
-// Measured, M x K x N: int8 16384 x 4096 x 4096 232 us = 2.37 POP/s (a library's int8 product on this card: 2.47), bfloat16
-// 8192 x 4096 x 4096 205 us = 1.34 PFLOP/s (1.57).  The matrix cores are busy 55 - 62 % of the cycles at the 2.0 - 2.2
+// Measured, M x K x N: int8 16384 x 4096 x 4096 232 - 241 us = 2.3 POP/s (a library's int8 product on this card: 2.47),
+// bfloat16 8192 x 4096 x 4096 205 - 217 us = 1.3 PFLOP/s (1.57).  The matrix cores are busy 55 - 62 % of the cycles at the 2.0 - 2.2
 // GHz that their power leaves.  4 waves of 128 x 128 read a third less from LDS, but a wave alone on its SIMD waits
 // for every read: int8 392 us.  Half slices (64 bytes of a row) five deep: 255 us; memory prefers whole lines.
 template <int MODE, int DT, int BM, int BN, int WM, int WN>
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 // 2048 x 1024 x 4096 (1.1e-6); 2000 x 256 x 256 with one input of 10^6 beside those of 1: 1.9e-7 (x1 without its 2^11
 // 6e-6, a plain product 2.9e-7; the 2^11 cost 2 - 3 % of a product).  Six products of exact bfloat16 planes, 2.5e-7 and
 // 5.1e-7 there for the longer chain of sums, are twice the work for matrix cores that are bound by their
-// power: 4096 x 4096 x 4096 740 us, here 385 - 465 by the clock.
+// power: 4096 x 4096 x 4096 740 us on a card where these took 385, before the 2^11.
 // Planes lie in LDS as rows of 64 bytes, 16-byte chunk c of row r at c ^ F((r >> 2) & 3), F = (0, 2, 3, 1):
 // conflict-free for ds_read_b128 (the third weight plane's layout of nc_device.h).  A's floats go into a piece of
 // LDS of their own, where each lane finds the 8 columns that it asked for; it reads them, asks for those two
@@ -421,8 +421,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 // slices: the next tile's first slices are on their way while a tile ends, and its results leave from
 // registers and are not waited for.
 // RELU: of max(A, 0); MASK: the output is masked by codes and has no bias (each would take 16 registers).
-// Measured, M x K x N: 220000 x 256 x 256 141 us (450 MB: 91 us at a copy's rate; all workgroups store at once, and
-// loads behind stores wait for them), 4096 x 4096 x 4096 385 - 400 us = 1.05 PFLOP/s of plane products.
+// Measured, M x K x N: 220000 x 256 x 256 147 us (450 MB: 91 us at a copy's rate; all workgroups store at once, and
+// loads behind stores wait for them), 4096 x 4096 x 4096 464 us = 0.89 PFLOP/s of plane products.
 constexpr int A_UP = 11;  // bits of a half: x1 2^11 is as large as x0
 template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
 __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, int32_t tiles, int32_t nt) {
@@ -1148,8 +1148,8 @@ int launch_low_small(const LowSmall& a, hipStream_t s) {
 // make the 8 sum indices of a lane's operand: m = 4 q + e and 16 + 4 q + e, the same for both operands.
 // Rows of BN (BK) elements are cut into 32-byte units; unit u of row m lies at u ^ (m & 7): the 8 rows
 // that 32 lanes read together then cover all 64 banks.
-// Measured, M x K x N: bfloat16 8192 x 4096 x 4096 227 us = 1.21 PFLOP/s (the values' decoding 11 us besides), 220000 x 256 x
-// 256 81 us; float 220000 x 256 x 256 101 us = 0.86 PFLOP/s of plane products, both with the sums of the parts.
+// Measured, M x K x N: bfloat16 8192 x 4096 x 4096 239 us = 1.15 PFLOP/s with the values' decoding (11 us) and a call from Python,
+// 220000 x 256 x 256 67 us; float 220000 x 256 x 256 100 us = 0.86 PFLOP/s of plane products, both with the sums of the parts.
 __device__ __forceinline__ uint2 tr_read(uint32_t at) {
   typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)at));
