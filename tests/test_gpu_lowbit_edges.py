@@ -12,7 +12,7 @@ import torch
 import torch.utils.checkpoint
 
 from oracle import lowbit_oracle as LO
-from test_gpu_lowbit import BF16, F16, F32, TYPES, U, acts, check, gen, layer_run, lb, out_tol, sum_tol
+from test_gpu_lowbit import BF16, F16, F32, TYPES, U, acts, check, gen, layer_case, layer_run, lb, out_tol, sum_tol
 
 pytestmark = pytest.mark.gpu
 
@@ -327,3 +327,124 @@ def test_row_scales_are_those_of_the_devices_own_division(dtype):
     q = lb().quantize_rows(ends)
     assert torch.equal(q.scales, (ends.float().abs().amax(1) / 127).clamp_min(2.0 ** -126))
     assert torch.isfinite(q.dequantize()).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_offsets_past_32_bits(dtype):
+    """1,100,000 rows of 2,048 channels: the last rows' codes, products and gradients, and the sums over all."""
+    m, k, n, last = 1100000, 2048, 64, 1000
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(m, k, generator=g, device="cuda", dtype=dtype).requires_grad_()
+    w = (torch.randn(n, k, generator=g, device="cuda") / 45).to(dtype).requires_grad_()
+    b = torch.zeros(n, device="cuda", dtype=dtype, requires_grad=True)
+    dy = torch.randn(m, n, generator=g, device="cuda", dtype=dtype)
+    end = x.detach()[-last:]
+    with torch.no_grad():
+        q, part = lb().quantize_rows(x), lb().quantize_rows(end)
+        assert torch.equal(q.codes[-last:], part.codes) and torch.equal(q.scales[-last:], part.scales)
+        assert torch.equal(q.dequantize()[-last:], part.dequantize())
+        w8 = lb().quantize_rows(w)
+        assert torch.equal(lb().quantized_linear(x, w8)[-last:], lb().quantized_linear(end, w8))  # (exact sums)
+        del q
+        p, part = lb().pack_activations(x, relu=True), lb().pack_activations(end, relu=True)
+        assert torch.equal(p.codes[-last:], part.codes) and torch.equal(p.scales[-last:], part.scales)
+    y = lb().checkpointed_linear(x, w, b, relu=True)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    wd, ed = w.detach().double(), dy[-last:].double()
+    f = 6 if dtype == F32 else 1
+
+    def near(out, want, terms, count, planes):
+        tol = sum_tol(terms, count, planes)
+        step = torch.finfo(dtype).eps / 2
+        assert ((out.detach().double() - want).abs() <= tol + step * (want.abs() + tol)).all()
+
+    a = torch.relu(end).double()
+    wt = wd.t().contiguous()
+    near(y[-last:], a @ wt, a.abs() @ wt.abs(), k, f)
+    near(dx[-last:], (ed @ wd) * (end > 0), ed.abs() @ wd.abs(), n, f)
+    want, terms, sums, mags = torch.zeros_like(wd), torch.zeros_like(wd), torch.zeros(n, device="cuda", dtype=torch.float64), 0
+    for at in range(0, m, 100000):
+        v = lb().pack_activations(x.detach()[at:at + 100000], relu=True).dequantize().double()
+        d = dy[at:at + 100000].double().t().contiguous()
+        want, terms, sums, mags = want + d @ v, terms + d.abs() @ v, sums + d.sum(1), mags + d.abs().sum(1)
+    near(dw, want, terms, m, 3 if dtype == F32 else 1)
+    tol = (m / 8 + 300) * U * mags
+    assert ((db.detach().double() - sums).abs() <= tol + torch.finfo(dtype).eps / 2 * (sums.abs() + tol)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(3, 131072, 5), (3, 5, 131072), (140, 131072, 3)])
+def test_layers_of_the_most_channels(m, k, n, dtype):
+    layer_case(m, k, n, dtype, True, m + k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("stride", [1 << 22, (1 << 22) + 8])
+def test_rows_far_apart(dtype, stride):
+    """The longest row stride that is read in place, and one that is copied: rows of x and dy 2^22 elements apart."""
+    m, k, n = 260, 192, 64
+    x, w, dy = acts(m, k, dtype, 1).cuda(), acts(n, k, dtype, 2).cuda(), acts(m, n, dtype, 3).cuda()
+    want = layer_run(x, w, None, dy, True)
+    room = torch.empty(m * stride, device="cuda", dtype=dtype)
+    far = room.as_strided((m, k), (stride, 1))
+    fard = room.as_strided((m, n), (stride, 1), 1 << 20)
+    far.copy_(x)
+    fard.copy_(dy)
+    leaves = [far.requires_grad_(), w.clone().requires_grad_()]
+    y = lb().checkpointed_linear(*leaves, relu=True)
+    for a, b in zip((y, *torch.autograd.grad(y, leaves, fard)), want):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        w8 = lb().quantize_rows(w)
+        assert torch.equal(lb().quantized_linear(far, w8), lb().quantized_linear(x, w8))
+        assert torch.equal(lb().pack_activations(far).codes, lb().pack_activations(x).codes)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_empty_leading_dimensions_and_weights_of_other_types(dtype):
+    w = acts(12, 40, dtype, 1).cuda()
+    for shape in ((0, 5, 40), (2, 0, 40), (0, 40)):
+        x = torch.empty(shape, device="cuda", dtype=dtype, requires_grad=True)
+        wl = w.clone().requires_grad_()
+        y = lb().checkpointed_linear(x, wl, relu=True)
+        assert y.shape == (*shape[:-1], 12)
+        dx, dw = torch.autograd.grad(y, (x, wl), torch.empty_like(y))
+        assert dx.shape == x.shape and not dw.any()
+        with torch.no_grad():
+            assert lb().quantized_linear(x, lb().quantize_rows(w)).shape == y.shape
+            assert lb().quantize_rows(x).dequantize().shape == x.shape and lb().pack_activations(x).codes.shape == x.shape
+    x = acts(30, 40, F32, 2)
+    xq, xs = LO.row_codes(x)
+    wq, ws = LO.row_codes(w.cpu())
+    want = LO.quantized_linear(xq, xs, wq, ws)
+    check(lb().quantized_linear(x.cuda(), lb().quantize_rows(w)), want, 4 * U * want.abs())
+
+
+def test_graphs_that_share_a_pool_and_eager_calls_between():
+    """Two captured training steps of one memory pool, replayed in turn with eager steps between them."""
+    cases = []
+    pool = torch.cuda.graph_pool_handle()
+    for i, (m, k, n, dtype) in enumerate(((300, 256, 64, F32), (777, 100, 50, BF16))):
+        x, w, dy = acts(m, k, dtype, i).cuda(), acts(n, k, dtype, i + 5).cuda(), acts(m, n, dtype, i + 9).cuda()
+
+        def body(x, w=w, dy=dy):
+            leaves = [t.detach().requires_grad_() for t in (x, w)]
+            y = lb().checkpointed_linear(*leaves, relu=True)
+            return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            body(x)
+        torch.cuda.current_stream().wait_stream(side)
+        graph, held = torch.cuda.CUDAGraph(), x.clone()
+        with torch.cuda.graph(graph, pool=pool):
+            out = body(held)
+        cases.append((graph, held, x, body, out))
+    for r in range(3):
+        for graph, held, x, body, out in cases:
+            held.copy_(x.roll(r, 0))
+            graph.replay()
+            got = [t.clone() for t in out]  # (the other graph writes the shared pool)
+            for a, b in zip(got, body(x.roll(r, 0))):
+                assert torch.equal(a, b)
