@@ -646,7 +646,8 @@ int nc_quantized_linear(const nc_qlinear_args* args, void* workspace, size_t wor
  * NC_CODES_GROUP), all that the backward reads of x:
  *   dx = (dy W) [code != 0 if relu],  dw = dy^T value(codes),  db = sum_m dy.
  * NC_F32: y and dx from operands of 22 bits, with floors of 2^-47 of the largest in a row of x or dy and 2^-38 of the
- * largest in a row of w (dx: of w^T); infinities make NaN there.  dw: dy whole (an infinity makes NaN).
+ * largest in a row of w (dx: of w^T); infinities give what the formula does, but NaN with a factor
+ * below those digits or another infinity.  dw: dy whole.
  * codes may be NULL in a forward without a backward.  Every output of the backward may be NULL.
  * The workspace of either call is free again when the call's work on the stream has ended.  Its size is asked for with
  * the call's arguments: it goes by the addresses' alignment (16-bit types) and by the backward's outputs (dx, dw, db;

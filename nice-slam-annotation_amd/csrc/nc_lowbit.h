@@ -171,8 +171,7 @@ __device__ __forceinline__ uint16_t f32_elem(float x) {  // round to nearest eve
 __device__ __forceinline__ float relu_keep_nan(float x) { return x <= 0.f ? 0.f : x; }  // (of -0: +0)
 
 // x = x0 + x1 + x2, exactly, in bfloat16: each plane is what is left cut to its upper half (8 significant
-// bits, 24 in all; the third is whole by then).  Of 8 values: a plane is 4 words.  An infinity or NaN
-// leaves a NaN in the second plane.
+// bits, 24 in all; the third is whole by then).  Of 8 values: a plane is 4 words.  Behind an infinity the planes are 0.
 __device__ __forceinline__ uint32_t upper_halves(float lo, float hi) {
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
 }
@@ -180,21 +179,28 @@ __device__ __forceinline__ float cut_bf16(float x) {
   return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u);
 }
 __device__ __forceinline__ void split3(const float (&x)[8], uint4 (&plane)[3]) {
-  float r[8];
+  float r[8], top = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = x[e];
+  for (int e = 0; e < 8; ++e) {
+    r[e] = x[e];
+    top = __builtin_fmaxf(top, __builtin_fabsf(x[e]));
+  }
+  const bool infinite = __any(top == __builtin_inff());  // (a wave's own: seldom)
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
     plane[k] = uint4{upper_halves(r[0], r[1]), upper_halves(r[2], r[3]), upper_halves(r[4], r[5]), upper_halves(r[6], r[7])};
     if (k < 2)
 #pragma unroll
       for (int e = 0; e < 8; ++e) r[e] = r[e] - cut_bf16(r[e]);
+    if (k == 0 && infinite)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = __builtin_fabsf(x[e]) == __builtin_inff() ? 0.f : r[e];
   }
 }
 
 // x scale = x0 + x1 in half, |x scale| < 2^15: x0 the nearest, x1 what is left, rounded.  x1 is given times 2^UP: within
-// 2^-22 of |x|, or 2^-(25 + UP) / scale for small ones.  Of 8 values: a plane is 4 words.  An infinity leaves a NaN in
-// the second plane.  (Written as fused multiply-adds that end in half: one instruction an element and plane.)
+// 2^-22 of |x|, or 2^-(25 + UP) / scale for small ones.  Of 8 values: a plane is 4 words.  An infinity leaves an infinity and a
+// NaN, which split2_infinite replaces.  (Written as fused multiply-adds that end in half: one instruction an element and plane.)
 template <int UP>
 __device__ __forceinline__ void split2(const float (&x)[8], float scale, uint4 (&plane)[2]) {
   uint32_t w[2][4];
@@ -213,6 +219,21 @@ __device__ __forceinline__ void split2(const float (&x)[8], float scale, uint4 (
   }
 #pragma unroll
   for (int p = 0; p < 2; ++p) plane[p] = uint4{w[p][0], w[p][1], w[p][2], w[p][3]};
+}
+// the planes of infinities: 0 and the infinity, so that its products are what the formula's are (a wave takes this
+// branch where it holds one)
+__device__ __forceinline__ void split2_infinite(const float (&x)[8], uint4 (&plane)[2]) {
+  uint32_t h[4] = {plane[0].x, plane[0].y, plane[0].z, plane[0].w}, l[4] = {plane[1].x, plane[1].y, plane[1].z, plane[1].w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool inf = __builtin_fabsf(x[e]) == __builtin_inff();
+    const uint32_t keep = inf ? (e & 1 ? 0xffffu : 0xffff0000u) : ~0u;
+    const uint32_t v = inf ? (x[e] > 0.f ? 0x7c00u : 0xfc00u) << (e & 1 ? 16 : 0) : 0u;
+    h[e / 2] &= keep;
+    l[e / 2] = (l[e / 2] & keep) | v;
+  }
+  plane[0] = uint4{h[0], h[1], h[2], h[3]};
+  plane[1] = uint4{l[0], l[1], l[2], l[3]};
 }
 // biased exponent of the largest magnitude, for scales (times 2^UP) that are normal floats too: zero and what is below
 // 2^(UP - 112) count as 15 + UP, infinities as 254

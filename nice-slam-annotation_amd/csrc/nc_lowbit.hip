@@ -214,6 +214,7 @@ __global__ void __launch_bounds__(256) k_split(const SplitCtx a) {
     clear8<VEC>(c, a.cols, v);
     uint4 p[2];
     split2<0>(v, scale_to(141, e), p);
+    if (top >= 0x7f800000u) split2_infinite(v, p);
 #pragma unroll
     for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(a.dst + k * a.plane + r * a.dst_stride + 8 * c) = p[k];
   }
@@ -285,10 +286,12 @@ __global__ void __launch_bounds__(256) k_transpose(const TransposeCtx a) {
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = tile[cc][r8 + e];
-      const int e = top_exponent<0>(max(max(red[0][cc], red[1][cc]), max(red[2][cc], red[3][cc])));
+      const uint32_t top = max(max(red[0][cc], red[1][cc]), max(red[2][cc], red[3][cc]));
+      const int e = top_exponent<0>(top);
       if (r0 + r8 == 0) a.exponent[c0 + cc] = e;
       uint4 p[2];
       split2<0>(x, scale_to(141, e), p);
+      if (top >= 0x7f800000u) split2_infinite(x, p);
 #pragma unroll
       for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(d + k * a.plane) = p[k];
     } else {

@@ -420,9 +420,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm(const LowGemm g, int6
 // A layer's sums are short (8 slices for 256 inputs), so a workgroup goes through its tiles as one stream of
 // slices: the next tile's first slices are on their way while a tile ends, and its results leave from
 // registers and are not waited for.
+// An infinity of A or B has the planes 0 and infinity (split2_infinite): products with it alone.
 // RELU: of max(A, 0); MASK: the output is masked by codes and has no bias (each would take 16 registers).
-// Measured, M x K x N: 220000 x 256 x 256 147 us (450 MB: 91 us at a copy's rate; all workgroups store at once, and
-// loads behind stores wait for them), 4096 x 4096 x 4096 464 us = 0.89 PFLOP/s of plane products.
+// Measured, M x K x N: 220000 x 256 x 256 148 us (450 MB: 91 us at a copy's rate; all workgroups store at once, and
+// loads behind stores wait for them), 4096 x 4096 x 4096 464 - 473 us = 0.88 PFLOP/s of plane products.
 constexpr int A_UP = 11;  // bits of a half: x1 2^11 is as large as x0
 template <int BM, int BN, int WM, int WN, bool VEC, bool RELU, bool MASK>
 __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, int32_t tiles, int32_t nt) {
@@ -582,6 +583,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_low_gemm_f(const LowGemm g, in
       if (c == 0) exps[half * BM + r] = xe[l];
       uint4 p[2];
       split2<A_UP>(x, scale_to(138, xe[l]), p);
+      if (__any(bits == 0x7f800000u)) split2_infinite(x, p);
 #pragma unroll
       for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(s + k * APL + r * 64 + hchunk3(r, c)) = p[k];
     }

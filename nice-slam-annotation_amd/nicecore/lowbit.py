@@ -329,8 +329,9 @@ def checkpointed_linear(x, weight, bias=None, relu=False):
     float32 layer keep 22 bits of a value of x or dy down to 2^-25 of the largest in its row (a floor of 2^-47 of
     that) and of W down to 2^-17 of the largest in its row (of W^T for dx; 2^-38), and are as near to the exact result as a
     plain float32 product unless rows span more: an input of 1e8 beside ones of 1, with a weight of 1e-8, leaves
-    1.4e-5 (float32 3e-7).  An infinity in float32 x or dy makes NaN of its row of y or dx, one in W of its column, one in dy
-    of its output's row of dW.  A chain of such layers trains an MLP.  Has no second derivative.
+    1.4e-5 (float32 3e-7).  An infinity in float32 x, W or dy gives the infinities and NaNs of the formula, but NaN where its
+    factor is below the digits above (a weight under 2^-28, an x or dy under 2^-36 of the row's largest) or infinite too.
+    A chain of such layers trains an MLP.  Has no second derivative.
     The checkpoint is a saved tensor: a backward frees it, and saved-tensor hooks may move it."""
     if not torch.is_grad_enabled():  # no backward, no checkpoint (a Function sees the inputs' own requires_grad)
         x, weight, bias = (t.detach() if isinstance(t, torch.Tensor) else t for t in (x, weight, bias))

@@ -448,3 +448,43 @@ def test_graphs_that_share_a_pool_and_eager_calls_between():
             got = [t.clone() for t in out]  # (the other graph writes the shared pool)
             for a, b in zip(got, body(x.roll(r, 0))):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("m,k,n", [(5, 40, 30), (300, 93, 256), (2000, 256, 256), (140, 2100, 300), (4100, 1024, 1500)])
+def test_float32_infinities(m, k, n, relu):
+    """Infinities in x, W or dy of a float32 layer: infinite or NaN where the formula is, finite elsewhere."""
+    g = gen(m)
+    x, w = acts(m, k, F32, 1), torch.randn(n, k, generator=g)
+    dy = torch.randn(m, n, generator=g)
+    plain = (x.clone(), w.clone(), dy.clone())
+
+    def same(got, want, terms, count, planes):
+        got, fine = got.detach().double().cpu(), torch.isfinite(want)
+        assert torch.equal(torch.isfinite(got), fine) and torch.equal(got.isnan(), want.isnan())
+        over = ~fine & ~want.isnan()
+        assert torch.equal(got[over], want[over])
+        t = sum_tol(terms, count, planes)
+        check(got[fine], want[fine], (t + out_tol(want.abs() + t, F32))[fine])
+
+    for place in range(3):
+        x, w, dy = (t.clone() for t in plain)
+        t = (x, w, dy)[place]
+        t[1, 3], t[-1, -1], t[2, 5], t[2, 9] = math.inf, -math.inf, math.inf, -math.inf
+        if place == 0:
+            w[4, 3] = 0.0  # inf x 0
+        elif place == 1:
+            x[3, 3] = 0.0
+            dy[3, 1] = 0.0
+        else:
+            w[1, 7] = 0.0 if m > 5 else w[1, 7]
+        y, dx, dw = layer_run(x, w, None, dy, relu)
+        a = torch.relu(x.double()) if relu else x.double()
+        wd, d = w.double(), dy.double()
+        nz = lambda u: torch.nan_to_num(u.abs(), posinf=0.0)  # noqa: E731
+        same(y, a @ wd.t(), nz(a) @ nz(wd).t(), k, 6)
+        full = d @ wd
+        same(dx, torch.where(x > 0, full, torch.zeros_like(full)) if relu else full, nz(d) @ nz(wd), n, 6)
+        if place != 0:  # (x's infinities make NaN of their groups in the checkpoint)
+            v = LO.group_codes(x, relu)[2]
+            same(dw, d.t() @ v, nz(d).t() @ nz(v), m, 3)
